@@ -238,6 +238,72 @@ size_t qsp_attn_workspace_bytes(int32_t batch, int32_t tokens, int32_t n_heads,
 #define QSP_ATTN_STATIC_SCRATCH_BYTES ((size_t)16 << 20)
 int qsp_attn_verify_static(const qsp_attn_layer* layer, void* stream);
 
+/* ---------------------------------------------------------------- 8-bit KV cache */
+
+/*
+ * The paged cache with keys and values in 8 bits (e4m3) and one scale for each block of
+ * `scale_block` tokens of a page and kv head; it has no counterpart in the reference, whose cache
+ * holds the model dtype (kv.py:26-33). Half the bytes of a bf16 cache per token.
+ *
+ *   k_pages, v_pages    [num_pages, n_kv, page_size, head_dim] e4m3 codes, 16-byte aligned
+ *   k_scales, v_scales  [num_pages, n_kv, page_size / scale_block] fp32 powers of two
+ *   key of position p = k_pages[page, g, p % page_size, :] · k_scales[page, g, (p % page_size) / scale_block]
+ * with page = page_table[b, p / page_size]; likewise the values. Everything else is as in
+ * qsp_attn_layer: the qkv row layout, the T new tokens of sequence b at positions seq_lens[b] + t,
+ * positions outside the pages or the RoPE table flagged in *bad_index and left out.
+ *
+ * Limits: head_dim 32, 64, 128 or 256; scale_block a power of two up to 64 that divides
+ * page_size; q_buf 16-byte aligned. Only qsp_attn_kv8_prep writes the pages (a value code must
+ * not be NaN in a position that a query can see).
+ */
+typedef struct qsp_attn_kv8_layer {
+  int32_t batch, tokens;
+  int32_t n_heads, n_kv_heads, head_dim, rotary_dim;
+  int32_t page_size, max_pages, num_pages, scale_block;
+  int32_t rope_rows;
+  int32_t dtype;
+  float eps, scale;
+  const void* qkv;
+  int64_t ld_qkv;
+  const void* q_norm_w;   /* [hd] */
+  const void* k_norm_w;   /* [hd] */
+  const void* rope_cos;   /* [rope_rows, rotary_dim] dtype */
+  const void* rope_sin;
+  void* k_pages;
+  void* v_pages;
+  float* k_scales;
+  float* v_scales;
+  const int32_t* page_table;  /* [B, max_pages] */
+  const int32_t* seq_lens;    /* [B] committed tokens before this call */
+  void* q_buf;                /* [B*T, n_heads, hd] normed + rotated q */
+  void* out;                  /* [B*T, ld_out] gated attention output */
+  int64_t ld_out;
+  void* workspace;            /* qsp_attn_kv8_workspace_bytes(...) bytes, 16-byte aligned */
+  size_t workspace_bytes;
+  int32_t* bad_index;         /* optional [1] */
+} qsp_attn_kv8_layer;
+
+/* QK-norm + partial RoPE on q and k (blocks.py:218-227), q into q_buf, k and v quantised into the
+ * pages. The scale of a block is the least 2^e (e >= -40) with 448·2^e >= the largest magnitude
+ * among this call's tokens of the block, and at least the block's present scale if it holds
+ * earlier tokens; when it grows, the earlier codes are rescaled (exact, but for e4m3 subnormals).
+ * k is computed in 64 bits and rounded to fp32 before it is quantised, so the stored codes do not
+ * depend on the order of a sum. A token whose key or value has a non-finite element in a kv head
+ * is stored there as a NaN key and a zero value: every query that sees it gives NaN, no other.
+ * Repeating a call without moving seq_lens stores the same again. */
+int qsp_attn_kv8_prep(const qsp_attn_kv8_layer* layer, void* stream);
+
+/* Offset-causal GQA attention of the T new queries over the seq_lens[b]+T keys of the 8-bit
+ * pages, times σ(gate) (attention.py:43-51, 84-91; blocks.py:229-235), rounded to dtype once. The
+ * keys of all sequences are divided evenly over the SMs and the parts merged by a second launch,
+ * in a fixed order (repeated calls give the same bits). A query that sees no key gives zero.
+ * `workspace` must not be shared by two calls that overlap in time. */
+int qsp_attn_kv8_verify(const qsp_attn_kv8_layer* layer, void* stream);
+
+/* Bytes of workspace qsp_attn_kv8_verify needs on the current device (0 for invalid sizes). */
+size_t qsp_attn_kv8_workspace_bytes(int32_t batch, int32_t tokens, int32_t n_heads, int32_t n_kv_heads,
+                                    int32_t head_dim, int dtype);
+
 /* MTP attention with no cache over a single position: softmax over one key is 1, so the
  * output is the GQA-expanded v times σ(gate) (mtp.py:71-72 via blocks.py:226-235).
  * gate of head h at gate[r·ld_gate + h·gate_head_stride + d] (2·hd for the q_proj

@@ -53,6 +53,18 @@ class AttnLayer(C.Structure):
                 ("bad_index", vp)]
 
 
+class AttnKv8Layer(C.Structure):
+    """Mirror of `qsp_attn_kv8_layer`."""
+    _fields_ = [("batch", i32), ("tokens", i32), ("n_heads", i32), ("n_kv_heads", i32),
+                ("head_dim", i32), ("rotary_dim", i32), ("page_size", i32), ("max_pages", i32),
+                ("num_pages", i32), ("scale_block", i32), ("rope_rows", i32), ("dtype", i32),
+                ("eps", f32), ("scale", f32), ("qkv", vp), ("ld_qkv", i64), ("q_norm_w", vp),
+                ("k_norm_w", vp), ("rope_cos", vp), ("rope_sin", vp), ("k_pages", vp), ("v_pages", vp),
+                ("k_scales", vp), ("v_scales", vp), ("page_table", vp), ("seq_lens", vp), ("q_buf", vp),
+                ("out", vp), ("ld_out", i64), ("workspace", vp), ("workspace_bytes", sz),
+                ("bad_index", vp)]
+
+
 class MoeLayer(C.Structure):
     """Mirror of `qsp_moe_layer`."""
     _fields_ = [("tokens", i32), ("hidden", i32), ("n_experts", i32), ("top_k", i32), ("inter", i32),
@@ -83,6 +95,9 @@ SIGNATURES = {
     "qsp_attn_verify": (C.c_int, [C.POINTER(AttnLayer), vp]),
     "qsp_attn_workspace_bytes": (sz, [i32, i32, i32, i32, i32]),
     "qsp_attn_verify_static": (C.c_int, [C.POINTER(AttnLayer), vp]),
+    "qsp_attn_kv8_prep": (C.c_int, [C.POINTER(AttnKv8Layer), vp]),
+    "qsp_attn_kv8_verify": (C.c_int, [C.POINTER(AttnKv8Layer), vp]),
+    "qsp_attn_kv8_workspace_bytes": (sz, [i32, i32, i32, i32, i32, C.c_int]),
     "qsp_mtp_single_token_attn": (C.c_int, [vp, i64, i64, vp, i64, vp, i64, i64, i32, i32, i32,
                                             C.c_int, vp]),
     "qsp_select_rows": (C.c_int, [vp, i64, i32, i32, vp, vp, i64, i64, C.c_int, vp]),

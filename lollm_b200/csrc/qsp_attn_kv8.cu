@@ -1,0 +1,531 @@
+// The 8-bit KV cache: prep (QK-norm, partial RoPE, quantisation into the pages), the attention
+// on CUDA cores (fp32 models, and shapes outside the tensor-core kernel's), the merge of divided
+// units, and the C entry points.
+#include "qsp_attn_kv8.cuh"
+#include "qsp_tc.cuh"
+
+#include <algorithm>
+
+namespace qsp {
+namespace kv8 {
+
+// ------------------------------------------------------------------ prep
+// Two kinds of CTA (128 threads) in one launch. The first n_kv_jobs quantise: one (sequence, touched
+// block of tokens, kv head, K or V) each, so that the block's largest magnitude is reduced and its
+// scale and earlier codes are rewritten by one CTA, without atomics. The others norm and rotate q,
+// a warp per (token row, head). A few µs of latency bound the small calls; the chunk of a prompt is
+// bound by its bytes, 9/10 of them q in and out.
+//
+// k is normed and rotated in fp64: with 3 mantissa bits a value next to a rounding border would
+// otherwise fall to either side with the order of the sum, and a cached code lives as long as its
+// sequence. There are 1/8 as many k as q heads, and B200 runs fp64 at half the fp32 rate.
+constexpr int PREP_THREADS = 128;
+
+template <typename T, int EPL>
+__device__ __forceinline__ void load_row(const T* p, int lane, bool vec, float (&x)[EPL]) {
+  if constexpr (EPL * sizeof(T) >= 4) {
+    if (vec) {
+      constexpr int BYTES = EPL * sizeof(T), W = BYTES > 16 ? 16 : BYTES, N = BYTES / W, PER = W / (int)sizeof(T);
+      const char* src = reinterpret_cast<const char*>(p) + (size_t)lane * BYTES;
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        alignas(16) T t[PER];
+        if constexpr (W == 16) *reinterpret_cast<uint4*>(t) = *reinterpret_cast<const uint4*>(src + n * W);
+        else if constexpr (W == 8) *reinterpret_cast<uint2*>(t) = *reinterpret_cast<const uint2*>(src + n * W);
+        else *reinterpret_cast<uint32_t*>(t) = *reinterpret_cast<const uint32_t*>(src + n * W);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) x[n * PER + i] = dt<T>::to_f(t[i]);
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) x[i] = dt<T>::to_f(p[lane * EPL + i]);
+}
+
+// EPL codes of a lane, EPL bytes at dst + lane·EPL
+template <int EPL>
+__device__ __forceinline__ void store_codes(uint8_t* dst, int lane, const float (&x)[EPL], float inv) {
+  if constexpr (EPL == 1) {
+    dst[lane] = (uint8_t)to_e4m3x2(x[0] * inv, 0.f);
+  } else {
+    alignas(8) uint16_t c[EPL / 2];
+#pragma unroll
+    for (int i = 0; i < EPL / 2; ++i) c[i] = to_e4m3x2(x[2 * i] * inv, x[2 * i + 1] * inv);
+    if constexpr (EPL == 2) reinterpret_cast<uint16_t*>(dst)[lane] = c[0];
+    else if constexpr (EPL == 4) reinterpret_cast<uint32_t*>(dst)[lane] = *reinterpret_cast<uint32_t*>(c);
+    else reinterpret_cast<uint2*>(dst)[lane] = *reinterpret_cast<uint2*>(c);
+  }
+}
+
+// one head's row in F (float for q, double for k): norm, times 1 + w, rotate the first rd dims
+template <typename T, int HD, typename F>
+__device__ __forceinline__ void norm_rotate(const qsp_attn_kv8_layer& L, const float (&x)[HD / 32], const T* w, int pos, int lane,
+                                            F* xs, F (&y)[HD / 32]) {
+  constexpr int EPL = HD / 32;
+  F ss = 0;
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) ss += (F)x[i] * (F)x[i];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  const F inv = rsqrt(ss / (F)HD + (F)L.eps);
+  const int rd = L.rotary_dim, half = rd / 2;
+  __syncwarp();   // the warp's previous row has been read
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) {
+    const int d = lane * EPL + i;
+    y[i] = (F)x[i] * inv * ((F)dt<T>::to_f(w[d]) + (F)1);
+    if (d < rd) xs[d] = y[i];
+  }
+  __syncwarp();
+  if (lane * EPL < rd) {
+    const T* cosr = static_cast<const T*>(L.rope_cos) + (int64_t)pos * rd;
+    const T* sinr = static_cast<const T*>(L.rope_sin) + (int64_t)pos * rd;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+      const int d = lane * EPL + i;
+      if (d < rd) {
+        const F r = d < half ? -xs[d + half] : xs[d - half];
+        y[i] = y[i] * (F)dt<T>::to_f(cosr[d]) + r * (F)dt<T>::to_f(sinr[d]);
+      }
+    }
+  }
+}
+
+template <int EPL>
+__device__ __forceinline__ bool warp_finite(const float (&x)[EPL]) {
+  bool ok = true;
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) ok = ok && isfinite(x[i]);
+  return __all_sync(0xffffffffu, ok);
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(PREP_THREADS) prep_kernel(const qsp_attn_kv8_layer L, int n_kv_jobs, int most, bool vec) {
+  pdl_trigger();
+  pdl_wait();
+  constexpr int EPL = HD / 32;
+  __shared__ double xs[4][HD];
+  __shared__ float red[4];
+  extern __shared__ float vals[];   // [scale_block][HD] of a quantising CTA
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int nh = L.n_heads, nkv = L.n_kv_heads;
+  const T* qkv = static_cast<const T*>(L.qkv);
+
+  if ((int)blockIdx.x >= n_kv_jobs) {
+    const int64_t idx = ((int64_t)blockIdx.x - n_kv_jobs) * 4 + warp;
+    if (idx >= (int64_t)L.batch * L.tokens * nh) return;
+    const int64_t m = idx / nh;
+    const int h = (int)(idx - m * nh);
+    const long long pos = (long long)L.seq_lens[m / L.tokens] + m % L.tokens;
+    float x[EPL], y[EPL];
+    load_row<T, EPL>(qkv + m * L.ld_qkv + (int64_t)h * 2 * HD, lane, vec, x);
+    // a position outside the table is flagged by the quantising CTAs; its q is rotated as position 0
+    norm_rotate<T, HD, float>(L, x, static_cast<const T*>(L.q_norm_w), pos >= 0 && pos < L.rope_rows ? (int)pos : 0, lane,
+                              reinterpret_cast<float*>(xs[warp]), y);
+    alignas(16) T o[EPL];
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) o[i] = dt<T>::from_f(y[i]);
+    T* dst = static_cast<T*>(L.q_buf) + (m * nh + h) * HD + lane * EPL;
+    constexpr int BYTES = EPL * sizeof(T);
+    if constexpr (BYTES >= 16) {
+#pragma unroll
+      for (int n = 0; n < BYTES / 16; ++n) reinterpret_cast<uint4*>(dst)[n] = reinterpret_cast<uint4*>(o)[n];
+    } else if constexpr (BYTES == 8) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(o);
+    else if constexpr (BYTES == 4) *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<uint32_t*>(o);
+    else *dst = o[0];
+    return;
+  }
+
+  // ---- quantise one block of one head
+  int job = blockIdx.x;
+  const bool is_v = job & 1;
+  job >>= 1;
+  const int g = job % nkv;
+  job /= nkv;
+  const int b = job / most, sb = L.scale_block;
+  const long long base = L.seq_lens[b];
+  const long long p0 = max(base, 0ll);                   // a negative length: positions below 0 are left out
+  const long long blk = p0 / sb + job % most;
+  const long long lo = max(p0, blk * sb);
+  long long hi = min(base + L.tokens, (blk + 1) * sb);
+  const bool any = lo < hi;
+  const long long lp = lo / L.page_size;
+  int page = -1;
+  if (any && lo < L.rope_rows && lp < L.max_pages) page = L.page_table[(int64_t)b * L.max_pages + lp];
+  const bool ok = page >= 0 && page < L.num_pages;
+  if (threadIdx.x == 0 && L.bad_index != nullptr && (base < 0 || (any && (!ok || hi > L.rope_rows)))) *L.bad_index = 1;
+  if (!ok) return;
+  hi = min(hi, (long long)L.rope_rows);
+  const int n_new = (int)(hi - lo), n_old = (int)(lo - blk * sb);
+  const int slot0 = (int)(blk * sb % L.page_size);
+  uint8_t* codes = static_cast<uint8_t*>(is_v ? L.v_pages : L.k_pages) + (((int64_t)page * nkv + g) * L.page_size + slot0) * HD;
+  float* scale = (is_v ? L.v_scales : L.k_scales) + ((int64_t)page * nkv + g) * (L.page_size / sb) + slot0 / sb;
+  const int e_old = n_old > 0 ? exp_of(*scale) : -128;
+
+  float amax = 0.f;
+  for (int j = warp; j < n_new; j += 4) {
+    const int pos = (int)lo + j;
+    const T* row = qkv + ((int64_t)b * L.tokens + (pos - base)) * L.ld_qkv + (int64_t)nh * 2 * HD + (int64_t)g * HD;
+    float v[EPL];
+    load_row<T, EPL>(row + (int64_t)nkv * HD, lane, vec, v);
+    bool fine = warp_finite(v);
+    float y[EPL];
+    if (is_v) {
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) y[i] = fine ? v[i] : 0.f;
+    } else {
+      float x[EPL];
+      double z[EPL];
+      load_row<T, EPL>(row, lane, vec, x);
+      norm_rotate<T, HD, double>(L, x, static_cast<const T*>(L.k_norm_w), pos, lane, xs[warp], z);
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) y[i] = (float)z[i];
+      fine = warp_finite(y) && fine;
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) y[i] = fine ? y[i] : NAN;
+    }
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+      vals[j * HD + lane * EPL + i] = y[i];
+      amax = fmaxf(amax, fabsf(y[i]));   // NaN is passed over
+    }
+  }
+  amax = warp_max(amax);
+  if (lane == 0) red[warp] = amax;
+  __syncthreads();
+  amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const int e = min(max(scale_exp(amax), e_old), MAX_EXP);
+  if (threadIdx.x == 0) *scale = exp2i(e);
+  if (e_old < e && n_old > 0) {   // earlier tokens of the block take the larger scale
+    const float f = ldexpf(1.f, e_old - e);
+    uint32_t* c4 = reinterpret_cast<uint32_t*>(codes);
+    for (int k = threadIdx.x; k < n_old * (HD / 4); k += PREP_THREADS) {
+      const uint32_t c = c4[k];
+      const float2 a = from_e4m3x2((uint16_t)c), z = from_e4m3x2((uint16_t)(c >> 16));
+      c4[k] = (uint32_t)to_e4m3x2(a.x * f, a.y * f) | (uint32_t)to_e4m3x2(z.x * f, z.y * f) << 16;
+    }
+  }
+  const float inv = exp2i(-e);
+  for (int j = warp; j < n_new; j += 4) {   // a warp's own rows of vals
+    float y[EPL];
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) y[i] = vals[j * HD + lane * EPL + i];
+    store_codes<EPL>(codes + (int64_t)(n_old + j) * HD, lane, y, inv);
+  }
+}
+
+template <typename T, int HD>
+static int launch_prep(const qsp_attn_kv8_layer& L, cudaStream_t st) {
+  const int sb = L.scale_block;
+  const int64_t most = (L.tokens + sb - 2) / sb + 1;    // blocks that T tokens can touch
+  const int64_t jobs = 2 * most * L.n_kv_heads * L.batch;
+  const int64_t rows = ((int64_t)L.batch * L.tokens * L.n_heads + 3) / 4;
+  QSP_REQUIRE(jobs + rows < (1ll << 31), "qsp_attn_kv8_prep: too many tokens for one call");
+  constexpr int A = std::min<int>(16, HD / 32 * sizeof(T));
+  const bool vec = aligned(L.qkv, A) && (L.ld_qkv * (int64_t)sizeof(T)) % A == 0;
+  const size_t smem = (size_t)sb * HD * sizeof(float);
+  auto kern = prep_kernel<T, HD>;
+  if (smem > 32 * 1024) {   // with the static arrays past the 48 KB that need no leave
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return set_error(QSP_ERR_CUDA, "qsp_attn_kv8_prep: %s", cudaGetErrorString(e));
+  }
+  return launch_pdl("qsp_attn_kv8_prep", kern, dim3((unsigned)(jobs + rows)), dim3(PREP_THREADS), smem, st, L, (int)jobs,
+                    (int)most, vec);
+}
+
+// ------------------------------------------------------------------ attention on CUDA cores
+// fp32 throughout: for fp32 models, and for bf16 shapes that the tensor-core kernel does not take.
+// A CTA of 4 warps runs its pieces (see Piece) with 16 query rows, 4 a warp; keys are staged 32 at a
+// time as fp32 values, lane j scores key j. Bound by its shared-memory reads (two per product).
+constexpr int SIMT_R = 16, SIMT_KT = 32, SIMT_THREADS = 128;
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(SIMT_THREADS) simt_kernel(const qsp_attn_kv8_layer L, int n_rg) {
+  pdl_trigger();
+  pdl_wait();
+  constexpr int DPL = HD / 32, RPW = SIMT_R / 4;
+  extern __shared__ float smem[];
+  __shared__ long long sh[34];
+  float* Qs = smem;                       // [16][HD]
+  float* Ks = Qs + SIMT_R * HD;           // [32][HD + 1]
+  float* Vs = Ks + SIMT_KT * (HD + 1);    // [32][HD]
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int nrep = L.n_heads / L.n_kv_heads, rows_total = nrep * L.tokens;
+  const T* qb = static_cast<const T*>(L.q_buf);
+  const uint8_t* kp = static_cast<const uint8_t*>(L.k_pages);
+  const uint8_t* vp = static_cast<const uint8_t*>(L.v_pages);
+  const Scratch ws = scratch(L, gridDim.x, SIMT_R);
+  const float sl2 = L.scale * LOG2E;
+
+  Walk w = share(L, n_rg, SIMT_R, sh);
+  Piece p;
+  p.n = 0;
+  while (next_piece(L, n_rg, SIMT_R, w, p)) {
+    const int row0 = p.rg * SIMT_R, nrows = min(SIMT_R, rows_total - row0);
+    const long long base = L.seq_lens[p.b];
+    const long long kv_end = min(base + L.tokens, (long long)L.max_pages * L.page_size);
+    __syncthreads();   // the previous piece's q has been read
+    for (int e = tid; e < nrows * HD; e += SIMT_THREADS) {
+      const int r = e / HD, d = e % HD, t = (row0 + r) / nrep, hq = p.g * nrep + (row0 + r) % nrep;
+      Qs[r * HD + d] = dt<T>::to_f(qb[(((int64_t)p.b * L.tokens + t) * L.n_heads + hq) * HD + d]);
+    }
+    float acc[RPW][DPL], mrow[RPW], lrow[RPW];
+#pragma unroll
+    for (int i = 0; i < RPW; ++i) {
+      mrow[i] = -INFINITY;
+      lrow[i] = 0.f;
+#pragma unroll
+      for (int j = 0; j < DPL; ++j) acc[i][j] = 0.f;
+    }
+    const long long k_begin = (long long)p.j0 * TILE, k_end = min(kv_end, k_begin + (long long)p.n * TILE);
+    for (long long k0 = k_begin; k0 < k_end; k0 += SIMT_KT) {
+      __syncthreads();
+      bool mapped = false;   // key `lane` of this step has a page
+      for (int e = tid; e < SIMT_KT * HD / 4; e += SIMT_THREADS) {
+        const int j = e / (HD / 4), d = e % (HD / 4) * 4;
+        const long long pos = k0 + j;
+        float2 k01 = {0, 0}, k23 = {0, 0}, v01 = {0, 0}, v23 = {0, 0};
+        float ks = 0.f, vs = 0.f;
+        if (pos < k_end) {
+          const int page = L.page_table[(int64_t)p.b * L.max_pages + pos / L.page_size];
+          if (page >= 0 && page < L.num_pages) {
+            const int slot = (int)(pos % L.page_size);
+            const int64_t ph = (int64_t)page * L.n_kv_heads + p.g;
+            const int64_t off = (ph * L.page_size + slot) * HD + d;
+            const uint32_t kc = *reinterpret_cast<const uint32_t*>(kp + off), vc = *reinterpret_cast<const uint32_t*>(vp + off);
+            const int64_t so = ph * (L.page_size / L.scale_block) + slot / L.scale_block;
+            ks = L.k_scales[so];
+            vs = L.v_scales[so];
+            k01 = from_e4m3x2((uint16_t)kc), k23 = from_e4m3x2((uint16_t)(kc >> 16));
+            v01 = from_e4m3x2((uint16_t)vc), v23 = from_e4m3x2((uint16_t)(vc >> 16));
+          }
+        }
+        float* k = Ks + j * (HD + 1) + d;
+        k[0] = k01.x * ks, k[1] = k01.y * ks, k[2] = k23.x * ks, k[3] = k23.y * ks;
+        float* v = Vs + j * HD + d;
+        v[0] = v01.x * vs, v[1] = v01.y * vs, v[2] = v23.x * vs, v[3] = v23.y * vs;
+      }
+      const long long kpos = k0 + lane;
+      if (kpos < k_end) {
+        const int page = L.page_table[(int64_t)p.b * L.max_pages + kpos / L.page_size];
+        mapped = page >= 0 && page < L.num_pages;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < RPW; ++i) {
+        const int r = warp + 4 * i;
+        if (r >= nrows) break;
+        const float* q = Qs + r * HD;
+        const float* kr = Ks + lane * (HD + 1);
+        float sc = 0.f;
+#pragma unroll 8
+        for (int d = 0; d < HD; ++d) sc = fmaf(q[d], kr[d], sc);
+        const bool vis = mapped && kpos <= base + (row0 + r) / nrep;
+        sc = vis ? sc * sl2 : -INFINITY;
+        const float mnew = fmaxf(mrow[i], warp_max(sc));
+        const float mref = mnew == -INFINITY ? 0.f : mnew;   // nothing to see yet (a NaN score stays NaN below)
+        const float alpha = exp2f(mrow[i] - mref);
+        const float pr = vis ? exp2f(sc - mref) : 0.f;
+        lrow[i] = lrow[i] * alpha + warp_sum(pr);
+        mrow[i] = mnew;
+#pragma unroll
+        for (int j = 0; j < DPL; ++j) acc[i][j] *= alpha;
+        for (int jj = 0; jj < SIMT_KT; ++jj) {
+          const float pj = __shfl_sync(0xffffffffu, pr, jj);
+          if (pj != 0.f) {
+#pragma unroll
+            for (int j = 0; j < DPL; ++j) acc[i][j] = fmaf(pj, Vs[jj * HD + lane + 32 * j], acc[i][j]);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < RPW; ++i) {
+      const int r = warp + 4 * i;
+      if (r >= nrows) break;
+      if (p.whole()) {
+        const int t = (row0 + r) / nrep, hq = p.g * nrep + (row0 + r) % nrep;
+        const int64_t m = (int64_t)p.b * L.tokens + t;
+        const T* gate = static_cast<const T*>(L.qkv) + m * L.ld_qkv + (int64_t)hq * 2 * HD + HD;
+        T* o = static_cast<T*>(L.out) + m * L.ld_out + (int64_t)hq * HD;
+#pragma unroll
+        for (int j = 0; j < DPL; ++j) {
+          const int d = lane + 32 * j;
+          const float v = lrow[i] == 0.f ? 0.f : acc[i][j] / lrow[i];
+          o[d] = dt<T>::from_f(v * sigmoidf_(dt<T>::to_f(gate[d])));
+        }
+      } else {
+        const int64_t at = (int64_t)p.slot() * SIMT_R + r;
+#pragma unroll
+        for (int j = 0; j < DPL; ++j) ws.o[at * HD + lane + 32 * j] = acc[i][j];
+        if (lane == 0) ws.ml[at] = make_float2(mrow[i], lrow[i]);
+      }
+    }
+  }
+  if (tid == 0) put_meta(ws, w, p);
+}
+
+template <typename T, int HD>
+static int launch_simt(const qsp_attn_kv8_layer& L, int G, cudaStream_t st) {
+  const int rows = L.n_heads / L.n_kv_heads * L.tokens, n_rg = (rows + SIMT_R - 1) / SIMT_R;
+  const size_t smem = (size_t)(SIMT_R * HD + SIMT_KT * (HD + 1) + SIMT_KT * HD) * sizeof(float);
+  auto kern = simt_kernel<T, HD>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return set_error(QSP_ERR_CUDA, "qsp_attn_kv8_verify: %s", cudaGetErrorString(e));
+  const int rc = launch_pdl("qsp_attn_kv8_verify(simt)", kern, dim3(G), dim3(SIMT_THREADS), smem, st, L, n_rg);
+  return rc ? rc : launch_merge(L, G, SIMT_R, st);
+}
+
+// ------------------------------------------------------------------ merge of divided units
+// CTA (c, r): row r of the divided unit that begins in the share of attention CTA c, if one does.
+// Its partials are weighted with 2^(m_p − M), summed in their order (groups of hd/4 threads take every
+// 256/(hd/4)-th partial, the groups' sums are then added in order), divided by l and gated.
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) merge_kernel(const qsp_attn_kv8_layer L, int G, int R) {
+  pdl_trigger();
+  pdl_wait();
+  constexpr int TPP = HD / 4, NG = 256 / TPP;
+  __shared__ float4 part[256];
+  __shared__ float lpart[NG];
+  const Scratch ws = scratch(L, G, R);
+  const int4 meta = ws.meta[blockIdx.x];
+  const int np = meta.w, r = blockIdx.y;
+  if (np == 0) return;
+  const int nrep = L.n_heads / L.n_kv_heads, rr = meta.y * R + r;
+  if (rr >= nrep * L.tokens) return;
+  const int c = blockIdx.x, lane = threadIdx.x & 31;
+  const int first = 2 * c + (meta.z >> 30);
+  auto slot = [&](int q) { return (int64_t)(q == 0 ? first : 2 * (c + q)) * R + r; };
+  float M = -INFINITY;
+  for (int q = lane; q < np; q += 32) M = fmaxf(M, ws.ml[slot(q)].x);
+  M = warp_max(M);
+  const float ref = M == -INFINITY ? 0.f : M;
+  const int grp = threadIdx.x / TPP, col = threadIdx.x % TPP;
+  float4 acc = {0, 0, 0, 0};
+  float den = 0.f;
+#pragma unroll 4
+  for (int q = grp; q < np; q += NG) {
+    const float2 ml = ws.ml[slot(q)];
+    const float4 v = *reinterpret_cast<const float4*>(ws.o + slot(q) * HD + 4 * col);
+    const float f = exp2f(ml.x - ref);
+    if (ml.y != 0.f) {   // a part of which the row saw nothing
+      den = fmaf(f, ml.y, den);
+      acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
+    }
+  }
+  part[threadIdx.x] = acc;
+  if (col == 0) lpart[grp] = den;
+  __syncthreads();
+  if (threadIdx.x < HD) {
+    const int d = threadIdx.x, t = rr / nrep, hq = (meta.z & ((1 << 30) - 1)) * nrep + rr % nrep;
+    float s = 0.f, l = 0.f;
+#pragma unroll
+    for (int q = 0; q < NG; ++q) {
+      s += reinterpret_cast<const float*>(part)[q * HD + d];
+      l += lpart[q];
+    }
+    const int64_t m = (int64_t)meta.x * L.tokens + t;
+    const T* gate = static_cast<const T*>(L.qkv) + m * L.ld_qkv + (int64_t)hq * 2 * HD + HD;
+    const float v = l == 0.f ? 0.f : s / l;
+    static_cast<T*>(L.out)[m * L.ld_out + (int64_t)hq * HD + d] = dt<T>::from_f(v * sigmoidf_(dt<T>::to_f(gate[d])));
+  }
+}
+
+template <typename T>
+static int launch_merge_t(const qsp_attn_kv8_layer& L, int G, int R, cudaStream_t st) {
+  const int rows = std::min(R, L.n_heads / L.n_kv_heads * L.tokens);
+  const dim3 grid(G, rows), block(256);
+  switch (L.head_dim) {
+    case 32: return launch_pdl("qsp_attn_kv8_verify(merge)", merge_kernel<T, 32>, grid, block, 0, st, L, G, R);
+    case 64: return launch_pdl("qsp_attn_kv8_verify(merge)", merge_kernel<T, 64>, grid, block, 0, st, L, G, R);
+    case 128: return launch_pdl("qsp_attn_kv8_verify(merge)", merge_kernel<T, 128>, grid, block, 0, st, L, G, R);
+    default: return launch_pdl("qsp_attn_kv8_verify(merge)", merge_kernel<T, 256>, grid, block, 0, st, L, G, R);
+  }
+}
+
+int launch_merge(const qsp_attn_kv8_layer& L, int G, int R, cudaStream_t st) {
+  if ((int64_t)L.max_pages * L.page_size <= TILE) return QSP_OK;   // one tile a unit: none is divided
+  QSP_DISPATCH_DTYPE(L.dtype, T, { return launch_merge_t<T>(L, G, R, st); });
+}
+
+// CTAs of the CUDA-core kernel: three fit an SM at head_dim 256 (82 KB of shared memory each is the
+// limit at two); two keep its loads and products overlapped
+static int simt_grid() { return 2 * tc::sm_count(); }
+
+static int validate(const char* what, const qsp_attn_kv8_layer* p, bool verify) {
+  QSP_REQUIRE(p != nullptr, "%s: null layer", what);
+  const qsp_attn_kv8_layer& L = *p;
+  QSP_REQUIRE(L.qkv && L.k_pages && L.v_pages && L.k_scales && L.v_scales && L.page_table && L.seq_lens && L.q_buf,
+              "%s: null pointer", what);
+  QSP_REQUIRE(L.batch > 0 && L.tokens > 0 && (int64_t)L.batch * L.tokens < (1 << 30), "%s: bad batch/tokens", what);
+  QSP_REQUIRE(L.n_heads > 0 && L.n_kv_heads > 0 && L.n_heads % L.n_kv_heads == 0 && L.n_heads <= (1 << 16),
+              "%s: n_heads must be a multiple of n_kv_heads", what);
+  QSP_REQUIRE(L.head_dim == 32 || L.head_dim == 64 || L.head_dim == 128 || L.head_dim == 256, "%s: head_dim %d not built", what,
+              L.head_dim);
+  QSP_REQUIRE(L.page_size > 0 && L.max_pages > 0 && L.num_pages > 0 && (int64_t)L.max_pages * L.page_size < (1ll << 31),
+              "%s: bad paging", what);
+  QSP_REQUIRE(L.scale_block > 0 && L.scale_block <= 64 && (L.scale_block & (L.scale_block - 1)) == 0 &&
+                  L.page_size % L.scale_block == 0,
+              "%s: scale_block %d must be a power of two up to 64 that divides the page size %d", what, L.scale_block, L.page_size);
+  QSP_REQUIRE(aligned(L.k_pages, 16) && aligned(L.v_pages, 16) && aligned(L.q_buf, 16), "%s: pages and q_buf must be 16-byte aligned",
+              what);
+  QSP_REQUIRE(L.ld_qkv >= (2ll * L.n_heads + 2ll * L.n_kv_heads) * L.head_dim, "%s: ld_qkv too small", what);
+  QSP_REQUIRE(L.dtype == QSP_F32 || L.dtype == QSP_BF16, "%s: unsupported dtype %d", what, L.dtype);
+  if (!verify) {
+    QSP_REQUIRE(L.q_norm_w && L.k_norm_w && (L.rotary_dim == 0 || (L.rope_cos && L.rope_sin)) && L.rope_rows > 0,
+                "%s: null pointer or empty RoPE table", what);
+    QSP_REQUIRE(L.rotary_dim >= 0 && L.rotary_dim <= L.head_dim && L.rotary_dim % 2 == 0, "%s: bad rotary_dim", what);
+    return QSP_OK;
+  }
+  const size_t need = qsp_attn_kv8_workspace_bytes(L.batch, L.tokens, L.n_heads, L.n_kv_heads, L.head_dim, L.dtype);
+  QSP_REQUIRE(L.out && L.ld_out >= (int64_t)L.n_heads * L.head_dim, "%s: missing output or ld_out too small", what);
+  QSP_REQUIRE(L.workspace && aligned(L.workspace, 16) && L.workspace_bytes >= need,
+              "%s: workspace of %zu bytes (16-byte aligned) needed, %zu given", what, need, L.workspace ? L.workspace_bytes : 0);
+  return QSP_OK;
+}
+
+}  // namespace kv8
+}  // namespace qsp
+
+using namespace qsp;
+
+extern "C" {
+
+int qsp_attn_kv8_prep(const qsp_attn_kv8_layer* layer, void* stream) {
+  const int rc = kv8::validate("qsp_attn_kv8_prep", layer, false);
+  if (rc) return rc;
+  const cudaStream_t st = as_stream(stream);
+  QSP_DISPATCH_DTYPE(layer->dtype, T, {
+    switch (layer->head_dim) {
+      case 32: return kv8::launch_prep<T, 32>(*layer, st);
+      case 64: return kv8::launch_prep<T, 64>(*layer, st);
+      case 128: return kv8::launch_prep<T, 128>(*layer, st);
+      default: return kv8::launch_prep<T, 256>(*layer, st);
+    }
+  });
+}
+
+int qsp_attn_kv8_verify(const qsp_attn_kv8_layer* layer, void* stream) {
+  const int rc = kv8::validate("qsp_attn_kv8_verify", layer, true);
+  if (rc) return rc;
+  const cudaStream_t st = as_stream(stream);
+  const int G = kv8::simt_grid();
+  QSP_DISPATCH_DTYPE(layer->dtype, T, {
+    switch (layer->head_dim) {
+      case 32: return kv8::launch_simt<T, 32>(*layer, G, st);
+      case 64: return kv8::launch_simt<T, 64>(*layer, G, st);
+      case 128: return kv8::launch_simt<T, 128>(*layer, G, st);
+      default: return kv8::launch_simt<T, 256>(*layer, G, st);
+    }
+  });
+}
+
+size_t qsp_attn_kv8_workspace_bytes(int32_t batch, int32_t tokens, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int dtype) {
+  if (batch <= 0 || tokens <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads != 0 || head_dim <= 0 ||
+      (dtype != QSP_F32 && dtype != QSP_BF16))
+    return 0;
+  return kv8::scratch_bytes(kv8::simt_grid(), kv8::SIMT_R, head_dim);
+}
+
+}  // extern "C"

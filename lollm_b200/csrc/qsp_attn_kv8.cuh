@@ -1,0 +1,173 @@
+// Shared by the kernels of the 8-bit KV cache: e4m3 conversions, power-of-two scales, and the
+// division of the attention's work over the CTAs.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "qsp_common.cuh"
+
+namespace qsp {
+namespace kv8 {
+
+constexpr int TILE = 128;      // keys of a work tile
+constexpr int MIN_EXP = -40;   // least exponent of a scale
+constexpr int MAX_EXP = 120;   // 448·2^120 holds every fp32 value
+constexpr float LOG2E = 1.4426950408889634f;
+
+// ---------------------------------------------------------------- e4m3
+// two fp32 -> two codes (round to nearest even, saturating; NaN -> 0x7f), lo in the low byte
+__device__ __forceinline__ uint16_t to_e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ __half2 e4m3x2_to_half2(uint16_t v) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(v));
+  return *reinterpret_cast<__half2*>(&r);
+}
+__device__ __forceinline__ float2 from_e4m3x2(uint16_t v) { return __half22float2(e4m3x2_to_half2(v)); }
+
+// ---------------------------------------------------------------- scales
+// least e in [MIN_EXP, MAX_EXP] with amax <= 448·2^e (448 = 0.875·2^9), amax finite and >= 0
+__device__ __forceinline__ int scale_exp(float amax) {
+  int x;
+  const float m = frexpf(amax, &x);
+  const int e = amax > 0.f ? x - 9 + (m > 0.875f ? 1 : 0) : MIN_EXP;
+  return min(max(e, MIN_EXP), MAX_EXP);
+}
+__device__ __forceinline__ float exp2i(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
+__device__ __forceinline__ int exp_of(float scale) { return ((__float_as_int(scale) >> 23) & 0xff) - 127; }
+
+// ---------------------------------------------------------------- work division
+// A unit is (sequence b, row group rg, kv head g): `R` query rows (t, q head of the group) against
+// the keys the last of them sees, cut into tiles of 128 keys. The tiles of all units, in the
+// order b, rg, g, are divided evenly over the CTAs, so a ragged batch, one long sequence and many
+// short ones all keep every SM equally busy. A CTA's share is a run of pieces (parts of units).
+// A piece that is a whole unit is written out by its CTA; the others leave a partial (o, m, l)
+// in the workspace: slot 2c for the first piece of CTA c, 2c + 1 for its last. The CTA in whose
+// share a divided unit begins describes it in meta[c] for the merge kernel.
+struct Piece {
+  int b, rg, g;
+  int j0, n;        // first tile and tiles of this piece
+  int unit_tiles;   // tiles of the unit
+  bool first;       // the CTA's first piece
+  __device__ __forceinline__ bool whole() const { return n == unit_tiles; }
+  __device__ __forceinline__ int slot() const { return 2 * (int)blockIdx.x + (first ? 0 : 1); }
+};
+
+__device__ __forceinline__ int unit_tiles(const qsp_attn_kv8_layer& L, int i, int n_rg, int R) {
+  const int b = i / n_rg, rg = i - b * n_rg;
+  const int nrep = L.n_heads / L.n_kv_heads;
+  const int t_last = min(L.tokens - 1, ((rg + 1) * R - 1) / nrep);
+  const long long cap = (long long)L.max_pages * L.page_size;
+  const long long kv = min((long long)L.seq_lens[b] + t_last + 1, cap);
+  return kv <= TILE ? 1 : (int)((kv + TILE - 1) / TILE);   // a unit without keys has a tile too: it writes zeros
+}
+
+struct Walk {
+  int i, g, j0;         // unit (i = b·n_rg + rg, g) and the tile in it to go on at
+  long long pos;                 // that tile's number among all tiles
+  long long begin, end;          // this CTA's share
+  long long total, parts;        // tiles of all units, and the CTAs that share them
+};
+
+// This CTA's share, found by all threads of the CTA; `sh` holds 34 long longs of shared memory.
+// Begins and ends with a __syncthreads.
+__device__ __forceinline__ Walk share(const qsp_attn_kv8_layer& L, int n_rg, int R, long long* sh) {
+  const int n = L.batch * n_rg, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
+  long long s = 0;
+  for (int i = tid; i < n; i += blockDim.x) s += unit_tiles(L, i, n_rg, R);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  __syncthreads();
+  if (lane == 0) sh[warp] = s;
+  __syncthreads();
+  long long all = 0;
+  for (int w = 0; w < nw; ++w) all += sh[w];
+  all *= L.n_kv_heads;
+  const long long parts = min((long long)gridDim.x, all);   // no more CTAs than tiles: every one of them has some
+  const long long begin = min((long long)blockIdx.x, parts) * all / parts;
+  const long long end = min((long long)blockIdx.x + 1, parts) * all / parts;
+  if (warp == 0) {
+    long long before = 0;   // tiles of one kv head in the units before i0
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      const int i = i0 + lane;
+      const int mine = i < n ? unit_tiles(L, i, n_rg, R) : 0;
+      long long incl = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+      }
+      const long long a = (before + incl - mine) * L.n_kv_heads, z = (before + incl) * L.n_kv_heads;
+      const bool here = mine > 0 && a <= begin && begin < z;
+      if (here) {
+        sh[32] = ((long long)i << 32) | (unsigned)((begin - a) / mine);
+        sh[33] = (begin - a) % mine;
+      }
+      if (__any_sync(0xffffffffu, here)) break;
+      before += __shfl_sync(0xffffffffu, incl, 31);
+    }
+  }
+  __syncthreads();
+  Walk w;
+  w.i = (int)(sh[32] >> 32);
+  w.g = (int)(sh[32] & 0xffffffff);
+  w.j0 = (int)sh[33];
+  w.pos = w.begin = begin;
+  w.end = end;
+  w.total = all;
+  w.parts = parts;
+  return w;
+}
+
+__device__ __forceinline__ bool next_piece(const qsp_attn_kv8_layer& L, int n_rg, int R, Walk& w, Piece& p) {
+  if (w.pos >= w.end) return false;
+  p.b = w.i / n_rg;
+  p.rg = w.i - p.b * n_rg;
+  p.g = w.g;
+  p.j0 = w.j0;
+  p.unit_tiles = unit_tiles(L, w.i, n_rg, R);
+  p.n = (int)min((long long)(p.unit_tiles - w.j0), w.end - w.pos);
+  p.first = w.pos == w.begin;
+  w.pos += p.n;
+  w.j0 = 0;
+  if (++w.g == L.n_kv_heads) {
+    w.g = 0;
+    ++w.i;
+  }
+  return true;
+}
+
+// workspace: meta [G] int4, then partials: ml [2G][R] float2 (m in log2 units, l), o [2G][R][hd]
+struct Scratch {
+  int4* meta;
+  float2* ml;
+  float* o;
+};
+__host__ __device__ __forceinline__ Scratch scratch(const qsp_attn_kv8_layer& L, int G, int R) {
+  Scratch s;
+  s.meta = static_cast<int4*>(L.workspace);
+  s.ml = reinterpret_cast<float2*>(s.meta + G);
+  s.o = reinterpret_cast<float*>(s.ml + 2ll * G * R);
+  return s;
+}
+inline size_t scratch_bytes(int G, int R, int hd) { return (size_t)G * 16 + 2ull * G * R * (8 + 4ull * hd); }
+
+// meta of this CTA: {b, rg, g | 2^30 when its partial is in slot 2c + 1, partials (0: no unit that is
+// divided begins here)}. Called by one thread after the last piece `p` (p.n == 0: no piece at all).
+__device__ __forceinline__ void put_meta(const Scratch& s, const Walk& w, const Piece& p) {
+  int4 m = make_int4(0, 0, 0, 0);
+  if (p.n > 0 && !p.whole() && p.j0 == 0) {
+    const long long last = w.end - p.n + p.unit_tiles - 1;               // the unit's last tile
+    const int c1 = (int)(((last + 1) * w.parts - 1) / w.total);         // ... and the CTA that has it
+    m = make_int4(p.b, p.rg, p.g | (p.first ? 0 : 1 << 30), c1 - (int)blockIdx.x + 1);
+  }
+  s.meta[blockIdx.x] = m;
+}
+
+int launch_merge(const qsp_attn_kv8_layer& L, int G, int R, cudaStream_t st);
+
+}  // namespace kv8
+}  // namespace qsp

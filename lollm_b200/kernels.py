@@ -146,6 +146,113 @@ def attn_workspace_bytes(batch, tokens, n_heads, head_dim, num_splits) -> int:
     return int(L.load().qsp_attn_workspace_bytes(batch, tokens, n_heads, head_dim, num_splits))
 
 
+def attn_kv8_workspace_bytes(batch, tokens, n_heads, n_kv_heads, head_dim, dtype) -> int:
+    """Bytes of workspace one attn_kv8_verify call needs (on the current device)."""
+    n = int(L.load().qsp_attn_kv8_workspace_bytes(batch, tokens, n_heads, n_kv_heads, head_dim, L.dtype_code(dtype)))
+    if n <= 0:
+        raise RuntimeError("qsp_attn_kv8_workspace_bytes: invalid sizes")
+    return n
+
+
+def attn_kv8_layer(qkv, q_norm_w, k_norm_w, rope_cos, rope_sin, k_pages, v_pages, k_scales, v_scales, page_table,
+                   seq_lens, q_buf, out, *, tokens, n_heads, eps, scale=None, workspace=None, bad_index=None) -> L.AttnKv8Layer:
+    """qsp_attn_kv8_layer of one attention layer over an 8-bit paged cache: `tokens` new tokens of
+    each of page_table.shape[0] sequences.
+
+    qkv [B·T, ≥ 2·n_heads·hd + 2·n_kv·hd] (rows [q|gate per head, k, v]), norm weights [hd], RoPE
+    tables [rows, rotary_dim], q_buf and out [B·T, n_heads·hd]: all in the model dtype.
+    k_pages, v_pages [pages, n_kv, page_size, hd] float8_e4m3fn; k_scales, v_scales
+    [pages, n_kv, page_size / scale_block] fp32; page_table [B, max_pages], seq_lens [B] int32.
+    `scale` multiplies the scores (hd ** -0.5 when None). The descriptor holds the tensors, and may be
+    used again while they keep their meaning; without `workspace` it has one of its own, so that two
+    descriptors never share one."""
+    dev = qkv.device
+    given = dict(qkv=qkv, q_norm_w=q_norm_w, k_norm_w=k_norm_w, rope_cos=rope_cos, rope_sin=rope_sin, k_pages=k_pages,
+                 v_pages=v_pages, k_scales=k_scales, v_scales=v_scales, page_table=page_table, seq_lens=seq_lens,
+                 q_buf=q_buf, out=out)
+    if workspace is not None:
+        given["workspace"] = workspace
+    if bad_index is not None:
+        given["bad_index"] = bad_index
+    for name, t in given.items():
+        L.require_cuda(t, name)
+        if t.device != dev:
+            raise RuntimeError(f"attn_kv8_layer: {name} is on {t.device}, qkv on {dev}")
+        if name in ("qkv", "out"):
+            if t.dim() != 2 or t.stride(1) != 1:
+                raise RuntimeError(f"attn_kv8_layer: {name} must be 2-D with unit inner stride")
+        elif not t.is_contiguous():
+            raise RuntimeError(f"attn_kv8_layer: {name} must be contiguous")
+
+    def want(name, dtype, *shape):
+        t = given[name]
+        if t.dtype != dtype or tuple(t.shape) != shape:
+            raise RuntimeError(f"attn_kv8_layer: {name} must be {dtype} {shape}, not {t.dtype} {tuple(t.shape)}")
+
+    dt, B, T = qkv.dtype, page_table.shape[0], int(tokens)
+    if k_pages.dim() != 4 or k_scales.dim() != 3 or page_table.dim() != 2 or rope_cos.dim() != 2:
+        raise RuntimeError("attn_kv8_layer: pages are 4-D, scales 3-D, page_table and RoPE tables 2-D")
+    P, nkv, ps, hd = k_pages.shape
+    nb, (rows, rd) = k_scales.shape[2], rope_cos.shape
+    if nb == 0 or ps % nb != 0:
+        raise RuntimeError(f"attn_kv8_layer: {nb} scales do not divide a page of {ps} tokens")
+    code = L.dtype_code(dt)
+    for name in ("k_pages", "v_pages"):
+        want(name, torch.float8_e4m3fn, P, nkv, ps, hd)
+    for name in ("k_scales", "v_scales"):
+        want(name, torch.float32, P, nkv, nb)
+    for name in ("q_norm_w", "k_norm_w"):
+        want(name, dt, hd)
+    for name in ("rope_cos", "rope_sin"):
+        want(name, dt, rows, rd)
+    want("page_table", torch.int32, B, page_table.shape[1])
+    want("seq_lens", torch.int32, B)
+    if qkv.shape[0] < B * T or qkv.shape[1] < (2 * n_heads + 2 * nkv) * hd:
+        raise RuntimeError(f"attn_kv8_layer: qkv {tuple(qkv.shape)} is too small for {B} x {T} tokens")
+    if out.dtype != dt or out.shape[0] < B * T or out.shape[1] < n_heads * hd:
+        raise RuntimeError(f"attn_kv8_layer: out must be {dt}, at least {(B * T, n_heads * hd)}")
+    if q_buf.dtype != dt or q_buf.numel() < B * T * n_heads * hd:
+        raise RuntimeError(f"attn_kv8_layer: q_buf must be {dt} with {B * T * n_heads * hd} elements")
+    if bad_index is not None:
+        want("bad_index", torch.int32, 1)
+    if workspace is None:
+        workspace = torch.empty(attn_kv8_workspace_bytes(B, T, n_heads, nkv, hd, dt), dtype=torch.uint8, device=dev)
+    d = L.AttnKv8Layer()
+    d.batch, d.tokens, d.n_heads, d.n_kv_heads, d.head_dim, d.rotary_dim = B, T, n_heads, nkv, hd, rd
+    d.page_size, d.max_pages, d.num_pages, d.scale_block, d.rope_rows = ps, page_table.shape[1], P, ps // nb, rows
+    d.dtype, d.eps, d.scale = code, eps, hd ** -0.5 if scale is None else scale
+    d.qkv, d.ld_qkv = qkv.data_ptr(), qkv.stride(0)
+    d.q_norm_w, d.k_norm_w = q_norm_w.data_ptr(), k_norm_w.data_ptr()
+    d.rope_cos, d.rope_sin = rope_cos.data_ptr(), rope_sin.data_ptr()
+    d.k_pages, d.v_pages = k_pages.data_ptr(), v_pages.data_ptr()
+    d.k_scales, d.v_scales = k_scales.data_ptr(), v_scales.data_ptr()
+    d.page_table, d.seq_lens, d.q_buf = page_table.data_ptr(), seq_lens.data_ptr(), q_buf.data_ptr()
+    d.out, d.ld_out = out.data_ptr(), out.stride(0)
+    d.workspace, d.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    d.bad_index = L.ptr(bad_index)
+    given["workspace"] = workspace
+    d._keep = given   # the struct holds raw pointers: keep the tensors alive
+    return d
+
+
+def _on_its_device(desc):
+    dev = desc._keep["qkv"].device if hasattr(desc, "_keep") else None
+    if dev is not None and dev.index != torch.cuda.current_device():
+        raise RuntimeError(f"the layer's tensors are on {dev}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def attn_kv8_prep(desc: L.AttnKv8Layer):
+    """Norm and rotate q into q_buf, append k and v to the 8-bit pages."""
+    _on_its_device(desc)
+    L.call("qsp_attn_kv8_prep", C.byref(desc), _s())
+
+
+def attn_kv8_verify(desc: L.AttnKv8Layer):
+    """Gated attention of the new tokens' q_buf over the 8-bit pages, into out."""
+    _on_its_device(desc)
+    L.call("qsp_attn_kv8_verify", C.byref(desc), _s())
+
+
 def mtp_single_token_attn(gate, gate_head_stride, v, out, n_heads, n_kv, hd, rows=None):
     _cuda(gate, v, out)
     n = out.shape[0] if rows is None else rows
