@@ -21,41 +21,14 @@ namespace kv8 {
 // sequence. There are 1/8 as many k as q heads, and B200 runs fp64 at half the fp32 rate.
 constexpr int PREP_THREADS = 128;
 
-template <typename T, int EPL>
-__device__ __forceinline__ void load_row(const T* p, int lane, bool vec, float (&x)[EPL]) {
-  if constexpr (EPL * sizeof(T) >= 4) {
-    if (vec) {
-      constexpr int BYTES = EPL * sizeof(T), W = BYTES > 16 ? 16 : BYTES, N = BYTES / W, PER = W / (int)sizeof(T);
-      const char* src = reinterpret_cast<const char*>(p) + (size_t)lane * BYTES;
-#pragma unroll
-      for (int n = 0; n < N; ++n) {
-        alignas(16) T t[PER];
-        if constexpr (W == 16) *reinterpret_cast<uint4*>(t) = *reinterpret_cast<const uint4*>(src + n * W);
-        else if constexpr (W == 8) *reinterpret_cast<uint2*>(t) = *reinterpret_cast<const uint2*>(src + n * W);
-        else *reinterpret_cast<uint32_t*>(t) = *reinterpret_cast<const uint32_t*>(src + n * W);
-#pragma unroll
-        for (int i = 0; i < PER; ++i) x[n * PER + i] = dt<T>::to_f(t[i]);
-      }
-      return;
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < EPL; ++i) x[i] = dt<T>::to_f(p[lane * EPL + i]);
-}
-
 // EPL codes of a lane, EPL bytes at dst + lane·EPL
 template <int EPL>
 __device__ __forceinline__ void store_codes(uint8_t* dst, int lane, const float (&x)[EPL], float inv) {
-  if constexpr (EPL == 1) {
-    dst[lane] = (uint8_t)to_e4m3x2(x[0] * inv, 0.f);
-  } else {
-    alignas(8) uint16_t c[EPL / 2];
+  uint32_t c[2] = {0, 0};
 #pragma unroll
-    for (int i = 0; i < EPL / 2; ++i) c[i] = to_e4m3x2(x[2 * i] * inv, x[2 * i + 1] * inv);
-    if constexpr (EPL == 2) reinterpret_cast<uint16_t*>(dst)[lane] = c[0];
-    else if constexpr (EPL == 4) reinterpret_cast<uint32_t*>(dst)[lane] = *reinterpret_cast<uint32_t*>(c);
-    else reinterpret_cast<uint2*>(dst)[lane] = *reinterpret_cast<uint2*>(c);
-  }
+  for (int i = 0; i < EPL; i += 2)
+    c[i / 4] |= (uint32_t)to_e4m3x2(x[i] * inv, EPL > 1 ? x[EPL > 1 ? i + 1 : 0] * inv : 0.f) << (i % 4 * 8);
+  store_bytes<EPL>(dst + lane * EPL, c[0], c[1]);
 }
 
 // one head's row in F (float for q, double for k): norm, times 1 + w, rotate the first rd dims
@@ -123,17 +96,27 @@ __global__ void __launch_bounds__(PREP_THREADS) prep_kernel(const qsp_attn_kv8_l
     // a position outside the table is flagged by the quantising CTAs; its q is rotated as position 0
     norm_rotate<T, HD, float>(L, x, static_cast<const T*>(L.q_norm_w), pos >= 0 && pos < L.rope_rows ? (int)pos : 0, lane,
                               reinterpret_cast<float*>(xs[warp]), y);
-    alignas(16) T o[EPL];
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) o[i] = dt<T>::from_f(y[i]);
     T* dst = static_cast<T*>(L.q_buf) + (m * nh + h) * HD + lane * EPL;
-    constexpr int BYTES = EPL * sizeof(T);
-    if constexpr (BYTES >= 16) {
+    if constexpr (sizeof(T) == 4) {
+      if constexpr (EPL % 4 == 0) {
 #pragma unroll
-      for (int n = 0; n < BYTES / 16; ++n) reinterpret_cast<uint4*>(dst)[n] = reinterpret_cast<uint4*>(o)[n];
-    } else if constexpr (BYTES == 8) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(o);
-    else if constexpr (BYTES == 4) *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<uint32_t*>(o);
-    else *dst = o[0];
+        for (int i = 0; i < EPL; i += 4) *reinterpret_cast<float4*>(dst + i) = make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) dst[i] = dt<T>::from_f(y[i]);
+      }
+    } else {
+      uint32_t o[EPL > 1 ? EPL / 2 : 1];
+#pragma unroll
+      for (int i = 0; i < EPL; i += 2) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(y[i], EPL > 1 ? y[EPL > 1 ? i + 1 : 0] : 0.f);
+        o[i / 2] = *reinterpret_cast<const uint32_t*>(&v);
+      }
+      if constexpr (EPL == 8) *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+      else if constexpr (EPL == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(o[0], o[1]);
+      else if constexpr (EPL == 2) *reinterpret_cast<uint32_t*>(dst) = o[0];
+      else *dst = dt<T>::from_f(y[0]);
+    }
     return;
   }
 
@@ -510,6 +493,10 @@ int qsp_attn_kv8_verify(const qsp_attn_kv8_layer* layer, void* stream) {
   const int rc = kv8::validate("qsp_attn_kv8_verify", layer, true);
   if (rc) return rc;
   const cudaStream_t st = as_stream(stream);
+  if (layer->dtype == QSP_BF16) {
+    const int rc2 = kv8::launch_tc(*layer, st);
+    if (rc2 != QSP_ERR_UNSUPPORTED) return rc2;
+  }
   const int G = kv8::simt_grid();
   QSP_DISPATCH_DTYPE(layer->dtype, T, {
     switch (layer->head_dim) {
@@ -525,7 +512,10 @@ size_t qsp_attn_kv8_workspace_bytes(int32_t batch, int32_t tokens, int32_t n_hea
   if (batch <= 0 || tokens <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads != 0 || head_dim <= 0 ||
       (dtype != QSP_F32 && dtype != QSP_BF16))
     return 0;
-  return kv8::scratch_bytes(kv8::simt_grid(), kv8::SIMT_R, head_dim);
+  const size_t simt = kv8::scratch_bytes(kv8::simt_grid(), kv8::SIMT_R, head_dim);
+  if (dtype == QSP_F32) return simt;
+  const int R = kv8::tc_rows(n_heads / n_kv_heads * std::min(tokens, 64));
+  return std::max(simt, kv8::scratch_bytes(kv8::tc_grid(head_dim, R), R, head_dim));
 }
 
 }  // extern "C"

@@ -28,6 +28,53 @@ __device__ __forceinline__ __half2 e4m3x2_to_half2(uint16_t v) {
 }
 __device__ __forceinline__ float2 from_e4m3x2(uint16_t v) { return __half22float2(e4m3x2_to_half2(v)); }
 
+// ---------------------------------------------------------------- a lane's elements of a row
+// EPL elements at p + lane·EPL; vec: that address is a multiple of min(16, EPL elements)
+template <typename T, int EPL>
+__device__ __forceinline__ void load_row(const T* p, int lane, bool vec, float (&x)[EPL]) {
+  const T* src = p + lane * EPL;
+  if constexpr (sizeof(T) == 4 && EPL % 4 == 0) {
+    if (vec) {
+#pragma unroll
+      for (int i = 0; i < EPL; i += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(src + i);
+        x[i] = v.x, x[i + 1] = v.y, x[i + 2] = v.z, x[i + 3] = v.w;
+      }
+      return;
+    }
+  }
+  if constexpr (sizeof(T) == 2 && EPL > 1) {
+    if (vec) {
+      uint32_t v[EPL / 2];   // bf16 pairs: the low half first, each the upper half of an fp32
+      if constexpr (EPL == 8) {
+        const uint4 u = *reinterpret_cast<const uint4*>(src);
+        v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
+      } else if constexpr (EPL == 4) {
+        const uint2 u = *reinterpret_cast<const uint2*>(src);
+        v[0] = u.x, v[1] = u.y;
+      } else {
+        v[0] = *reinterpret_cast<const uint32_t*>(src);
+      }
+#pragma unroll
+      for (int i = 0; i < EPL; i += 2) {
+        x[i] = __uint_as_float(v[i / 2] << 16);
+        x[i + 1] = __uint_as_float(v[i / 2] & 0xffff0000u);
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) x[i] = dt<T>::to_f(src[i]);
+}
+// N = 1, 2, 4 or 8 bytes, a first
+template <int N>
+__device__ __forceinline__ void store_bytes(uint8_t* dst, uint32_t a, uint32_t b) {
+  if constexpr (N == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(a, b);
+  else if constexpr (N == 4) *reinterpret_cast<uint32_t*>(dst) = a;
+  else if constexpr (N == 2) *reinterpret_cast<uint16_t*>(dst) = (uint16_t)a;
+  else *dst = (uint8_t)a;
+}
+
 // ---------------------------------------------------------------- scales
 // least e in [MIN_EXP, MAX_EXP] with amax <= 448·2^e (448 = 0.875·2^9), amax finite and >= 0
 __device__ __forceinline__ int scale_exp(float amax) {
@@ -168,6 +215,11 @@ __device__ __forceinline__ void put_meta(const Scratch& s, const Walk& w, const 
 }
 
 int launch_merge(const qsp_attn_kv8_layer& L, int G, int R, cudaStream_t st);
+// the tensor-core kernel; QSP_ERR_UNSUPPORTED when the shape is not one it takes
+int launch_tc(const qsp_attn_kv8_layer& L, cudaStream_t st);
+int tc_rows(int rows);            // its query rows per unit, for this many rows of a kv head
+int tc_grid(int hd, int R);       // its CTAs
+int device_error(int reset);
 
 }  // namespace kv8
 }  // namespace qsp

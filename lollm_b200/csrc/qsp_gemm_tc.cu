@@ -838,6 +838,9 @@ int gemm_pair_device_error(int reset);
 int core_device_error(int reset);
 int sample_device_error(int reset);
 int probe_device_error(int reset);
+namespace kv8 {
+int device_error(int reset);
+}
 }
 
 extern "C" int qsp_device_status(int32_t* code, int32_t reset) {
@@ -847,7 +850,8 @@ extern "C" int qsp_device_status(int32_t* code, int32_t reset) {
   const int moe = qsp::moe_device_error(reset);
   const int cl = qsp::gemm_cl_device_error(reset);
   const int others[] = {qsp::gemm_pair_device_error(reset), qsp::core_device_error(reset),
-                        qsp::sample_device_error(reset), qsp::probe_device_error(reset)};
+                        qsp::sample_device_error(reset), qsp::probe_device_error(reset),
+                        qsp::kv8::device_error(reset)};
   int v = 0;
   cudaError_t e = cudaMemcpyFromSymbol(&v, qsp::g_qsp_dev_error, sizeof(int));
   if (e != cudaSuccess) return qsp::set_error(QSP_ERR_CUDA, "qsp_device_status: %s", cudaGetErrorString(e));
