@@ -96,17 +96,17 @@ class _TokenLoop:
 
 @torch.no_grad()
 def generate(model, ids, decode, stop_ids, device, *, max_new_tokens=128, temperature=0.7,
-             top_k=20, top_p=0.8, repetition_penalty=1.1):
+             top_k=20, top_p=0.8, repetition_penalty=1.1, **cache_kw):
     """Drop-in for the reference's `generate` (src/generate.py:41-62): same signature, same
     defaults and the same output — prefill, then one token per forward until `stop_ids` or
     `max_new_tokens`, yielding the newly decoded text after each token (`decode(list[int])
     -> str`). The sampled token never leaves the device on its way into the next forward
     and the penalty context lives on the device; the host reads one token per step to
-    decide on stopping and to decode."""
+    decide on stopping and to decode. Further keywords are the cache's (kv_dtype)."""
     prompt = list(ids)
     loop = _TokenLoop(prompt, max_new_tokens, model.cfg.vocab_size, device, temperature, top_k, top_p,
                       repetition_penalty)
-    logits, past = model(torch.tensor([prompt], device=device))
+    logits, past = model(torch.tensor([prompt], device=device), model.new_cache(1, **cache_kw) if cache_kw else None)
     eos = set(stop_ids)
     out, shown = [], 0
     while len(out) < max_new_tokens:

@@ -8,6 +8,9 @@ kv.py:1-14 / modeling_qwen3_5.py:8-11):
 * full-attention layers keep K/V in fixed-size pages, [num_pages, n_kv, page_size, hd] per
   layer, addressed through a per-sequence page table, instead of a tensor grown by
   `torch.cat` (kv.py:26-33);
+* with `kv_dtype=torch.float8_e4m3fn` the pages hold 8-bit codes and one power-of-two scale for
+  each block of `scale_block` tokens and kv head ([num_pages, n_kv, page_size / scale_block] fp32
+  per layer): half the bytes of a bf16 cache. Appending quantises, the attention reads the codes;
 * every sequence has its own length (`seq_lens`, device int32) instead of one scalar
   `seen_tokens` (kv.py:23), so a batch can be ragged;
 * GDN layers keep the fp32 recurrent state [B, Hv, dk, dv] (the reference layout) plus a
@@ -30,10 +33,14 @@ from .. import _lib as L
 from .config import Qwen3_5Config
 
 
+F8 = torch.float8_e4m3fn
+
+
 class Qwen3_5Cache:
     def __init__(self, cfg: Qwen3_5Config, batch: int, max_len: int, *, dtype, device,
                  page_size: int = 64, max_spec_tokens: int = 8, num_pages: int | None = None,
-                 page_table: torch.Tensor | None = None):
+                 page_table: torch.Tensor | None = None, kv_dtype: torch.dtype | None = None,
+                 scale_block: int = 16):
         self.cfg, self.batch, self.dtype, self.device = cfg, batch, dtype, torch.device(device)
         self.page_size, self.max_spec_tokens = page_size, max_spec_tokens
         self.max_pages = math.ceil(max_len / page_size)
@@ -44,8 +51,23 @@ class Qwen3_5Cache:
         nkv, hd = cfg.num_key_value_heads, cfg.head_dim
         self.num_pages = num_pages or batch * self.max_pages
         dev = self.device
-        self.k_pages = torch.zeros(n_attn, self.num_pages, nkv, page_size, hd, dtype=dtype, device=dev)
-        self.v_pages = torch.zeros_like(self.k_pages)
+        self.kv_dtype = dtype if kv_dtype is None else kv_dtype
+        self.kv8 = self.kv_dtype == F8
+        if not self.kv8 and self.kv_dtype != dtype:
+            raise RuntimeError(f"kv_dtype must be {dtype} (the model's) or {F8}, not {kv_dtype}")
+        pages = (n_attn, self.num_pages, nkv, page_size, hd)
+        self.k_scales = self.v_scales = None
+        if self.kv8:
+            if scale_block not in (1, 2, 4, 8, 16, 32, 64) or page_size % scale_block != 0:
+                raise RuntimeError(f"scale_block {scale_block} must be a power of two up to 64 that divides the "
+                                   f"page size {page_size}")
+            self.k_pages, self.v_pages = (torch.zeros(pages, dtype=torch.uint8, device=dev).view(F8) for _ in range(2))
+            self.k_scales, self.v_scales = (torch.ones(n_attn, self.num_pages, nkv, page_size // scale_block,
+                                                       dtype=torch.float32, device=dev) for _ in range(2))
+        else:
+            self.k_pages = torch.zeros(pages, dtype=dtype, device=dev)
+            self.v_pages = torch.zeros_like(self.k_pages)
+        self.scale_block = scale_block
         if page_table is None:
             page_table = torch.arange(batch * self.max_pages, dtype=torch.int32).view(batch, self.max_pages)
         if tuple(page_table.shape) != (batch, self.max_pages):
@@ -90,6 +112,12 @@ class Qwen3_5Cache:
         s = self.attn_slot[layer]
         B, _, t, _ = k.shape
         lens = self.seq_lens.long()
+        if self.kv8:
+            for j in range(t):
+                for pages, scales, x in ((self.k_pages[s], self.k_scales[s], k), (self.v_pages[s], self.v_scales[s], v)):
+                    self._append8(pages, scales, x[:, :, j].float(), lens + j)
+            self.seq_lens += t
+            return self.read_kv(layer)
         for j in range(t):
             pos = lens + j
             page = self.page_table.long().gather(1, (pos // self.page_size)[:, None])[:, 0]
@@ -98,6 +126,27 @@ class Qwen3_5Cache:
             self.v_pages[s, page, :, slot] = v[:, :, j].to(self.dtype)
         self.seq_lens += t
         return self.read_kv(layer)
+
+    def _append8(self, pages, scales, x, pos):
+        """One token x (B, n_kv, hd) fp32 per sequence into 8-bit pages, by the rule of
+        `qsp_attn_kv8_prep`: the block's scale is the least power of two that holds the token and
+        what the block has; earlier codes follow when it grows."""
+        page = self.page_table.long().gather(1, (pos // self.page_size)[:, None])[:, 0]
+        slot, sb = pos % self.page_size, self.scale_block
+        blk = slot // sb
+        m, e = torch.frexp(x.abs().amax(-1))                                   # (B, n_kv)
+        e = torch.where(m > 0, e - 9 + (m > 0.875).int(), -40).clamp_min(-40)
+        was = torch.frexp(scales[page, :, blk])[1] - 1
+        now = torch.where((slot % sb > 0)[:, None], torch.maximum(e, was), e)
+        raw = pages.view(torch.uint8)
+        at = (blk * sb)[:, None] + torch.arange(sb, device=pos.device)         # (B, sb) slots of the block
+        heads = torch.arange(x.shape[1], device=pos.device)
+        index = (page[:, None, None], heads[:, None], at[:, None, :])
+        old = raw[index]
+        moved = torch.ldexp(old.view(F8).float(), (was - now)[..., None, None]).to(F8).view(torch.uint8)
+        raw[index] = torch.where((at < slot[:, None])[:, None, :, None], moved, old)
+        raw[page, :, slot] = torch.ldexp(x, -now[..., None]).to(F8).view(torch.uint8)
+        scales[page, :, blk] = torch.ldexp(torch.ones_like(x[..., 0]), now)
 
     def read_kv(self, layer: int):
         """(K, V) as (B, n_kv, L, hd) when all lengths are equal, else a list of per-sequence
@@ -110,12 +159,22 @@ class Qwen3_5Cache:
         for b, n in enumerate(lens):
             npg = math.ceil(n / self.page_size)
             pages = self.page_table[b, :npg].long()
+            if self.kv8:
+                per.append(tuple(self._read8(c[s], sc[s], pages)[:, :n] for c, sc in
+                                 ((self.k_pages, self.k_scales), (self.v_pages, self.v_scales))))
+                continue
             kk = self.k_pages[s, pages].permute(1, 0, 2, 3).reshape(self.cfg.num_key_value_heads, -1, self.cfg.head_dim)[:, :n]
             vv = self.v_pages[s, pages].permute(1, 0, 2, 3).reshape(self.cfg.num_key_value_heads, -1, self.cfg.head_dim)[:, :n]
             per.append((kk, vv))
         if len(set(lens)) == 1:
             return torch.stack([p[0] for p in per]), torch.stack([p[1] for p in per])
         return per
+
+    def _read8(self, codes, scales, pages):
+        """The values (n_kv, tokens, hd) of 8-bit pages, in the model dtype."""
+        x = codes.view(torch.uint8)[pages].view(F8).float()
+        x = x * scales[pages].repeat_interleave(self.scale_block, -1)[..., None]
+        return x.transpose(0, 1).reshape(x.shape[1], -1, x.shape[3]).to(self.dtype)
 
     def linear_state(self, layer: int):
         """(conv_state (B, conv_dim, K-1), recurrent_state (B, Hv, dk, dv) fp32) of a GDN layer,
@@ -146,7 +205,8 @@ class Qwen3_5Cache:
     def nbytes(self) -> int:
         """Bytes held by the cache tensors (kv.py:56-58)."""
         return sum(t.numel() * t.element_size() for t in
-                   (self.k_pages, self.v_pages, self.state, self.conv_hist, self.pending))
+                   (self.k_pages, self.v_pages, self.k_scales, self.v_scales, self.state, self.conv_hist, self.pending)
+                   if t is not None)
 
     def check(self):
         """Raise RuntimeError if a kernel flagged this cache or the device since the last check:

@@ -12,6 +12,7 @@ head consumes. Extensions, all keyword-only and off by default:
 Per layer (modeling_qwen3_5.py:47-61), every box a C-ABI launch:
     [GDN: in_proj(qkv|z|b|a) GEMM → qsp_gdn_verify → out_proj GEMM + residual + RMSNorm]
   | [attn: q|k|v GEMM → qsp_attn_prep → qsp_attn_verify → o_proj GEMM + residual + RMSNorm]
+    (over an 8-bit cache: qsp_attn_kv8_prep → qsp_attn_kv8_verify)
     gate|up GEMM + SwiGLU → down GEMM + residual + next layer's input RMSNorm
   | (qwen3_5_moe layers where cfg.is_moe_layer(i), modeling_qwen3_5_moe.py:42-43)
     qsp_moe_ffn: router + experts + shared expert + residual + next RMSNorm
@@ -47,7 +48,7 @@ class _Workspace:
     """Activation buffers for one (batch, tokens) shape, reused across calls (and stable
     under CUDA-graph capture)."""
 
-    def __init__(self, model: "Qwen3_5Model", B: int, T: int, num_splits: int):
+    def __init__(self, model: "Qwen3_5Model", B: int, T: int, num_splits: int | None):
         cfg, dt, dev = model.cfg, model.dtype, model.device
         M = B * T
         H = cfg.hidden_size
@@ -71,8 +72,13 @@ class _Workspace:
         self.last_logits = e(B, cfg.vocab_size)
         self.last_idx = torch.full((B,), T - 1, dtype=torch.int32, device=dev)
         self.num_splits = num_splits
-        ws = K.attn_workspace_bytes(B, T, cfg.num_attention_heads, cfg.head_dim, num_splits)
-        self.partial = torch.empty(max(ws // 4, 1), dtype=torch.float32, device=dev)
+        # split-KV partials; an 8-bit cache's attention has a workspace of its own (num_splits None)
+        if num_splits is None:
+            self.kv8_ws = torch.empty(K.attn_kv8_workspace_bytes(B, T, cfg.num_attention_heads, cfg.num_key_value_heads,
+                                                                 cfg.head_dim, dt), dtype=torch.uint8, device=dev)
+        else:
+            ws = K.attn_workspace_bytes(B, T, cfg.num_attention_heads, cfg.head_dim, num_splits)
+            self.partial = torch.empty(max(ws // 4, 1), dtype=torch.float32, device=dev)
 
     @property
     def logits(self):
@@ -142,6 +148,8 @@ class Qwen3_5Model:
 
     # ------------------------------------------------------------------ helpers
     def new_cache(self, batch: int, max_len: int | None = None, **kw) -> Qwen3_5Cache:
+        """A cache of `max_len` positions per sequence. kv_dtype=torch.float8_e4m3fn keeps keys and
+        values in 8 bits, with one scale for each `scale_block` tokens (16) and kv head."""
         max_len = max_len or self.max_positions
         if max_len > self.max_positions:
             raise RuntimeError(f"max_len {max_len} exceeds the RoPE table ({self.max_positions})")
@@ -154,9 +162,9 @@ class Qwen3_5Model:
         return attn_num_splits(cache.capacity, B * self.cfg.num_key_value_heads)
 
     def workspace(self, B: int, T: int, cache: Qwen3_5Cache) -> _Workspace:
-        key = (B, T, cache.capacity)
+        key = (B, T, cache.capacity) + (("kv8",) if cache.kv8 else ())
         if key not in self._ws:
-            self._ws[key] = _Workspace(self, B, T, self.default_splits(B, cache))
+            self._ws[key] = _Workspace(self, B, T, None if cache.kv8 else self.default_splits(B, cache))
         return self._ws[key]
 
     def attn_desc(self, lw, cache: Qwen3_5Cache, slot: int, ws: _Workspace, B: int, T: int):
@@ -175,6 +183,28 @@ class Qwen3_5Model:
         d.q_buf = ws.q_buf.data_ptr()
         d.out, d.ld_out = ws.core.data_ptr(), ws.core.stride(0)
         d.partial, d.num_splits = ws.partial.data_ptr(), ws.num_splits
+        d.bad_index = cache.bad_index.data_ptr()
+        return d
+
+    def attn_kv8_desc(self, lw, cache: Qwen3_5Cache, slot: int, ws: _Workspace, B: int, T: int):
+        """The layer over an 8-bit cache; the tensors live in the model, the cache and the workspace."""
+        cfg = self.cfg
+        d = L.AttnKv8Layer()
+        d.batch, d.tokens = B, T
+        d.n_heads, d.n_kv_heads, d.head_dim, d.rotary_dim = (cfg.num_attention_heads, cfg.num_key_value_heads,
+                                                             cfg.head_dim, cfg.rotary_dim)
+        d.page_size, d.max_pages, d.num_pages = cache.page_size, cache.max_pages, cache.num_pages
+        d.scale_block, d.rope_rows = cache.scale_block, self.max_positions
+        d.dtype, d.eps, d.scale = L.dtype_code(self.dtype), cfg.rms_norm_eps, cfg.head_dim ** -0.5
+        d.qkv, d.ld_qkv = ws.proj.data_ptr(), ws.proj.stride(0)
+        d.q_norm_w, d.k_norm_w = lw["q_norm"].data_ptr(), lw["k_norm"].data_ptr()
+        d.rope_cos, d.rope_sin = self.rope_cos.data_ptr(), self.rope_sin.data_ptr()
+        d.k_pages, d.v_pages = cache.k_pages[slot].data_ptr(), cache.v_pages[slot].data_ptr()
+        d.k_scales, d.v_scales = cache.k_scales[slot].data_ptr(), cache.v_scales[slot].data_ptr()
+        d.page_table, d.seq_lens = cache.page_table.data_ptr(), cache.seq_lens.data_ptr()
+        d.q_buf = ws.q_buf.data_ptr()
+        d.out, d.ld_out = ws.core.data_ptr(), ws.core.stride(0)
+        d.workspace, d.workspace_bytes = ws.kv8_ws.data_ptr(), ws.kv8_ws.numel()
         d.bad_index = cache.bad_index.data_ptr()
         return d
 
@@ -231,9 +261,14 @@ class Qwen3_5Model:
             if lw["type"] == "full_attention":
                 slot = cache.attn_slot[i]
                 K.gemm(ws.xn, lw["w_qkv"], ws.proj, m=M)
-                d = self.attn_desc(lw, cache, slot, ws, B, T)
-                K.attn_prep(d)
-                K.attn_verify(d)
+                if cache.kv8:
+                    d = self.attn_kv8_desc(lw, cache, slot, ws, B, T)
+                    K.attn_kv8_prep(d)
+                    K.attn_kv8_verify(d)
+                else:
+                    d = self.attn_desc(lw, cache, slot, ws, B, T)
+                    K.attn_prep(d)
+                    K.attn_verify(d)
                 K.gemm_residual_rmsnorm(ws.core, lw["o_proj"], ws.x, lw["post_norm"], ws.xn, eps, m=M)
             else:
                 slot = cache.gdn_slot[i]

@@ -113,7 +113,8 @@ class MTP:
 
 
 class SpecDecoder:
-    """Batched k-deep speculative decoding over independent sequences on one GPU."""
+    """Batched k-deep speculative decoding over independent sequences on one GPU. Further keywords
+    are the cache's (kv_dtype=torch.float8_e4m3fn keeps keys and values in 8 bits)."""
 
     def __init__(self, model: Qwen3_5Model, mtp: MTP, batch: int, k: int, max_len: int, *,
                  temperature: float = 0.0, top_k: int = 0, top_p: float = 1.0,
@@ -230,17 +231,17 @@ class SpecDecoder:
 @torch.no_grad()
 def generate_mtp(model: Qwen3_5Model, mtp: MTP, ids, decode, stop_ids, device=None, *,
                  max_new_tokens=128, temperature=0.7, top_k=20, top_p=0.8,
-                 repetition_penalty=1.1, k: int = 1, seed: int = 0):
+                 repetition_penalty=1.1, k: int = 1, seed: int = 0, **cache_kw):
     """Drop-in for the reference generator (mtp.py:92-162), same defaults: yields text pieces
     of one sequence. Greedy (temperature <= 0) output equals `generate()` with the same
     repetition penalty. temperature > 0 uses the lossless p/q sampler over the filtered
     target and draft distributions (penalty → temperature → top-k → top-p, as sample_next),
-    with uniforms from a seeded device generator."""
+    with uniforms from a seeded device generator. Further keywords are the cache's (kv_dtype)."""
     eos = set(stop_ids)
     prompt = torch.tensor([list(ids)], dtype=torch.int64, device=model.device)
     dec = SpecDecoder(model, mtp, 1, k, prompt.shape[1] + max_new_tokens + k + 2,
                       temperature=temperature, top_k=top_k, top_p=top_p,
-                      repetition_penalty=repetition_penalty, out_capacity=max_new_tokens + k + 1)
+                      repetition_penalty=repetition_penalty, out_capacity=max_new_tokens + k + 1, **cache_kw)
     gen = torch.Generator(device=model.device)
     gen.manual_seed(seed)
     rand = lambda *s: torch.rand(*s, generator=gen, device=model.device)

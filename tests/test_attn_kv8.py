@@ -131,3 +131,52 @@ def test_oracle_non_finite_tokens():
     assert torch.isnan(kk[0, 1]).all() and (vv[0, 1] == 0).all() and torch.isfinite(kk[0, [0, 2]]).all()
     out = kv8.attend(c, q, gate, 3, 32 ** -0.5)
     assert torch.isfinite(out[0]).all() and torch.isnan(out[1:]).all()
+
+
+# ---------------------------------------------------------------- the family cache
+def _cache(**kw):
+    from lollm_b200.qwen3_5 import Qwen3_5Cache, Qwen3_5Config
+    from lollm_b200.qwen3_5.config import MICRO
+    return Qwen3_5Cache(Qwen3_5Config.from_hf(MICRO), 2, 40, dtype=torch.bfloat16, device="cpu", page_size=16, **kw)
+
+
+def test_cache_refuses():
+    for kw in (dict(kv_dtype=torch.float16), dict(kv_dtype=torch.float32), dict(kv_dtype=kv8.F8, scale_block=3),
+               dict(kv_dtype=kv8.F8, scale_block=32), dict(kv_dtype=kv8.F8, scale_block=0)):
+        with pytest.raises(RuntimeError):
+            _cache(**kw)
+
+
+def test_cache_bytes_and_clone():
+    a, b = _cache(), _cache(kv_dtype=kv8.F8, scale_block=8)
+    kv = a.k_pages.numel() * 2
+    scales = b.k_scales.numel() * 4
+    assert a.nbytes() - b.nbytes() == 2 * (kv - kv // 2 - scales)
+    c = b.clone()
+    c.k_scales.fill_(3.0)
+    c.k_pages.view(torch.uint8).fill_(1)
+    assert (b.k_scales == 1).all() and (b.k_pages.view(torch.uint8) == 0).all()
+
+
+def test_cache_append_kv_matches_the_rule():
+    """The compatibility path token by token against the oracle's append (values: no norm there)."""
+    c = _cache(kv_dtype=kv8.F8, scale_block=8)
+    layer, s = c.cfg.attn_layers[1], 1
+    nkv, hd = c.cfg.num_key_value_heads, c.cfg.head_dim
+    g = torch.Generator().manual_seed(0)
+    o = kv8.new_cache(c.num_pages, nkv, 16, hd, 8, c.page_table.tolist(), [0, 0])
+    z = torch.zeros(hd)
+    for step, t in enumerate([3, 1, 9, 5]):
+        x = torch.randn(2, nkv, t, hd, generator=g) * [1.0, 8.0, 0.1, 100.0][step]
+        got = c.append_kv(layer, -x, x)
+        qkv = torch.zeros(2 * t, 2 * hd + 2 * nkv * hd)
+        qkv[:, 2 * hd + nkv * hd:] = x.transpose(1, 2).reshape(2 * t, -1)
+        for j in range(t):    # token by token, as the path appends
+            rows = qkv.view(2, t, -1)[:, j].contiguous()
+            kv8.append(o, rows, 1, 1, z, z, torch.ones(64, 8), torch.zeros(64, 8))
+            o["lens"] = [n + 1 for n in o["lens"]]
+        for b in range(2):
+            want = kv8.read(o, b, o["lens"][b])[1]
+            assert torch.equal(got[1][b].double(), want.to(torch.bfloat16).double())
+            assert torch.equal(got[0][b], -got[1][b])
+    assert c.seen_tokens == 18
