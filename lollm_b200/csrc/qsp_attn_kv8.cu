@@ -446,7 +446,7 @@ static int validate(const char* what, const qsp_attn_kv8_layer* p, bool verify) 
               "%s: n_heads must be a multiple of n_kv_heads", what);
   QSP_REQUIRE(L.head_dim == 32 || L.head_dim == 64 || L.head_dim == 128 || L.head_dim == 256, "%s: head_dim %d not built", what,
               L.head_dim);
-  QSP_REQUIRE(L.page_size > 0 && L.max_pages > 0 && L.num_pages > 0 && (int64_t)L.max_pages * L.page_size < (1ll << 31),
+  QSP_REQUIRE(L.page_size > 0 && L.max_pages > 0 && L.num_pages > 0 && (int64_t)L.max_pages * L.page_size < (1ll << 30),
               "%s: bad paging", what);
   QSP_REQUIRE(L.scale_block > 0 && L.scale_block <= 64 && (L.scale_block & (L.scale_block - 1)) == 0 &&
                   L.page_size % L.scale_block == 0,

@@ -20,9 +20,9 @@
 // keys need not be known exactly: m is raised (and O rescaled in TMEM) only when some score passes it
 // by more than 2^SLACK; until then the check is one barrier with a vote.
 //
-// Warps: 4 (R = 64: 8) softmax warps, one that loads (TMA), one that issues the MMAs. K and V tiles of
-// 128 keys stream through one ring in the order K0 K1 V0 K2 V1 ..., the scores are double-buffered
-// in TMEM, so the next tile's scores are computed while this one's weights are.
+// Warps: a softmax warpgroup for each 8 rows (R = 64: 16), two warps that load K and V (TMA), one that
+// issues the MMAs. K and V tiles of 128 keys stream through a ring each, scores and weights are
+// double-buffered, so the next tile's scores are computed while this one's weights are.
 //
 // Bound by HBM: a tile of 128 keys at hd 256 is 64 KB, 2800 cycles of an SM's share of 6.5 TB/s; its
 // products take 520 cycles of the tensor cores at R = 32.
@@ -44,22 +44,23 @@ constexpr float NOTHING = -1e30f;    // maximum of a row that has seen nothing
 template <int HD, int R_>
 struct Cfg {
   static constexpr int R = R_, N = 2 * R;                   // query rows, columns (hi | lo)
-  static constexpr int NWG = R == 64 ? 2 : 1, RW = R / NWG;  // softmax warpgroups, rows of each
+  static constexpr int NWG = R < 32 ? R / 8 : 4, RW = R / NWG;   // softmax warpgroups, rows of each
   static constexpr int CW = HD < 128 ? HD : 128;            // bytes of a swizzled row
   static constexpr int CB = HD / CW;                        // column blocks of a tile
   static constexpr int SLOT = TILE * HD;                    // bytes of a K or V tile
   static constexpr int QB = N * HD, PB = TILE * N;
-  static constexpr int OCC = HD == 256 || R == 64 ? 1 : 2;  // CTAs per SM
+  static constexpr int OCC = HD == 256 || R >= 32 ? 1 : 2;  // CTAs per SM
   static constexpr int BUDGET = OCC == 1 ? 232448 : 115712;
   // barriers, row scales, row maxima, reduction buffer
-  static constexpr int SMALL = 8 * 26 + 4 * (R + 2 * R + 4 * R) + 16;
+  static constexpr int SMALL = 8 * 28 + 4 * (R + 2 * R + 4 * R) + 16;
   static constexpr int FIT = (BUDGET - 1024 - SMALL - QB - 2 * PB) / SLOT;
   static constexpr int NS = FIT < 8 ? FIT : 8;              // ring slots
+  static constexpr int NSV = (NS + 1) / 2, NSK = NS - NSV;  // a V tile waits for its weights, a K tile does not
   static constexpr size_t BYTES = 1024 + (size_t)NS * SLOT + QB + 2 * PB + SMALL;
-  static constexpr int THREADS = 128 * NWG + 64;
+  static constexpr int SOFTMAX = 128 * NWG, THREADS = SOFTMAX + 96;
   static constexpr int COLS_USED = 2 * N + CB * N;
   static constexpr int COLS = COLS_USED <= 64 ? 64 : COLS_USED <= 128 ? 128 : COLS_USED <= 256 ? 256 : 512;
-  static_assert(NS >= 4, "ring too short");
+  static_assert(NSK >= 2, "ring too short");
   static_assert(2 * PB >= 34 * 8, "the weights' buffers first hold share()'s 34 long longs");
 };
 
@@ -169,9 +170,9 @@ __device__ __forceinline__ int row_of(int lane) {
 }
 
 // page of a key's position, or -1
-__device__ __forceinline__ int page_of(const qsp_attn_kv8_layer& L, int b, long long key, long long kv_end) {
+__device__ __forceinline__ int page_of(const qsp_attn_kv8_layer& L, int b, int key, int kv_end) {
   if (key >= kv_end) return -1;
-  const int page = L.page_table[(int64_t)b * L.max_pages + (int)key / L.page_size];
+  const int page = L.page_table[(int64_t)b * L.max_pages + key / L.page_size];
   return page >= 0 && page < L.num_pages ? page : -1;
 }
 
@@ -180,45 +181,48 @@ __global__ void __launch_bounds__(Cfg<HD, R_>::THREADS, Cfg<HD, R_>::OCC)
 tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const qsp_attn_kv8_layer L, int n_rg,
           int box_rows) {
   using C = Cfg<HD, R_>;
-  constexpr int R = C::R, N = C::N, RW = C::RW, NS = C::NS, CW = C::CW, CB = C::CB, EPL = HD / 32;
+  constexpr int R = C::R, N = C::N, RW = C::RW, NWG = C::NWG, NSK = C::NSK, NSV = C::NSV, CW = C::CW, CB = C::CB, EPL = HD / 32;
   pdl_trigger();
   extern __shared__ uint8_t raw[];
-  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sQ = ring + NS * C::SLOT;
+  uint8_t* sK = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sV = sK + NSK * C::SLOT;
+  uint8_t* sQ = sV + NSV * C::SLOT;
   uint8_t* sP = sQ + C::QB;                                      // [2][128 keys][N]
-  uint64_t* full = reinterpret_cast<uint64_t*>(sP + 2 * C::PB);
-  uint64_t* empty = full + NS;
-  uint64_t* sfull = empty + NS;   // scores of a tile are in TMEM
-  uint64_t* sempty = sfull + 2;   // ... and have been read
-  uint64_t* pfull = sempty + 2;   // weights of a tile are in shared memory
-  uint64_t* pdone = pfull + 2;    // ... and their product with V is done
+  uint64_t* kfull = reinterpret_cast<uint64_t*>(sP + 2 * C::PB);
+  uint64_t* kempty = kfull + NSK;
+  uint64_t* vfull = kempty + NSK;
+  uint64_t* vempty = vfull + NSV;
+  uint64_t* sfull = vempty + NSV;  // scores of a tile are in TMEM
+  uint64_t* sempty = sfull + 2;    // ... and have been read
+  uint64_t* pfull = sempty + 2;    // weights of a tile are in shared memory
+  uint64_t* pdone = pfull + 2;     // ... and their product with V is done
   uint64_t* qfull = pdone + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(full + 25);   // after at most 2·8 + 9 barriers
-  float* qs = reinterpret_cast<float*>(full + 26);   // [R] scale of a row's scores, in log2 units
-  float* mcur = qs + R;                              // [R] running maximum
-  float* aux = mcur + R;                             // [R] rescaling factor; 1 / l at the end
-  float* red = aux + R;                              // [NWG][4][RW]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kfull + 27);   // after at most 2·8 + 9 barriers
+  float* qs = reinterpret_cast<float*>(kfull + 28);   // [R] scale of a row's scores, in log2 units
+  float* mcur = qs + R;                               // [R] running maximum
+  float* aux = mcur + R;                              // [R] rescaling factor; 1 / l at the end
+  float* red = aux + R;                               // [NWG][4][RW]
   volatile int* abort = reinterpret_cast<volatile int*>(red + 4 * R);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  constexpr int W_LOAD = 4 * C::NWG, W_MMA = W_LOAD + 1;
+  constexpr int W_K = 4 * NWG, W_V = W_K + 1, W_MMA = W_K + 2;
   const int nrep = L.n_heads / L.n_kv_heads, rows_total = nrep * L.tokens;
 
   if (tid == 0) {
-    for (int i = 0; i < NS; ++i) {
-      tc::mbar_init(&full[i], 1);
-      tc::mbar_init(&empty[i], 1);
-    }
+    for (int i = 0; i < 2 * C::NS; ++i) tc::mbar_init(&kfull[i], 1);   // kfull, kempty, vfull, vempty
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(&sfull[i], 1);
-      tc::mbar_init(&sempty[i], 4 * C::NWG);
-      tc::mbar_init(&pfull[i], 4 * C::NWG);
+      tc::mbar_init(&sempty[i], 4 * NWG);
+      tc::mbar_init(&pfull[i], 4 * NWG);
       tc::mbar_init(&pdone[i], 1);
     }
-    tc::mbar_init(qfull, 4 * C::NWG);
+    tc::mbar_init(qfull, 4 * NWG);
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == W_MMA) tc::tmem_alloc(tmem_slot, C::COLS);
+  if (warp == W_MMA) {
+    tc::tmem_alloc(tmem_slot, C::COLS);
+    tc::fence_before();
+  }
   pdl_wait();
   // the weights' buffers are not in use yet: room for share()'s 34 long longs
   Walk w = share(L, n_rg, R, reinterpret_cast<long long*>(sP));
@@ -226,74 +230,80 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
   const Scratch ws = scratch(L, gridDim.x, R);
   auto wait = [&](uint64_t* bar, uint32_t parity) { tc::mbar_wait(bar, parity, CODE_WAIT, &g_kv8_error, abort); };
-  auto kv_end_of = [&](int b) {   // keys of the sequence that can have a page
-    return min((long long)L.seq_lens[b] + L.tokens, (long long)L.max_pages * L.page_size);
-  };
+  const int cap = L.max_pages * L.page_size;
+  auto base_of = [&](int b) { return min(L.seq_lens[b], cap); };
+  auto kv_end_of = [&](int base) { return min(base + L.tokens, cap); };   // keys that can have a page
   Piece p;
   p.n = 0;
 
-  if (warp == W_LOAD) {
-    // ---------------- loads: lane (cb, chunk) brings box_rows keys of a column block
+  if (warp == W_K || warp == W_V) {
+    // ---------------- loads of K and of V: up to 32 boxes a tile (box_rows keys x a column block each),
+    // lane i looks up the page of box i, one tile ahead
+    const bool is_v = warp == W_V;
+    const CUtensorMap* map = is_v ? &tmV : &tmK;
+    uint8_t* ring = is_v ? sV : sK;
+    uint64_t* full = is_v ? vfull : kfull;
+    uint64_t* empty = is_v ? vempty : kempty;
+    const int slots = is_v ? NSV : NSK;
     const int chunks = TILE / box_rows, boxes = chunks * CB;
-    uint32_t idx = 0;   // ring slots used so far
+    int slot = 0;
+    uint32_t turn = 1;   // parity of "empty" for this turn of the ring
     while (next_piece(L, n_rg, R, w, p)) {
-      const long long kv_end = kv_end_of(p.b);
-      auto row_at = [&](int j, int box) -> int {   // row of the pages' [pages·n_kv·page_size, hd] view, or -1
-        const long long key = ((long long)p.j0 + j) * TILE + box % chunks * box_rows;
-        const int page = j < p.n ? page_of(L, p.b, key, kv_end) : -1;
-        return page < 0 ? -1 : (page * L.n_kv_heads + p.g) * L.page_size + (int)key % L.page_size;
+      const int kv_end = kv_end_of(base_of(p.b));
+      auto row_at = [&](int j) -> int {   // row of the pages' [pages·n_kv·page_size, hd] view, or -1
+        const int key = (p.j0 + j) * TILE + lane % chunks * box_rows;
+        const int page = j < p.n && lane < boxes ? page_of(L, p.b, key, kv_end) : -1;
+        return page < 0 ? -1 : (page * L.n_kv_heads + p.g) * L.page_size + key % L.page_size;
       };
-      // up to 32 boxes (box_rows 8 and two column blocks) are one a lane
-      auto load = [&](const CUtensorMap* map, int row) {
-        const int slot = idx % NS;
-        wait(&empty[slot], ((idx / NS) & 1u) ^ 1u);
-        const int n = __popc(__ballot_sync(0xffffffffu, row >= 0));
-        if (lane == 0) tc::mbar_expect_tx(&full[slot], n * box_rows * CW);
-        __syncwarp();
-        if (row >= 0)
-          tc::tma_load_2d(ring + slot * C::SLOT + lane / chunks * (TILE * CW) + lane % chunks * (box_rows * CW), map, &full[slot],
-                          lane / chunks * CW, row);
-        __syncwarp();
-        ++idx;
-      };
-      int row = lane < boxes ? row_at(0, lane) : -1;
-      load(&tmK, row);
+      int row = row_at(0);
       for (int j = 0; j < p.n; ++j) {
-        const int next = lane < boxes ? row_at(j + 1, lane) : -1;
-        if (j + 1 < p.n) load(&tmK, next);
-        load(&tmV, row);
+        const int next = row_at(j + 1);
+        wait(&empty[slot], turn);
+        const uint32_t there = __ballot_sync(0xffffffffu, row >= 0);
+        tc::mbar_expect_tx_warp(&full[slot], __popc(there) * box_rows * CW);
+        uint8_t* dst = ring + slot * C::SLOT;
+        for (int i = 0; i < boxes; ++i) {
+          const int r = __shfl_sync(0xffffffffu, row, i);
+          if (r >= 0) {
+            const int cb = i / chunks;
+            tc::tma_load_2d_warp(dst + cb * (TILE * CW) + (i - cb * chunks) * (box_rows * CW), map, &full[slot], cb * CW, r);
+          }
+        }
         row = next;
+        if (++slot == slots) {
+          slot = 0;
+          turn ^= 1u;
+        }
       }
     }
   } else if (warp == W_MMA) {
     // ---------------- products
     constexpr uint32_t ID_QK = idesc_e4m3(128, N, false), ID_PV = idesc_e4m3(128, N, true);
-    uint32_t idx = 0, tile = 0, piece = 0;
+    uint32_t tile = 0, piece = 0;
     while (next_piece(L, n_rg, R, w, p)) {
       wait(qfull, piece & 1u);
       ++piece;
       const uint32_t t0 = tile;
       auto qk = [&](uint32_t t) {
-        const int slot = idx % NS, sb = t & 1;
-        wait(&full[slot], (idx / NS) & 1u);
+        const int slot = t % NSK, sb = t & 1;
+        wait(&kfull[slot], (t / NSK) & 1u);
         wait(&sempty[sb], ((t >> 1) & 1u) ^ 1u);
         tc::fence_after();
-        const uint32_t a = tc::smem_u32(ring + slot * C::SLOT), q = tc::smem_u32(sQ);
+        const uint32_t a = tc::smem_u32(sK + slot * C::SLOT), q = tc::smem_u32(sQ);
 #pragma unroll
         for (int k = 0; k < HD / 32; ++k) {
           const int cb = k * 32 / CW, off = k * 32 % CW;
           umma_e4m3_warp(tmem + sb * N, sdesc<CW>(a + cb * (TILE * CW) + off, 16), sdesc<CW>(q + cb * (N * CW) + off, 16), ID_QK, k > 0);
         }
-        tc::umma_commit_warp(&empty[slot]);
+        tc::umma_commit_warp(&kempty[slot]);
         tc::umma_commit_warp(&sfull[sb]);
-        ++idx;
       };
       auto pv = [&](uint32_t t) {
-        const int slot = idx % NS, pb = t & 1;
-        wait(&full[slot], (idx / NS) & 1u);
+        const int slot = t % NSV, pb = t & 1;
+        wait(&vfull[slot], (t / NSV) & 1u);
         wait(&pfull[pb], (t >> 1) & 1u);
         tc::fence_after();
-        const uint32_t v = tc::smem_u32(ring + slot * C::SLOT), pp = tc::smem_u32(sP + pb * C::PB);
+        const uint32_t v = tc::smem_u32(sV + slot * C::SLOT), pp = tc::smem_u32(sP + pb * C::PB);
 #pragma unroll
         for (int k = 0; k < TILE / 32; ++k) {
 #pragma unroll
@@ -302,9 +312,8 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
                            N == 16 ? sdesc<16>(pp + k * 32 * N, 8 * 16) : sdesc<N < 32 ? 32 : N>(pp + k * 32 * N, 0), ID_PV,
                            t > t0 || k > 0);
         }
-        tc::umma_commit_warp(&empty[slot]);
+        tc::umma_commit_warp(&vempty[slot]);
         tc::umma_commit_warp(&pdone[pb]);
-        ++idx;
       };
       qk(t0);
       for (int j = 0; j < p.n; ++j) {
@@ -314,30 +323,64 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
       tile = t0 + p.n;
     }
   } else {
-    // ---------------- softmax: thread = key of the tile
+    // ---------------- softmax: thread = key of the tile, RW rows
     const int wg = warp >> 2, wq = warp & 3, key_in = wq * 32 + lane, r0 = wg * RW, bar = 1 + wg;
     const uint32_t tlane = tmem + ((uint32_t)(wq * 32) << 16);
     const int my_row = r0 + row_of<RW>(lane);
-    const int nb = L.page_size / L.scale_block;
-    uint32_t tile = 0, ring0 = 0;   // ring0: slots used before this piece
+    const bool reducer = lane % (32 / RW) == 0;    // its lane of a row's reduction
+    const int nb = L.page_size / L.scale_block, sb_log = __ffs(L.scale_block) - 1;
+    uint32_t tile = 0;
     while (next_piece(L, n_rg, R, w, p)) {
       const int row0 = p.rg * R, nrows = min(R, rows_total - row0);
-      const long long base = L.seq_lens[p.b], kv_end = kv_end_of(p.b);
+      const int base = base_of(p.b), kv_end = kv_end_of(base);
+      // this thread's key: page and slot one tile ahead of its scales, scales one tile ahead of their use
+      const int key0 = p.j0 * TILE + key_in;
+      struct At {
+        int page, blk;
+      };
+      auto at = [&](int j) -> At {
+        const int key = key0 + j * TILE;
+        if (j >= p.n || key >= kv_end) return {-1, 0};
+        const int lp = key / L.page_size;
+        const int page = L.page_table[(int64_t)p.b * L.max_pages + lp];
+        return {page >= 0 && page < L.num_pages ? page : -1, (key - lp * L.page_size) >> sb_log};
+      };
+      auto scales_of = [&](At a, float& ks, float& vs) {
+        ks = vs = 1.f;
+        if (a.page >= 0) {
+          const int64_t i = ((int64_t)a.page * L.n_kv_heads + p.g) * nb + a.blk;
+          ks = L.k_scales[i];
+          vs = L.v_scales[i];
+        }
+      };
+      At a0 = at(0), a1 = at(1);
+      float ks, vs, ks1, vs1;
+
       // stage Q: a warp per row, hi at row r and lo at row R + r of the swizzled tile
-      for (int r = warp; r < R; r += 4 * C::NWG) {
-        float x[EPL];
+      constexpr int ROWS = R / (4 * NWG);
+      float x[ROWS][EPL];
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) {
+        const int r = warp + i * 4 * NWG;
+        if (r < nrows) {
+          const int rr = row0 + r, t = rr / nrep, hq = p.g * nrep + rr - t * nrep;
+          load_row<__nv_bfloat16, EPL>(
+              static_cast<const __nv_bfloat16*>(L.q_buf) + (((int64_t)p.b * L.tokens + t) * L.n_heads + hq) * HD, lane, true, x[i]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < EPL; ++k) x[i][k] = 0.f;
+        }
+      }
+      scales_of(a0, ks, vs);
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) {
+        const int r = warp + i * 4 * NWG;
         float amax = 0.f;
         bool fine = true;
-        if (r < nrows) {
-          const int rr = row0 + r, t = rr / nrep, hq = p.g * nrep + rr % nrep;
-          const __nv_bfloat16* src =
-              static_cast<const __nv_bfloat16*>(L.q_buf) + (((int64_t)p.b * L.tokens + t) * L.n_heads + hq) * HD + lane * EPL;
-          load_row<__nv_bfloat16, EPL>(src, 0, true, x);
 #pragma unroll
-          for (int i = 0; i < EPL; ++i) {
-            amax = fmaxf(amax, fabsf(x[i]));
-            fine = fine && isfinite(x[i]);
-          }
+        for (int k = 0; k < EPL; ++k) {
+          amax = fmaxf(amax, fabsf(x[i][k]));
+          fine = fine && isfinite(x[i][k]);
         }
         amax = warp_max(amax);
         fine = __all_sync(0xffffffffu, fine);
@@ -346,57 +389,51 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
         // pairs of codes, packed to the lane's EPL bytes
         uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
 #pragma unroll
-        for (int i = 0; i < EPL; i += 2) {
-          const bool use = fine && r < nrows;
-          const float a = use ? x[i] * inv : 0.f, z = use && EPL > 1 ? x[EPL > 1 ? i + 1 : 0] * inv : 0.f;
+        for (int k = 0; k < EPL; k += 2) {
+          const float a = fine ? x[i][k] * inv : 0.f, z = fine && EPL > 1 ? x[i][EPL > 1 ? k + 1 : 0] * inv : 0.f;
           const uint16_t h = to_e4m3x2(a, z);
           const float2 f = from_e4m3x2(h);
-          hi[i / 4] |= (uint32_t)h << (i % 4 * 8);
-          lo[i / 4] |= (uint32_t)to_e4m3x2((a - f.x) * 16.f, (z - f.y) * 16.f) << (i % 4 * 8);
+          hi[k / 4] |= (uint32_t)h << (k % 4 * 8);
+          lo[k / 4] |= (uint32_t)to_e4m3x2((a - f.x) * 16.f, (z - f.y) * 16.f) << (k % 4 * 8);
         }
         const int byte = lane * EPL, cb = byte / CW, in = byte % CW;
-        uint8_t* dh = sQ + cb * (N * CW) + swz<CW>(r, in / 16) + in % 16;
-        uint8_t* dl = sQ + cb * (N * CW) + swz<CW>(R + r, in / 16) + in % 16;
-        store_bytes<EPL>(dh, hi[0], hi[1]);
-        store_bytes<EPL>(dl, lo[0], lo[1]);
+        store_bytes<EPL>(sQ + cb * (N * CW) + swz<CW>(r, in / 16) + in % 16, hi[0], hi[1]);
+        store_bytes<EPL>(sQ + cb * (N * CW) + swz<CW>(R + r, in / 16) + in % 16, lo[0], lo[1]);
         if (lane == 0) {
-          qs[r] = r < nrows ? (fine ? exp2i(e) * (L.scale * LOG2E) : NAN) : 0.f;
+          qs[r] = fine ? exp2i(e) * (L.scale * LOG2E) : NAN;
           mcur[r] = NOTHING;
         }
       }
       tc::fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(qfull);
+      asm volatile("barrier.cta.sync 15, %0;" ::"n"(C::SOFTMAX) : "memory");   // qs and mcur of all rows are written
 
-      // this thread's key: page one tile ahead of its scales, scales one tile ahead of their use
-      const long long key0 = (long long)p.j0 * TILE + key_in;
-      auto scales_of = [&](int page, long long key, float& ks, float& vs) {
-        ks = vs = 1.f;
-        if (page >= 0) {
-          const int64_t at = ((int64_t)page * L.n_kv_heads + p.g) * nb + (int)key % L.page_size / L.scale_block;
-          ks = L.k_scales[at];
-          vs = L.v_scales[at];
-        }
-      };
-      auto page_at = [&](int j) { return j < p.n ? page_of(L, p.b, key0 + (long long)j * TILE, kv_end) : -1; };
-      int page = page_at(0), page1 = page_at(1);
-      float ks, vs, ks1, vs1;
-      scales_of(page, key0, ks, vs);
-
-      float m[RW], l[RW];
+      float m[RW], l[RW], qr[RW];
 #pragma unroll
       for (int i = 0; i < RW; ++i) {
         m[i] = NOTHING;
         l[i] = 0.f;
+        qr[i] = qs[r0 + i];
       }
-      if (C::NWG == 2) asm volatile("barrier.cta.sync 3, 256;" ::: "memory");   // qs and mcur of all rows are written
-      else bar_sync(bar);
+      // last key that the first of all rows of this warpgroup sees
+      const int seen_by_all = base + (row0 + r0) / nrep;
 
       for (int j = 0; j < p.n; ++j, ++tile) {
         const uint32_t sb = tile & 1, ph = (tile >> 1) & 1;
-        const long long key = key0 + (long long)j * TILE;
-        scales_of(page1, key + TILE, ks1, vs1);
-        const int page2 = page_at(j + 2);
+        const int key = key0 + j * TILE;
+        scales_of(a1, ks1, vs1);
+        const At a2 = at(j + 2);
+        const bool mine = a0.page >= 0;   // the key exists
+        const float ve = (float)exp_of(vs) + BIAS, ivs = exp2i(-max(exp_of(vs), -126));
+        // rows that may see this key: all, but for missing keys and the tiles of the new tokens
+        uint32_t sees = mine ? 0xffffffffu : 0u;
+        if (mine && key > seen_by_all) {
+#pragma unroll
+          for (int i = 1; i < RW; ++i)
+            if (key > base + (row0 + r0 + i) / nrep) sees &= ~(1u << i);
+          sees &= ~1u;
+        }
         wait(&sfull[sb], ph);
         tc::fence_after();
         uint32_t sh[RW], sl[RW];
@@ -407,43 +444,33 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(&sempty[sb]);
 
-        const bool mine = page >= 0;   // the key exists
-        const float ve = (float)exp_of(vs) + BIAS, ivs = exp2i(-max(exp_of(vs), -126));
+        // d: exponents of the weights; scores times qr·ks are in log2 units
         float x[RW], d[RW];
-        // x: scores of the row in log2 units; causal limit only where a row may not see the whole tile
-        const long long tile_end = (long long)(p.j0 + j + 1) * TILE;
-        const bool edge = tile_end > base + row0 / nrep + 1;
-#pragma unroll
-        for (int i = 0; i < RW; ++i) x[i] = fmaf(__uint_as_float(sl[i]), 0.0625f, __uint_as_float(sh[i])) * (qs[r0 + i] * ks);
-        if (edge) {
-#pragma unroll
-          for (int i = 0; i < RW; ++i)
-            if (key > base + (row0 + r0 + i) / nrep) x[i] = -INFINITY;
-        }
-        if (!mine) {
-#pragma unroll
-          for (int i = 0; i < RW; ++i) x[i] = -INFINITY;
-        }
         float top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < RW; ++i) {
-          d[i] = x[i] + (ve - m[i]);
-          top = fmaxf(top, d[i]);
+          x[i] = fmaf(__uint_as_float(sl[i]), 0.0625f, __uint_as_float(sh[i]));
+          d[i] = fmaf(x[i], qr[i] * ks, ve - m[i]);
         }
+        if (sees != 0xffffffffu) {
+#pragma unroll
+          for (int i = 0; i < RW; ++i)
+            if (!(sees >> i & 1)) d[i] = -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < RW; ++i) top = fmaxf(top, d[i]);
         if (bar_any(bar, top > SLACK + BIAS)) {
           // raise the maxima to what they are, rescale l and O
           float y[RW];
 #pragma unroll
-          for (int i = 0; i < RW; ++i) y[i] = x[i] + (ve - BIAS);
+          for (int i = 0; i < RW; ++i) y[i] = sees >> i & 1 ? fmaf(x[i], qr[i] * ks, ve - BIAS) : -INFINITY;
           const float best = warp_transpose_reduce<RW, true>(y, lane);
-          if (lane % (32 / RW) == 0) red[(wg * 4 + wq) * RW + row_of<RW>(lane)] = best;
+          if (reducer) red[wg * 4 * RW + row_of<RW>(lane) * 4 + wq] = best;
           bar_sync(bar);
-          if (wq == 0 && lane % (32 / RW) == 0) {
-            float v = red[wg * 4 * RW + row_of<RW>(lane)];
-#pragma unroll
-            for (int k = 1; k < 4; ++k) v = fmaxf(v, red[(wg * 4 + k) * RW + row_of<RW>(lane)]);
+          if (wq == 0 && reducer) {
+            const float4 v = *reinterpret_cast<const float4*>(red + wg * 4 * RW + row_of<RW>(lane) * 4);
             const float was = mcur[my_row];
-            const float now = fmaxf(was, v);
+            const float now = fmaxf(was, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
             mcur[my_row] = now;
             aux[my_row] = ex2(was - now);
           }
@@ -452,7 +479,7 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
           for (int i = 0; i < RW; ++i) {
             m[i] = mcur[r0 + i];
             l[i] *= aux[r0 + i];
-            d[i] = x[i] + (ve - m[i]);
+            d[i] = sees >> i & 1 ? fmaf(x[i], qr[i] * ks, ve - m[i]) : -INFINITY;
           }
           if (j > 0) {
             const uint32_t t1 = tile - 1;
@@ -461,12 +488,12 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
 #pragma unroll 1
             for (int c = 0; c < CB * 2; ++c) {
               uint32_t o[RW];
-              const uint32_t at = tlane + 2 * N + (c >> 1) * N + (c & 1) * R + r0;
-              tm_ld<RW>(at, o);
+              const uint32_t where = tlane + 2 * N + (c >> 1) * N + (c & 1) * R + r0;
+              tm_ld<RW>(where, o);
               tm_wait_ld();
 #pragma unroll
               for (int i = 0; i < RW; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * aux[r0 + i]);
-              tm_st<RW>(at, o);
+              tm_st<RW>(where, o);
             }
             tm_wait_st();
             tc::fence_before();
@@ -493,21 +520,19 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
         // the buffer's previous product is done (tile - 2)
         wait(&pdone[sb], ph ^ 1u);
         uint8_t* pr = sP + sb * C::PB;
-        if constexpr (RW == 8) {
+        if constexpr (R == 8) {
           *reinterpret_cast<uint4*>(pr + key_in * 16) = make_uint4(hi[0], hi[1], lo[0], lo[1]);
+        } else if constexpr (RW == 8) {
+          *reinterpret_cast<uint2*>(pr + swz<N>(key_in, r0 / 16) + r0 % 16) = make_uint2(hi[0], hi[1]);
+          *reinterpret_cast<uint2*>(pr + swz<N>(key_in, (R + r0) / 16) + r0 % 16) = make_uint2(lo[0], lo[1]);
         } else {
-#pragma unroll
-          for (int k = 0; k < RW / 16; ++k) {
-            *reinterpret_cast<uint4*>(pr + swz<N>(key_in, r0 / 16 + k)) = make_uint4(hi[4 * k], hi[4 * k + 1], hi[4 * k + 2], hi[4 * k + 3]);
-            *reinterpret_cast<uint4*>(pr + swz<N>(key_in, R / 16 + r0 / 16 + k)) =
-                make_uint4(lo[4 * k], lo[4 * k + 1], lo[4 * k + 2], lo[4 * k + 3]);
-          }
+          *reinterpret_cast<uint4*>(pr + swz<N>(key_in, r0 / 16)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          *reinterpret_cast<uint4*>(pr + swz<N>(key_in, (R + r0) / 16)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
         if (!mine && wg == 0) {
           // a key that is not there: its value row is whatever lies in the slot, and 0·NaN is NaN
-          const uint32_t vi = ring0 + (j == p.n - 1 ? 2 * p.n - 1 : 2 * j + 2);
-          wait(&full[vi % NS], (vi / NS) & 1u);
-          uint8_t* v = ring + vi % NS * C::SLOT + key_in * CW;
+          wait(&vfull[tile % NSV], (tile / NSV) & 1u);
+          uint8_t* v = sV + tile % NSV * C::SLOT + key_in * CW;
 #pragma unroll
           for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
@@ -516,60 +541,55 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
         tc::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(&pfull[sb]);
-        page = page1;
-        page1 = page2;
+        a0 = a1;
+        a1 = a2;
         ks = ks1;
         vs = vs1;
       }
-      ring0 += 2 * p.n;
 
       // ---- the piece is done: l over the keys, O out of TMEM (thread = head dim)
-      {
-        const float s = warp_transpose_reduce<RW, false>(l, lane);
-        if (lane % (32 / RW) == 0) red[(wg * 4 + wq) * RW + row_of<RW>(lane)] = s;
-        const uint32_t t1 = tile - 1;
-        wait(&pdone[t1 & 1], (t1 >> 1) & 1);
-        tc::fence_after();
-        bar_sync(bar);
-        const bool whole = p.whole();
-        if (wq == 0 && lane % (32 / RW) == 0) {
-          float v = 0.f;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) v += red[(wg * 4 + k) * RW + row_of<RW>(lane)];
-          aux[my_row] = v == 0.f ? 0.f : 1.f / v;
-          if (!whole) ws.ml[(int64_t)p.slot() * R + my_row] = make_float2(v == 0.f ? -INFINITY : mcur[my_row], v);
-        }
-        bar_sync(bar);
+      const float s = warp_transpose_reduce<RW, false>(l, lane);
+      if (reducer) red[wg * 4 * RW + row_of<RW>(lane) * 4 + wq] = s;
+      const uint32_t t1 = tile - 1;
+      wait(&pdone[t1 & 1], (t1 >> 1) & 1);
+      tc::fence_after();
+      bar_sync(bar);
+      const bool whole = p.whole();
+      if (wq == 0 && reducer) {
+        const float4 v4 = *reinterpret_cast<const float4*>(red + wg * 4 * RW + row_of<RW>(lane) * 4);
+        const float v = (v4.x + v4.y) + (v4.z + v4.w);
+        aux[my_row] = v == 0.f ? 0.f : 1.f / v;
+        if (!whole) ws.ml[(int64_t)p.slot() * R + my_row] = make_float2(v == 0.f ? -INFINITY : mcur[my_row], v);
+      }
+      bar_sync(bar);
 #pragma unroll 1
-        for (int mb = 0; mb < CB; ++mb) {
-          uint32_t oh[RW], ol[RW];
-          tm_ld<RW>(tlane + 2 * N + mb * N + r0, oh);
-          tm_ld<RW>(tlane + 2 * N + mb * N + R + r0, ol);
-          tm_wait_ld();
-          const int dim = mb * 128 + key_in;
-          if (dim < HD) {
-            if (whole) {
+      for (int mb = 0; mb < CB; ++mb) {
+        uint32_t oh[RW], ol[RW];
+        tm_ld<RW>(tlane + 2 * N + mb * N + r0, oh);
+        tm_ld<RW>(tlane + 2 * N + mb * N + R + r0, ol);
+        tm_wait_ld();
+        const int dim = mb * 128 + key_in;
+        if (dim < HD) {
+          if (whole) {
 #pragma unroll
-              for (int i = 0; i < RW; ++i) {
-                if (r0 + i < nrows) {
-                  const int rr = row0 + r0 + i, t = rr / nrep, hq = p.g * nrep + rr % nrep;
-                  const int64_t mrow = (int64_t)p.b * L.tokens + t;
-                  const float gate = __bfloat162float(static_cast<const __nv_bfloat16*>(L.qkv)[mrow * L.ld_qkv + (int64_t)hq * 2 * HD + HD + dim]);
-                  const float o = fmaf(__uint_as_float(ol[i]), 0.0625f, __uint_as_float(oh[i])) * aux[r0 + i];
-                  static_cast<__nv_bfloat16*>(L.out)[mrow * L.ld_out + (int64_t)hq * HD + dim] = __float2bfloat16_rn(o * sigmoidf_(gate));
-                }
+            for (int i = 0; i < RW; ++i) {
+              if (r0 + i < nrows) {
+                const int rr = row0 + r0 + i, t = rr / nrep, hq = p.g * nrep + rr - t * nrep;
+                const int64_t mrow = (int64_t)p.b * L.tokens + t;
+                const float gate = __bfloat162float(static_cast<const __nv_bfloat16*>(L.qkv)[mrow * L.ld_qkv + (int64_t)hq * 2 * HD + HD + dim]);
+                const float o = fmaf(__uint_as_float(ol[i]), 0.0625f, __uint_as_float(oh[i])) * aux[r0 + i];
+                static_cast<__nv_bfloat16*>(L.out)[mrow * L.ld_out + (int64_t)hq * HD + dim] = __float2bfloat16_rn(o * sigmoidf_(gate));
               }
-            } else {
-              float* o = ws.o + ((int64_t)p.slot() * R + r0) * HD + dim;
-#pragma unroll
-              for (int i = 0; i < RW; ++i) o[i * HD] = fmaf(__uint_as_float(ol[i]), 0.0625f, __uint_as_float(oh[i]));
             }
+          } else {
+            float* o = ws.o + ((int64_t)p.slot() * R + r0) * HD + dim;
+#pragma unroll
+            for (int i = 0; i < RW; ++i) o[i * HD] = fmaf(__uint_as_float(ol[i]), 0.0625f, __uint_as_float(oh[i]));
           }
         }
-        tc::fence_before();   // the next piece's products overwrite O after its pfull
-        bar_sync(bar);        // aux, qs: written again for the next piece
-        if (C::NWG == 2) asm volatile("barrier.cta.sync 3, 256;" ::: "memory");
       }
+      tc::fence_before();   // the next piece's products overwrite O after its pfull
+      asm volatile("barrier.cta.sync 15, %0;" ::"n"(C::SOFTMAX) : "memory");   // qs, mcur, aux are written again
     }
     if (tid == 0) put_meta(ws, w, p);
   }
@@ -595,7 +615,7 @@ static bool make_map(CUtensorMap* m, const void* base, int64_t rows, int hd, int
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int tc_grid(int hd, int R) { return tc::sm_count() * (hd == 256 || R == 64 ? 1 : 2); }
+int tc_grid(int hd, int R) { return tc::sm_count() * (hd == 256 || R >= 32 ? 1 : 2); }
 
 // the least R that holds all query rows of a kv head, so that each key is read once; 64 at most
 int tc_rows(int rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
