@@ -53,11 +53,12 @@ struct Cfg {
   static constexpr int BUDGET = OCC == 1 ? 232448 : 115712;
   // barriers, row scales, row maxima, reduction buffer
   static constexpr int SMALL = 8 * 28 + 4 * (R + 2 * R + 4 * R) + 16;
-  static constexpr int FIT = (BUDGET - 1024 - SMALL - QB - 2 * PB) / SLOT;
+  static constexpr int FIT = (BUDGET - SMALL - 6 * 2 * TILE - QB - 2 * PB) / SLOT;
   static constexpr int NS = FIT < 8 ? FIT : 8;              // ring slots
   static constexpr int NSV = (NS + 1) / 2, NSK = NS - NSV;  // a V tile waits for its weights, a K tile does not
-  static constexpr size_t BYTES = 1024 + (size_t)NS * SLOT + QB + 2 * PB + SMALL;
-  static constexpr int SOFTMAX = 128 * NWG, THREADS = SOFTMAX + 96;
+  static constexpr int NSE = NSK + 2;                       // slots of scale exponents
+  static constexpr size_t BYTES = (size_t)NS * SLOT + QB + 2 * PB + SMALL + NSE * 2 * TILE;
+  static constexpr int SOFTMAX = 128 * NWG, THREADS = SOFTMAX + 128;
   static constexpr int COLS_USED = 2 * N + CB * N;
   static constexpr int COLS = COLS_USED <= 64 ? 64 : COLS_USED <= 128 ? 128 : COLS_USED <= 256 ? 256 : 512;
   static_assert(NSK >= 2, "ring too short");
@@ -169,12 +170,7 @@ __device__ __forceinline__ int row_of(int lane) {
   return lane / (32 / RW);
 }
 
-// page of a key's position, or -1
-__device__ __forceinline__ int page_of(const qsp_attn_kv8_layer& L, int b, int key, int kv_end) {
-  if (key >= kv_end) return -1;
-  const int page = L.page_table[(int64_t)b * L.max_pages + key / L.page_size];
-  return page >= 0 && page < L.num_pages ? page : -1;
-}
+constexpr uint32_t MISSING = 0xffffu;   // scale exponents of a key that has no page
 
 template <int HD, int R_>
 __global__ void __launch_bounds__(Cfg<HD, R_>::THREADS, Cfg<HD, R_>::OCC)
@@ -183,8 +179,7 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
   using C = Cfg<HD, R_>;
   constexpr int R = C::R, N = C::N, RW = C::RW, NWG = C::NWG, NSK = C::NSK, NSV = C::NSV, CW = C::CW, CB = C::CB, EPL = HD / 32;
   pdl_trigger();
-  extern __shared__ uint8_t raw[];
-  uint8_t* sK = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t sK[];                // the swizzles go by address: 1024-byte tiles
   uint8_t* sV = sK + NSK * C::SLOT;
   uint8_t* sQ = sV + NSV * C::SLOT;
   uint8_t* sP = sQ + C::QB;                                      // [2][128 keys][N]
@@ -203,12 +198,13 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
   float* aux = mcur + R;                              // [R] rescaling factor; 1 / l at the end
   float* red = aux + R;                               // [NWG][4][RW]
   volatile int* abort = reinterpret_cast<volatile int*>(red + 4 * R);
+  uint16_t* sE = reinterpret_cast<uint16_t*>(red + 4 * R + 4);   // [NSE][128] a key's scale exponents + 127: K low, V high byte
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  constexpr int W_K = 4 * NWG, W_V = W_K + 1, W_MMA = W_K + 2;
+  constexpr int W_K = 4 * NWG, W_V = W_K + 1, W_E = W_K + 2, W_MMA = W_K + 3;
   const int nrep = L.n_heads / L.n_kv_heads, rows_total = nrep * L.tokens;
 
   if (tid == 0) {
-    for (int i = 0; i < 2 * C::NS; ++i) tc::mbar_init(&kfull[i], 1);   // kfull, kempty, vfull, vempty
+    for (int i = 0; i < 2 * C::NS; ++i) tc::mbar_init(&kfull[i], i < NSK ? 2 : 1);   // kfull (K and its scales), kempty, vfull, vempty
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(&sfull[i], 1);
       tc::mbar_init(&sempty[i], 4 * NWG);
@@ -250,14 +246,15 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
     uint32_t turn = 1;   // parity of "empty" for this turn of the ring
     while (next_piece(L, n_rg, R, w, p)) {
       const int kv_end = kv_end_of(base_of(p.b));
-      auto row_at = [&](int j) -> int {   // row of the pages' [pages·n_kv·page_size, hd] view, or -1
-        const int key = (p.j0 + j) * TILE + lane % chunks * box_rows;
-        const int page = j < p.n && lane < boxes ? page_of(L, p.b, key, kv_end) : -1;
-        return page < 0 ? -1 : (page * L.n_kv_heads + p.g) * L.page_size + key % L.page_size;
-      };
-      int row = row_at(0);
+      const int32_t* pages = L.page_table + (int64_t)p.b * L.max_pages;
+      int key = p.j0 * TILE + lane % chunks * box_rows;
+      auto page_at = [&](int j) { return j < p.n && lane < boxes && key < kv_end ? pages[key / L.page_size] : -1; };
+      int page = page_at(0);
       for (int j = 0; j < p.n; ++j) {
-        const int next = row_at(j + 1);
+        // row of the pages' [pages·n_kv·page_size, hd] view, or -1
+        const int row = page >= 0 && page < L.num_pages ? (page * L.n_kv_heads + p.g) * L.page_size + key % L.page_size : -1;
+        key += TILE;
+        page = page_at(j + 1);
         wait(&empty[slot], turn);
         const uint32_t there = __ballot_sync(0xffffffffu, row >= 0);
         tc::mbar_expect_tx_warp(&full[slot], __popc(there) * box_rows * CW);
@@ -269,11 +266,57 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
             tc::tma_load_2d_warp(dst + cb * (TILE * CW) + (i - cb * chunks) * (box_rows * CW), map, &full[slot], cb * CW, r);
           }
         }
-        row = next;
         if (++slot == slots) {
           slot = 0;
           turn ^= 1u;
         }
+      }
+    }
+  } else if (warp == W_E) {
+    // ---------------- scale exponents of a tile's keys, 4 a lane, in step with the K ring: pages are loaded two
+    // tiles ahead, scales one. A slot is free when QK of the tile NSK before this one is done: that product was
+    // issued after the scores of the tile NSE before, and so its scales, had been read.
+    const int nb = L.page_size / L.scale_block, sb_log = __ffs(L.scale_block) - 1;
+    uint32_t tile = 0;
+    while (next_piece(L, n_rg, R, w, p)) {
+      const int kv_end = kv_end_of(base_of(p.b));
+      const int32_t* pages = L.page_table + (int64_t)p.b * L.max_pages;
+      int page[4], slot[4];      // of tile j + 1, then j + 2
+      float ks[4], vs[4];        // of tile j
+      bool here[4];
+      auto pages_at = [&](int j) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = (p.j0 + j) * TILE + i * 32 + lane;
+          const int lp = key / L.page_size;
+          slot[i] = key - lp * L.page_size;
+          page[i] = j < p.n && key < kv_end ? pages[lp] : -1;
+        }
+      };
+      auto scales_at = [&]() {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          here[i] = page[i] >= 0 && page[i] < L.num_pages;
+          const int64_t at = here[i] ? ((int64_t)page[i] * L.n_kv_heads + p.g) * nb + (slot[i] >> sb_log) : 0;
+          ks[i] = L.k_scales[at];
+          vs[i] = L.v_scales[at];
+        }
+      };
+      pages_at(0);
+      scales_at();
+      pages_at(1);
+      for (int j = 0; j < p.n; ++j, ++tile) {
+        const int s = tile % NSK;
+        wait(&kempty[s], ((tile / NSK) & 1u) ^ 1u);
+        uint16_t* e = sE + tile % C::NSE * TILE;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          e[i * 32 + lane] = here[i] ? (uint16_t)((__float_as_uint(ks[i]) >> 23 & 0xffu) | (__float_as_uint(vs[i]) >> 23 & 0xffu) << 8)
+                                     : (uint16_t)MISSING;
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&kfull[s]);
+        scales_at();
+        pages_at(j + 2);
       }
     }
   } else if (warp == W_MMA) {
@@ -328,33 +371,11 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
     const uint32_t tlane = tmem + ((uint32_t)(wq * 32) << 16);
     const int my_row = r0 + row_of<RW>(lane);
     const bool reducer = lane % (32 / RW) == 0;    // its lane of a row's reduction
-    const int nb = L.page_size / L.scale_block, sb_log = __ffs(L.scale_block) - 1;
     uint32_t tile = 0;
     while (next_piece(L, n_rg, R, w, p)) {
       const int row0 = p.rg * R, nrows = min(R, rows_total - row0);
-      const int base = base_of(p.b), kv_end = kv_end_of(base);
-      // this thread's key: page and slot one tile ahead of its scales, scales one tile ahead of their use
+      const int base = base_of(p.b);
       const int key0 = p.j0 * TILE + key_in;
-      struct At {
-        int page, blk;
-      };
-      auto at = [&](int j) -> At {
-        const int key = key0 + j * TILE;
-        if (j >= p.n || key >= kv_end) return {-1, 0};
-        const int lp = key / L.page_size;
-        const int page = L.page_table[(int64_t)p.b * L.max_pages + lp];
-        return {page >= 0 && page < L.num_pages ? page : -1, (key - lp * L.page_size) >> sb_log};
-      };
-      auto scales_of = [&](At a, float& ks, float& vs) {
-        ks = vs = 1.f;
-        if (a.page >= 0) {
-          const int64_t i = ((int64_t)a.page * L.n_kv_heads + p.g) * nb + a.blk;
-          ks = L.k_scales[i];
-          vs = L.v_scales[i];
-        }
-      };
-      At a0 = at(0), a1 = at(1);
-      float ks, vs, ks1, vs1;
 
       // stage Q: a warp per row, hi at row r and lo at row R + r of the swizzled tile
       constexpr int ROWS = R / (4 * NWG);
@@ -371,7 +392,6 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
           for (int k = 0; k < EPL; ++k) x[i][k] = 0.f;
         }
       }
-      scales_of(a0, ks, vs);
 #pragma unroll
       for (int i = 0; i < ROWS; ++i) {
         const int r = warp + i * 4 * NWG;
@@ -409,23 +429,27 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
       if (lane == 0) tc::mbar_arrive(qfull);
       asm volatile("barrier.cta.sync 15, %0;" ::"n"(C::SOFTMAX) : "memory");   // qs and mcur of all rows are written
 
-      float m[RW], l[RW], qr[RW];
+      float m[RW], l[RW], qr[RW == 8 ? 8 : 1];
 #pragma unroll
       for (int i = 0; i < RW; ++i) {
         m[i] = NOTHING;
         l[i] = 0.f;
-        qr[i] = qs[r0 + i];
+        if (RW == 8) qr[i] = qs[r0 + i];
       }
+      auto q_scale = [&](int i) { return RW == 8 ? qr[i] : qs[r0 + i]; };   // 16 rows: registers are short
       // last key that the first of all rows of this warpgroup sees
       const int seen_by_all = base + (row0 + r0) / nrep;
 
       for (int j = 0; j < p.n; ++j, ++tile) {
         const uint32_t sb = tile & 1, ph = (tile >> 1) & 1;
         const int key = key0 + j * TILE;
-        scales_of(a1, ks1, vs1);
-        const At a2 = at(j + 2);
-        const bool mine = a0.page >= 0;   // the key exists
-        const float ve = (float)exp_of(vs) + BIAS, ivs = exp2i(-max(exp_of(vs), -126));
+        wait(&sfull[sb], ph);
+        tc::fence_after();
+        uint32_t ev = sE[tile % C::NSE * TILE + key_in];
+        const bool mine = ev != MISSING;   // the key exists
+        if (!mine) ev = 127u << 8 | 127u;
+        const float ks = __uint_as_float((ev & 0xffu) << 23);
+        const float ve = (float)(int)(ev >> 8) - (127.f - BIAS), ivs = exp2i(127 - max((int)(ev >> 8), 1));
         // rows that may see this key: all, but for missing keys and the tiles of the new tokens
         uint32_t sees = mine ? 0xffffffffu : 0u;
         if (mine && key > seen_by_all) {
@@ -434,8 +458,6 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
             if (key > base + (row0 + r0 + i) / nrep) sees &= ~(1u << i);
           sees &= ~1u;
         }
-        wait(&sfull[sb], ph);
-        tc::fence_after();
         uint32_t sh[RW], sl[RW];
         tm_ld<RW>(tlane + sb * N + r0, sh);
         tm_ld<RW>(tlane + sb * N + R + r0, sl);
@@ -450,7 +472,7 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
 #pragma unroll
         for (int i = 0; i < RW; ++i) {
           x[i] = fmaf(__uint_as_float(sl[i]), 0.0625f, __uint_as_float(sh[i]));
-          d[i] = fmaf(x[i], qr[i] * ks, ve - m[i]);
+          d[i] = fmaf(x[i], q_scale(i) * ks, ve - m[i]);
         }
         if (sees != 0xffffffffu) {
 #pragma unroll
@@ -463,7 +485,7 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
           // raise the maxima to what they are, rescale l and O
           float y[RW];
 #pragma unroll
-          for (int i = 0; i < RW; ++i) y[i] = sees >> i & 1 ? fmaf(x[i], qr[i] * ks, ve - BIAS) : -INFINITY;
+          for (int i = 0; i < RW; ++i) y[i] = sees >> i & 1 ? fmaf(x[i], q_scale(i) * ks, ve - BIAS) : -INFINITY;
           const float best = warp_transpose_reduce<RW, true>(y, lane);
           if (reducer) red[wg * 4 * RW + row_of<RW>(lane) * 4 + wq] = best;
           bar_sync(bar);
@@ -479,7 +501,7 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
           for (int i = 0; i < RW; ++i) {
             m[i] = mcur[r0 + i];
             l[i] *= aux[r0 + i];
-            d[i] = sees >> i & 1 ? fmaf(x[i], qr[i] * ks, ve - m[i]) : -INFINITY;
+            d[i] = sees >> i & 1 ? fmaf(x[i], q_scale(i) * ks, ve - m[i]) : -INFINITY;
           }
           if (j > 0) {
             const uint32_t t1 = tile - 1;
@@ -517,8 +539,7 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
             lo[i / 4] |= (uint32_t)q << 16;
           }
         }
-        // the buffer's previous product is done (tile - 2)
-        wait(&pdone[sb], ph ^ 1u);
+        // (the buffer's previous product, of tile - 2, was issued before QK of this tile and so is done)
         uint8_t* pr = sP + sb * C::PB;
         if constexpr (R == 8) {
           *reinterpret_cast<uint4*>(pr + key_in * 16) = make_uint4(hi[0], hi[1], lo[0], lo[1]);
@@ -541,10 +562,6 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
         tc::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(&pfull[sb]);
-        a0 = a1;
-        a1 = a2;
-        ks = ks1;
-        vs = vs1;
       }
 
       // ---- the piece is done: l over the keys, O out of TMEM (thread = head dim)
