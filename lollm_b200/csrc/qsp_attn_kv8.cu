@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(SIMT_THREADS) simt_kernel(const qsp_attn_kv8_l
   pdl_wait();
   constexpr int DPL = HD / 32, RPW = SIMT_R / 4;
   extern __shared__ float smem[];
-  __shared__ long long sh[34];
+  __shared__ int sh[36];
   float* Qs = smem;                       // [16][HD]
   float* Ks = Qs + SIMT_R * HD;           // [32][HD + 1]
   float* Vs = Ks + SIMT_KT * (HD + 1);    // [32][HD]
@@ -361,64 +361,81 @@ static int launch_simt(const qsp_attn_kv8_layer& L, int G, cudaStream_t st) {
 }
 
 // ------------------------------------------------------------------ merge of divided units
-// CTA (c, r): row r of the divided unit that begins in the share of attention CTA c, if one does.
-// Its partials are weighted with 2^(m_p − M), summed in their order (groups of hd/4 threads take every
-// 256/(hd/4)-th partial, the groups' sums are then added in order), divided by l and gated.
+// CTA (c, y): rows 4y..4y+3 of the divided unit whose first tile attention CTA c had, if there is one; two
+// warps a row. Each warp weights its half of the partials with 2^(m_p − M) and adds them in their order,
+// a lane HD/32 columns; the halves are added, divided by l and gated. Latency-bound: eight partials
+// are in flight at a time.
+constexpr int MERGE_ROWS = 4;
+
 template <typename T, int HD>
-__global__ void __launch_bounds__(256) merge_kernel(const qsp_attn_kv8_layer L, int G, int R) {
+__global__ void __launch_bounds__(64 * MERGE_ROWS) merge_kernel(const qsp_attn_kv8_layer L, int G, int R) {
   pdl_trigger();
   pdl_wait();
-  constexpr int TPP = HD / 4, NG = 256 / TPP;
-  __shared__ float4 part[256];
-  __shared__ float lpart[NG];
+  constexpr int EPL = HD / 32, DEPTH = 8;
+  __shared__ float half[MERGE_ROWS][HD + 1];
   const Scratch ws = scratch(L, G, R);
   const int4 meta = ws.meta[blockIdx.x];
-  const int np = meta.w, r = blockIdx.y;
+  const int np = meta.w;
   if (np == 0) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = warp >> 1, h = warp & 1;
+  const int r = blockIdx.y * MERGE_ROWS + row;
   const int nrep = L.n_heads / L.n_kv_heads, rr = meta.y * R + r;
-  if (rr >= nrep * L.tokens) return;
-  const int c = blockIdx.x, lane = threadIdx.x & 31;
-  const int first = 2 * c + (meta.z >> 30);
+  const bool live = r < R && rr < nrep * L.tokens;
+  const int c = blockIdx.x, first = 2 * c + (meta.z >> 30), mid = (np + 1) / 2;
   auto slot = [&](int q) { return (int64_t)(q == 0 ? first : 2 * (c + q)) * R + r; };
-  float M = -INFINITY;
-  for (int q = lane; q < np; q += 32) M = fmaxf(M, ws.ml[slot(q)].x);
-  M = warp_max(M);
-  const float ref = M == -INFINITY ? 0.f : M;
-  const int grp = threadIdx.x / TPP, col = threadIdx.x % TPP;
-  float4 acc = {0, 0, 0, 0};
-  float den = 0.f;
-#pragma unroll 4
-  for (int q = grp; q < np; q += NG) {
-    const float2 ml = ws.ml[slot(q)];
-    const float4 v = *reinterpret_cast<const float4*>(ws.o + slot(q) * HD + 4 * col);
-    const float f = exp2f(ml.x - ref);
-    if (ml.y != 0.f) {   // a part of which the row saw nothing
-      den = fmaf(f, ml.y, den);
-      acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
+  float acc[EPL], den = 0.f;
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) acc[i] = 0.f;
+  if (live) {
+    float M = -INFINITY;
+    for (int q = lane; q < np; q += 32) M = fmaxf(M, ws.ml[slot(q)].x);
+    M = warp_max(M);
+    const float ref = M == -INFINITY ? 0.f : M;
+    const int q1 = h ? np : mid;
+    for (int q0 = h ? mid : 0; q0 < q1; q0 += DEPTH) {
+      float v[DEPTH][EPL];
+      float2 ml[DEPTH];
+#pragma unroll
+      for (int u = 0; u < DEPTH; ++u) {
+        if (q0 + u < q1) {
+          ml[u] = ws.ml[slot(q0 + u)];
+          load_row<float, EPL>(ws.o + slot(q0 + u) * HD, lane, true, v[u]);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < DEPTH; ++u) {
+        if (q0 + u < q1 && ml[u].y != 0.f) {   // else a part of which the row saw nothing
+          const float f = exp2f(ml[u].x - ref);
+          den = fmaf(f, ml[u].y, den);
+#pragma unroll
+          for (int i = 0; i < EPL; ++i) acc[i] = fmaf(f, v[u][i], acc[i]);
+        }
+      }
+    }
+    if (h) {
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) half[row][lane * EPL + i] = acc[i];
+      if (lane == 0) half[row][HD] = den;
     }
   }
-  part[threadIdx.x] = acc;
-  if (col == 0) lpart[grp] = den;
   __syncthreads();
-  if (threadIdx.x < HD) {
-    const int d = threadIdx.x, t = rr / nrep, hq = (meta.z & ((1 << 30) - 1)) * nrep + rr % nrep;
-    float s = 0.f, l = 0.f;
+  if (!live || h) return;
+  den += half[row][HD];
+  const int t = rr / nrep, hq = (meta.z & ((1 << 30) - 1)) * nrep + rr - t * nrep;
+  const int64_t m = (int64_t)meta.x * L.tokens + t;
+  const T* gate = static_cast<const T*>(L.qkv) + m * L.ld_qkv + (int64_t)hq * 2 * HD + HD + lane * EPL;
+  T* out = static_cast<T*>(L.out) + m * L.ld_out + (int64_t)hq * HD + lane * EPL;
 #pragma unroll
-    for (int q = 0; q < NG; ++q) {
-      s += reinterpret_cast<const float*>(part)[q * HD + d];
-      l += lpart[q];
-    }
-    const int64_t m = (int64_t)meta.x * L.tokens + t;
-    const T* gate = static_cast<const T*>(L.qkv) + m * L.ld_qkv + (int64_t)hq * 2 * HD + HD;
-    const float v = l == 0.f ? 0.f : s / l;
-    static_cast<T*>(L.out)[m * L.ld_out + (int64_t)hq * HD + d] = dt<T>::from_f(v * sigmoidf_(dt<T>::to_f(gate[d])));
+  for (int i = 0; i < EPL; ++i) {
+    const float v = den == 0.f ? 0.f : (acc[i] + half[row][lane * EPL + i]) / den;
+    out[i] = dt<T>::from_f(v * sigmoidf_(dt<T>::to_f(gate[i])));
   }
 }
 
 template <typename T>
 static int launch_merge_t(const qsp_attn_kv8_layer& L, int G, int R, cudaStream_t st) {
   const int rows = std::min(R, L.n_heads / L.n_kv_heads * L.tokens);
-  const dim3 grid(G, rows), block(256);
+  const dim3 grid(G, (rows + MERGE_ROWS - 1) / MERGE_ROWS), block(64 * MERGE_ROWS);
   switch (L.head_dim) {
     case 32: return launch_pdl("qsp_attn_kv8_verify(merge)", merge_kernel<T, 32>, grid, block, 0, st, L, G, R);
     case 64: return launch_pdl("qsp_attn_kv8_verify(merge)", merge_kernel<T, 64>, grid, block, 0, st, L, G, R);
@@ -451,6 +468,9 @@ static int validate(const char* what, const qsp_attn_kv8_layer* p, bool verify) 
   QSP_REQUIRE(L.scale_block > 0 && L.scale_block <= 64 && (L.scale_block & (L.scale_block - 1)) == 0 &&
                   L.page_size % L.scale_block == 0,
               "%s: scale_block %d must be a power of two up to 64 that divides the page size %d", what, L.scale_block, L.page_size);
+  const int64_t q_rows = (int64_t)L.n_heads / L.n_kv_heads * L.tokens;
+  QSP_REQUIRE((double)L.batch * L.n_kv_heads * (q_rows / 8 + 1) * ((int64_t)L.max_pages * L.page_size / kv8::TILE + 4) < 2e9,
+              "%s: more than 2^31 tiles of keys", what);
   QSP_REQUIRE(aligned(L.k_pages, 16) && aligned(L.v_pages, 16) && aligned(L.q_buf, 16), "%s: pages and q_buf must be 16-byte aligned",
               what);
   QSP_REQUIRE(L.ld_qkv >= (2ll * L.n_heads + 2ll * L.n_kv_heads) * L.head_dim, "%s: ld_qkv too small", what);

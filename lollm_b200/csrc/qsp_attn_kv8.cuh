@@ -90,10 +90,13 @@ __device__ __forceinline__ int exp_of(float scale) { return ((__float_as_int(sca
 // A unit is (sequence b, row group rg, kv head g): `R` query rows (t, q head of the group) against
 // the keys the last of them sees, cut into tiles of 128 keys. The tiles of all units, in the
 // order b, rg, g, are divided evenly over the CTAs, so a ragged batch, one long sequence and many
-// short ones all keep every SM equally busy. A CTA's share is a run of pieces (parts of units).
-// A piece that is a whole unit is written out by its CTA; the others leave a partial (o, m, l)
-// in the workspace: slot 2c for the first piece of CTA c, 2c + 1 for its last. The CTA in whose
-// share a divided unit begins describes it in meta[c] for the merge kernel.
+// short ones all keep every SM equally busy. Beginning a unit counts as UNIT_COST tiles (queries in,
+// output out). A CTA's share is a run of pieces (parts of units). A piece that is a whole unit is
+// written out by its CTA; the others leave a partial (o, m, l) in the workspace: slot 2c for the
+// first piece of CTA c, 2c + 1 for its last. The CTA that has the first tile of a divided unit
+// describes it in meta[c] for the merge kernel.
+constexpr int UNIT_COST = 2;
+
 struct Piece {
   int b, rg, g;
   int j0, n;        // first tile and tiles of this piece
@@ -103,88 +106,109 @@ struct Piece {
   __device__ __forceinline__ int slot() const { return 2 * (int)blockIdx.x + (first ? 0 : 1); }
 };
 
-__device__ __forceinline__ int unit_tiles(const qsp_attn_kv8_layer& L, int i, int n_rg, int R) {
-  const int b = i / n_rg, rg = i - b * n_rg;
-  const int nrep = L.n_heads / L.n_kv_heads;
-  const int t_last = min(L.tokens - 1, ((rg + 1) * R - 1) / nrep);
-  const long long cap = (long long)L.max_pages * L.page_size;
-  const long long kv = min((long long)L.seq_lens[b] + t_last + 1, cap);
-  return kv <= TILE ? 1 : (int)((kv + TILE - 1) / TILE);   // a unit without keys has a tile too: it writes zeros
+__device__ __forceinline__ int unit_tiles(const qsp_attn_kv8_layer& L, int b, int rg, int n_rg, int R) {
+  const int t_last = rg == n_rg - 1 ? L.tokens - 1 : ((rg + 1) * R - 1) / (L.n_heads / L.n_kv_heads);
+  const int cap = L.max_pages * L.page_size;
+  const int kv = min(min(L.seq_lens[b], cap) + t_last + 1, cap);
+  return kv <= TILE ? 1 : (kv + TILE - 1) / TILE;   // a unit without keys has a tile too: it writes zeros
 }
 
+// Positions count UNIT_COST + tiles for each unit; the host has checked that all fit 31 bits.
 struct Walk {
-  int i, g, j0;         // unit (i = b·n_rg + rg, g) and the tile in it to go on at
-  long long pos;                 // that tile's number among all tiles
-  long long begin, end;          // this CTA's share
-  long long total, parts;        // tiles of all units, and the CTAs that share them
+  int b, rg, g;       // unit to go on at
+  int at;             // position in that unit
+  int pos, end;       // the same position among all, and the end of this CTA's share
+  int total, parts;   // of all units, and the CTAs that share them
+  bool first;
 };
+__device__ __forceinline__ int share_begin(int c, int total, int parts) {
+  const int q = total / parts, r = total - q * parts;
+  return c * q + min(c, r);
+}
+__device__ __forceinline__ int share_owner(int pos, int total, int parts) {
+  const int q = total / parts, r = total - q * parts;
+  return pos < r * (q + 1) ? pos / (q + 1) : r + (pos - r * (q + 1)) / q;
+}
 
-// This CTA's share, found by all threads of the CTA; `sh` holds 34 long longs of shared memory.
-// Begins and ends with a __syncthreads.
-__device__ __forceinline__ Walk share(const qsp_attn_kv8_layer& L, int n_rg, int R, long long* sh) {
+// This CTA's share, found by all threads of the CTA; `sh` holds 36 ints of shared memory. Ends with
+// a __syncthreads.
+__device__ __forceinline__ Walk share(const qsp_attn_kv8_layer& L, int n_rg, int R, int* sh) {
   const int n = L.batch * n_rg, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
-  long long s = 0;
-  for (int i = tid; i < n; i += blockDim.x) s += unit_tiles(L, i, n_rg, R);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  __syncthreads();
+  auto cost = [&](int i) {
+    const int b = n_rg == 1 ? i : i / n_rg;
+    return UNIT_COST + unit_tiles(L, b, i - b * n_rg, n_rg, R);
+  };
+  int s = 0;
+  for (int i = tid; i < n; i += blockDim.x) s += cost(i);
+  s = __reduce_add_sync(0xffffffffu, s);
   if (lane == 0) sh[warp] = s;
   __syncthreads();
-  long long all = 0;
-  for (int w = 0; w < nw; ++w) all += sh[w];
-  all *= L.n_kv_heads;
-  const long long parts = min((long long)gridDim.x, all);   // no more CTAs than tiles: every one of them has some
-  const long long begin = min((long long)blockIdx.x, parts) * all / parts;
-  const long long end = min((long long)blockIdx.x + 1, parts) * all / parts;
+  int total = lane < nw ? sh[lane] : 0;
+  total = __reduce_add_sync(0xffffffffu, total) * L.n_kv_heads;
+  const int parts = min((int)gridDim.x, total);   // no more CTAs than tiles: every one of them has some
+  const int c = min((int)blockIdx.x, parts);
+  const int begin = share_begin(c, total, parts), end = share_begin(min(c + 1, parts), total, parts);
   if (warp == 0) {
-    long long before = 0;   // tiles of one kv head in the units before i0
+    int before = 0;   // positions of the units before i0
     for (int i0 = 0; i0 < n; i0 += 32) {
       const int i = i0 + lane;
-      const int mine = i < n ? unit_tiles(L, i, n_rg, R) : 0;
-      long long incl = mine;
+      const int mine = i < n ? cost(i) : 0;
+      int incl = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+        const int v = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += v;
       }
-      const long long a = (before + incl - mine) * L.n_kv_heads, z = (before + incl) * L.n_kv_heads;
+      const int a = before + (incl - mine) * L.n_kv_heads, z = before + incl * L.n_kv_heads;
       const bool here = mine > 0 && a <= begin && begin < z;
       if (here) {
-        sh[32] = ((long long)i << 32) | (unsigned)((begin - a) / mine);
-        sh[33] = (begin - a) % mine;
+        sh[32] = i;
+        sh[33] = (begin - a) / mine;
+        sh[34] = (begin - a) % mine;
       }
       if (__any_sync(0xffffffffu, here)) break;
-      before += __shfl_sync(0xffffffffu, incl, 31);
+      before += __shfl_sync(0xffffffffu, incl, 31) * L.n_kv_heads;
     }
   }
   __syncthreads();
   Walk w;
-  w.i = (int)(sh[32] >> 32);
-  w.g = (int)(sh[32] & 0xffffffff);
-  w.j0 = (int)sh[33];
-  w.pos = w.begin = begin;
+  w.b = sh[32] / n_rg;
+  w.rg = sh[32] - w.b * n_rg;
+  w.g = sh[33];
+  w.at = sh[34];
+  w.pos = begin;
   w.end = end;
-  w.total = all;
+  w.total = total;
   w.parts = parts;
+  w.first = true;
   return w;
 }
 
 __device__ __forceinline__ bool next_piece(const qsp_attn_kv8_layer& L, int n_rg, int R, Walk& w, Piece& p) {
-  if (w.pos >= w.end) return false;
-  p.b = w.i / n_rg;
-  p.rg = w.i - p.b * n_rg;
-  p.g = w.g;
-  p.j0 = w.j0;
-  p.unit_tiles = unit_tiles(L, w.i, n_rg, R);
-  p.n = (int)min((long long)(p.unit_tiles - w.j0), w.end - w.pos);
-  p.first = w.pos == w.begin;
-  w.pos += p.n;
-  w.j0 = 0;
-  if (++w.g == L.n_kv_heads) {
-    w.g = 0;
-    ++w.i;
+  while (w.pos < w.end) {
+    p.b = w.b;
+    p.rg = w.rg;
+    p.g = w.g;
+    p.unit_tiles = unit_tiles(L, w.b, w.rg, n_rg, R);
+    const int step = min(UNIT_COST + p.unit_tiles - w.at, w.end - w.pos);
+    p.j0 = max(w.at - UNIT_COST, 0);
+    p.n = max(w.at + step - UNIT_COST, 0) - p.j0;
+    w.pos += step;
+    w.at = 0;
+    if (++w.g == L.n_kv_heads) {
+      w.g = 0;
+      if (++w.rg == n_rg) {
+        w.rg = 0;
+        ++w.b;
+      }
+    }
+    if (p.n > 0) {
+      p.first = w.first;
+      w.first = false;
+      return true;
+    }
   }
-  return true;
+  return false;
 }
 
 // workspace: meta [G] int4, then partials: ml [2G][R] float2 (m in log2 units, l), o [2G][R][hd]
@@ -207,9 +231,8 @@ inline size_t scratch_bytes(int G, int R, int hd) { return (size_t)G * 16 + 2ull
 __device__ __forceinline__ void put_meta(const Scratch& s, const Walk& w, const Piece& p) {
   int4 m = make_int4(0, 0, 0, 0);
   if (p.n > 0 && !p.whole() && p.j0 == 0) {
-    const long long last = w.end - p.n + p.unit_tiles - 1;               // the unit's last tile
-    const int c1 = (int)(((last + 1) * w.parts - 1) / w.total);         // ... and the CTA that has it
-    m = make_int4(p.b, p.rg, p.g | (p.first ? 0 : 1 << 30), c1 - (int)blockIdx.x + 1);
+    const int last = w.end - p.n + p.unit_tiles - 1;   // position of the unit's last tile
+    m = make_int4(p.b, p.rg, p.g | (p.first ? 0 : 1 << 30), share_owner(last, w.total, w.parts) - (int)blockIdx.x + 1);
   }
   s.meta[blockIdx.x] = m;
 }

@@ -29,6 +29,8 @@
 #include "qsp_attn_kv8.cuh"
 #include "qsp_tc.cuh"
 
+#include <limits.h>
+
 #include <algorithm>
 
 namespace qsp {
@@ -37,8 +39,8 @@ namespace kv8 {
 __device__ int g_kv8_error = 0;
 
 constexpr int CODE_WAIT = 302;       // a bounded wait ran out
-constexpr float SLACK = 2.f;         // log2 units the running maximum may lag behind
-constexpr float BIAS = 6.f;          // weights are held times 2^BIAS: at most 2^(SLACK + BIAS) = 256 <= 448
+constexpr float SLACK = 4.f;         // log2 units the running maximum may lag behind
+constexpr float BIAS = 4.f;          // weights are held times 2^BIAS: at most 2^(SLACK + BIAS) = 256 <= 448
 constexpr float NOTHING = -1e30f;    // maximum of a row that has seen nothing
 
 template <int HD, int R_>
@@ -52,7 +54,8 @@ struct Cfg {
   static constexpr int OCC = HD == 256 || R >= 32 ? 1 : 2;  // CTAs per SM
   static constexpr int BUDGET = OCC == 1 ? 232448 : 115712;
   // barriers, row scales, row maxima, reduction buffer
-  static constexpr int SMALL = 8 * 28 + 4 * (R + 2 * R + 4 * R) + 16;
+  // barriers, row scales (of two pieces), maxima and factors, reduction buffer
+  static constexpr int SMALL = 8 * 26 + 4 * (2 * R + 2 * R + 4 * R) + 16;
   static constexpr int FIT = (BUDGET - SMALL - 6 * 2 * TILE - QB - 2 * PB) / SLOT;
   static constexpr int NS = FIT < 8 ? FIT : 8;              // ring slots
   static constexpr int NSV = (NS + 1) / 2, NSK = NS - NSV;  // a V tile waits for its weights, a K tile does not
@@ -61,18 +64,21 @@ struct Cfg {
   static constexpr int SOFTMAX = 128 * NWG, THREADS = SOFTMAX + 128;
   static constexpr int COLS_USED = 2 * N + CB * N;
   static constexpr int COLS = COLS_USED <= 64 ? 64 : COLS_USED <= 128 ? 128 : COLS_USED <= 256 ? 256 : 512;
-  static_assert(NSK >= 2, "ring too short");
-  static_assert(2 * PB >= 34 * 8, "the weights' buffers first hold share()'s 34 long longs");
+  static_assert(NSK >= 2 && NSK <= 4, "ring too short, or too long for the exponents' slots");
+  static_assert(2 * PB >= 36 * 4, "the weights' buffers first hold share()'s 36 ints");
 };
 
 // ---------------------------------------------------------------- descriptors
 // rows of W bytes (16, 32, 64 or 128), swizzled over W bytes, 8-row groups 8·W apart: the layout of
 // TMA boxes with inner extent W. K-major: rows are M/N, bytes along the row K. MN-major: the row is
 // M/N, rows are K; lead = distance of the next W elements along M/N (0: the same again).
+struct Sdesc {   // the address is in the low word; all offsets within shared memory are added there
+  uint32_t lo, hi;
+};
 template <int W>
-__device__ __forceinline__ uint64_t sdesc(uint32_t saddr, uint32_t lead) {
-  constexpr uint64_t type = W == 128 ? 2 : W == 64 ? 4 : W == 32 ? 6 : 0;
-  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(8 * W >> 4) << 32 | 1ull << 46 | type << 61;
+__device__ __forceinline__ Sdesc sdesc(const void* p, uint32_t lead) {
+  constexpr uint32_t type = W == 128 ? 2 : W == 64 ? 4 : W == 32 ? 6 : 0;
+  return {((tc::smem_u32(p) & 0x3FFFFu) >> 4) | (lead >> 4) << 16, (8 * W >> 4) | 1u << 14 | type << 29};
 }
 template <int W>
 __device__ __forceinline__ int swz(int row, int chunk) {   // byte offset of a 16-byte chunk of a row
@@ -83,14 +89,57 @@ __device__ __forceinline__ int swz(int row, int chunk) {   // byte offset of a 1
 __host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N, bool mn_major) {
   return (1u << 4) | (mn_major ? 3u << 15 : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
-__device__ __forceinline__ void umma_e4m3_warp(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred e, p;\n\t"
-      "elect.sync _|e, 0xffffffff;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
-      : "memory");
+// `STEPS` MMAs of K = 32 into the same accumulator, the operands' addresses a_step and b_step (in
+// 16-byte units) apart; the first accumulates iff acc != 0. Issued by a converged warp.
+template <int STEPS, int A_STEP, int B_STEP>
+__device__ __forceinline__ void umma_e4m3_warp(uint32_t d, Sdesc a, Sdesc b, uint32_t idesc, uint32_t acc) {
+  static_assert(STEPS == 1 || STEPS == 2 || STEPS == 4, "");
+  if constexpr (STEPS == 4) {
+    asm volatile(
+        "{\n\t.reg .pred e, p;\n\t.reg .b64 a, b;\n\t.reg .b32 x, y;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "mov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %5, p;\n\t"
+        "setp.eq.b32 p, %6, %6;\n\t"
+        "add.u32 x, %1, %7;\n\tadd.u32 y, %3, %8;\n\tmov.b64 a, {x, %2};\n\tmov.b64 b, {y, %4};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %5, p;\n\t"
+        "add.u32 x, x, %7;\n\tadd.u32 y, y, %8;\n\tmov.b64 a, {x, %2};\n\tmov.b64 b, {y, %4};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %5, p;\n\t"
+        "add.u32 x, x, %7;\n\tadd.u32 y, y, %8;\n\tmov.b64 a, {x, %2};\n\tmov.b64 b, {y, %4};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %5, p;\n\t}" ::"r"(d),
+        "r"(a.lo), "r"(a.hi), "r"(b.lo), "r"(b.hi), "r"(idesc), "r"(acc), "n"(A_STEP), "n"(B_STEP)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred e, p;\n\t.reg .b64 a, b;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "mov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %5, p;\n\t}" ::"r"(d),
+        "r"(a.lo), "r"(a.hi), "r"(b.lo), "r"(b.hi), "r"(idesc), "r"(acc)
+        : "memory");
+    if constexpr (STEPS == 2)
+      umma_e4m3_warp<1, A_STEP, B_STEP>(d, {a.lo + A_STEP, a.hi}, {b.lo + B_STEP, b.hi}, idesc, 1);
+  }
+}
+
+// ---------------------------------------------------------------- waits
+// Bounded; the poll is kept small (five roles share an instruction cache), the rest is out of line.
+__device__ __noinline__ bool give_up(uint32_t polls, volatile int* abort) {
+  if (*abort) return true;
+  if (polls < tc::WAIT_LIMIT) {
+    __nanosleep(64);
+    return false;
+  }
+  atomicExch(&g_kv8_error, CODE_WAIT);
+  *abort = 1;
+  return true;
+}
+__device__ __forceinline__ void wait_bar(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  uint32_t n = 0;
+  while (!tc::mbar_try_wait(bar, parity))
+    if ((++n & 255u) == 0 && give_up(n, abort)) return;
 }
 
 // ---------------------------------------------------------------- TMEM, n columns of this warp's 32 lanes
@@ -188,15 +237,14 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
   uint64_t* vfull = kempty + NSK;
   uint64_t* vempty = vfull + NSV;
   uint64_t* sfull = vempty + NSV;  // scores of a tile are in TMEM
-  uint64_t* sempty = sfull + 2;    // ... and have been read
-  uint64_t* pfull = sempty + 2;    // weights of a tile are in shared memory
+  uint64_t* pfull = sfull + 2;     // weights of a tile are in shared memory (and its scores have been read)
   uint64_t* pdone = pfull + 2;     // ... and their product with V is done
-  uint64_t* qfull = pdone + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kfull + 27);   // after at most 2·8 + 9 barriers
-  float* qs = reinterpret_cast<float*>(kfull + 28);   // [R] scale of a row's scores, in log2 units
-  float* mcur = qs + R;                               // [R] running maximum
+  uint64_t* qfull = pdone + 2;     // 2·8 + 7 barriers at most
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kfull + 25);
+  float* qs = reinterpret_cast<float*>(kfull + 26);   // [2][R] scale of a row's scores, in log2 units, by piece
+  float* mcur = qs + 2 * R;                           // [R] running maximum
   float* aux = mcur + R;                              // [R] rescaling factor; 1 / l at the end
-  float* red = aux + R;                               // [NWG][4][RW]
+  float* red = aux + R;                               // [NWG][RW][4]
   volatile int* abort = reinterpret_cast<volatile int*>(red + 4 * R);
   uint16_t* sE = reinterpret_cast<uint16_t*>(red + 4 * R + 4);   // [NSE][128] a key's scale exponents + 127: K low, V high byte
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -207,7 +255,6 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
     for (int i = 0; i < 2 * C::NS; ++i) tc::mbar_init(&kfull[i], i < NSK ? 2 : 1);   // kfull (K and its scales), kempty, vfull, vempty
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(&sfull[i], 1);
-      tc::mbar_init(&sempty[i], 4 * NWG);
       tc::mbar_init(&pfull[i], 4 * NWG);
       tc::mbar_init(&pdone[i], 1);
     }
@@ -215,17 +262,16 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (tid < R) mcur[tid] = NOTHING;
   if (warp == W_MMA) {
     tc::tmem_alloc(tmem_slot, C::COLS);
     tc::fence_before();
   }
   pdl_wait();
-  // the weights' buffers are not in use yet: room for share()'s 34 long longs
-  Walk w = share(L, n_rg, R, reinterpret_cast<long long*>(sP));
+  // the weights' buffers are not in use yet: room for share()'s 36 ints
+  Walk w = share(L, n_rg, R, reinterpret_cast<int*>(sP));
   tc::fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
-  const Scratch ws = scratch(L, gridDim.x, R);
-  auto wait = [&](uint64_t* bar, uint32_t parity) { tc::mbar_wait(bar, parity, CODE_WAIT, &g_kv8_error, abort); };
   const int cap = L.max_pages * L.page_size;
   auto base_of = [&](int b) { return min(L.seq_lens[b], cap); };
   auto kv_end_of = [&](int base) { return min(base + L.tokens, cap); };   // keys that can have a page
@@ -233,37 +279,44 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
   p.n = 0;
 
   if (warp == W_K || warp == W_V) {
-    // ---------------- loads of K and of V: up to 32 boxes a tile (box_rows keys x a column block each),
-    // lane i looks up the page of box i, one tile ahead
+    // ---------------- loads of K and of V: boxes of box_rows keys x a column block; lane i looks up the page
+    // of the tile's i-th box_rows keys, one tile ahead
     const bool is_v = warp == W_V;
     const CUtensorMap* map = is_v ? &tmV : &tmK;
     uint8_t* ring = is_v ? sV : sK;
     uint64_t* full = is_v ? vfull : kfull;
     uint64_t* empty = is_v ? vempty : kempty;
     const int slots = is_v ? NSV : NSK;
-    const int chunks = TILE / box_rows, boxes = chunks * CB;
+    const int chunks = TILE / box_rows, pages_step = TILE / L.page_size, slot_step = TILE % L.page_size;
     int slot = 0;
     uint32_t turn = 1;   // parity of "empty" for this turn of the ring
     while (next_piece(L, n_rg, R, w, p)) {
       const int kv_end = kv_end_of(base_of(p.b));
       const int32_t* pages = L.page_table + (int64_t)p.b * L.max_pages;
-      int key = p.j0 * TILE + lane % chunks * box_rows;
-      auto page_at = [&](int j) { return j < p.n && lane < boxes && key < kv_end ? pages[key / L.page_size] : -1; };
-      int page = page_at(0);
+      int key = lane < chunks ? p.j0 * TILE + lane * box_rows : INT_MAX - 2 * TILE;   // this lane's first key of the tile
+      int lp = key / L.page_size, in = key - lp * L.page_size;
+      int page = key < kv_end ? pages[lp] : -1;
       for (int j = 0; j < p.n; ++j) {
         // row of the pages' [pages·n_kv·page_size, hd] view, or -1
-        const int row = page >= 0 && page < L.num_pages ? (page * L.n_kv_heads + p.g) * L.page_size + key % L.page_size : -1;
-        key += TILE;
-        page = page_at(j + 1);
-        wait(&empty[slot], turn);
+        const int row = page >= 0 && page < L.num_pages ? (page * L.n_kv_heads + p.g) * L.page_size + in : -1;
+        if (lane < chunks) key += TILE;
+        lp += pages_step;
+        in += slot_step;
+        if (in >= L.page_size) {
+          in -= L.page_size;
+          ++lp;
+        }
+        page = j + 1 < p.n && key < kv_end ? pages[lp] : -1;
+        wait_bar(&empty[slot], turn, abort);
+        __syncwarp();
         const uint32_t there = __ballot_sync(0xffffffffu, row >= 0);
-        tc::mbar_expect_tx_warp(&full[slot], __popc(there) * box_rows * CW);
+        tc::mbar_expect_tx_warp(&full[slot], __popc(there) * box_rows * HD);
         uint8_t* dst = ring + slot * C::SLOT;
-        for (int i = 0; i < boxes; ++i) {
+        for (int i = 0; i < chunks; ++i, dst += box_rows * CW) {
           const int r = __shfl_sync(0xffffffffu, row, i);
           if (r >= 0) {
-            const int cb = i / chunks;
-            tc::tma_load_2d_warp(dst + cb * (TILE * CW) + (i - cb * chunks) * (box_rows * CW), map, &full[slot], cb * CW, r);
+#pragma unroll
+            for (int cb = 0; cb < CB; ++cb) tc::tma_load_2d_warp(dst + cb * (TILE * CW), map, &full[slot], cb * CW, r);
           }
         }
         if (++slot == slots) {
@@ -277,27 +330,39 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
     // tiles ahead, scales one. A slot is free when QK of the tile NSK before this one is done: that product was
     // issued after the scores of the tile NSE before, and so its scales, had been read.
     const int nb = L.page_size / L.scale_block, sb_log = __ffs(L.scale_block) - 1;
-    uint32_t tile = 0;
+    const int pages_step = TILE / L.page_size, slot_step = TILE % L.page_size;
+    int slot = 0, eslot = 0;
+    uint32_t turn = 1;
     while (next_piece(L, n_rg, R, w, p)) {
       const int kv_end = kv_end_of(base_of(p.b));
       const int32_t* pages = L.page_table + (int64_t)p.b * L.max_pages;
-      int page[4], slot[4];      // of tile j + 1, then j + 2
-      float ks[4], vs[4];        // of tile j
+      int page[4], blk[4], lp[4], in[4];   // of tile j + 1, then j + 2
+      float ks[4], vs[4];                  // of tile j
       bool here[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = p.j0 * TILE + i * 32 + lane;
+        lp[i] = key / L.page_size;
+        in[i] = key - lp[i] * L.page_size;
+      }
       auto pages_at = [&](int j) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int key = (p.j0 + j) * TILE + i * 32 + lane;
-          const int lp = key / L.page_size;
-          slot[i] = key - lp * L.page_size;
-          page[i] = j < p.n && key < kv_end ? pages[lp] : -1;
+          blk[i] = in[i] >> sb_log;
+          page[i] = j < p.n && (p.j0 + j) * TILE + i * 32 + lane < kv_end ? pages[lp[i]] : -1;
+          lp[i] += pages_step;
+          in[i] += slot_step;
+          if (in[i] >= L.page_size) {
+            in[i] -= L.page_size;
+            ++lp[i];
+          }
         }
       };
       auto scales_at = [&]() {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           here[i] = page[i] >= 0 && page[i] < L.num_pages;
-          const int64_t at = here[i] ? ((int64_t)page[i] * L.n_kv_heads + p.g) * nb + (slot[i] >> sb_log) : 0;
+          const int64_t at = here[i] ? ((int64_t)page[i] * L.n_kv_heads + p.g) * nb + blk[i] : 0;
           ks[i] = L.k_scales[at];
           vs[i] = L.v_scales[at];
         }
@@ -305,96 +370,100 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
       pages_at(0);
       scales_at();
       pages_at(1);
-      for (int j = 0; j < p.n; ++j, ++tile) {
-        const int s = tile % NSK;
-        wait(&kempty[s], ((tile / NSK) & 1u) ^ 1u);
-        uint16_t* e = sE + tile % C::NSE * TILE;
+      for (int j = 0; j < p.n; ++j) {
+        wait_bar(&kempty[slot], turn, abort);
+        uint16_t* e = sE + eslot * TILE;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           e[i * 32 + lane] = here[i] ? (uint16_t)((__float_as_uint(ks[i]) >> 23 & 0xffu) | (__float_as_uint(vs[i]) >> 23 & 0xffu) << 8)
                                      : (uint16_t)MISSING;
         __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&kfull[s]);
+        if (lane == 0) tc::mbar_arrive(&kfull[slot]);
+        if (++eslot == C::NSE) eslot = 0;
+        if (++slot == NSK) {
+          slot = 0;
+          turn ^= 1u;
+        }
         scales_at();
         pages_at(j + 2);
       }
     }
   } else if (warp == W_MMA) {
-    // ---------------- products
+    // ---------------- products, in the order QK(0) QK(1) PV(0) QK(2) PV(1) ... of each piece. QK(t) overwrites the
+    // scores of t - 2, which had been read when pfull(t - 2) came, before PV(t - 2) and so before QK(t).
     constexpr uint32_t ID_QK = idesc_e4m3(128, N, false), ID_PV = idesc_e4m3(128, N, true);
-    uint32_t tile = 0, piece = 0;
+    const Sdesc dK = sdesc<CW>(sK, 16), dV = sdesc<CW>(sV, 0), dQ = sdesc<CW>(sQ, 16);
+    const Sdesc dP = N == 16 ? sdesc<16>(sP, 8 * 16) : sdesc<N < 32 ? 32 : N>(sP, 0);
+    uint32_t tile = 0, piece = 0, kslot = 0, kturn = 0, vslot = 0, vturn = 0;
     while (next_piece(L, n_rg, R, w, p)) {
-      wait(qfull, piece & 1u);
+      wait_bar(qfull, piece & 1u, abort);
       ++piece;
-      const uint32_t t0 = tile;
       auto qk = [&](uint32_t t) {
-        const int slot = t % NSK, sb = t & 1;
-        wait(&kfull[slot], (t / NSK) & 1u);
-        wait(&sempty[sb], ((t >> 1) & 1u) ^ 1u);
+        const uint32_t sb = t & 1;
+        wait_bar(&kfull[kslot], kturn, abort);
+        __syncwarp();
         tc::fence_after();
-        const uint32_t a = tc::smem_u32(sK + slot * C::SLOT), q = tc::smem_u32(sQ);
 #pragma unroll
-        for (int k = 0; k < HD / 32; ++k) {
-          const int cb = k * 32 / CW, off = k * 32 % CW;
-          umma_e4m3_warp(tmem + sb * N, sdesc<CW>(a + cb * (TILE * CW) + off, 16), sdesc<CW>(q + cb * (N * CW) + off, 16), ID_QK, k > 0);
-        }
-        tc::umma_commit_warp(&kempty[slot]);
+        for (int cb = 0; cb < CB; ++cb)
+          umma_e4m3_warp<CW / 32, 2, 2>(tmem + sb * N, {dK.lo + (kslot * C::SLOT + cb * (TILE * CW)) / 16, dK.hi},
+                                        {dQ.lo + cb * (N * CW) / 16, dQ.hi}, ID_QK, cb > 0);
+        tc::umma_commit_warp(&kempty[kslot]);
         tc::umma_commit_warp(&sfull[sb]);
-      };
-      auto pv = [&](uint32_t t) {
-        const int slot = t % NSV, pb = t & 1;
-        wait(&vfull[slot], (t / NSV) & 1u);
-        wait(&pfull[pb], (t >> 1) & 1u);
-        tc::fence_after();
-        const uint32_t v = tc::smem_u32(sV + slot * C::SLOT), pp = tc::smem_u32(sP + pb * C::PB);
-#pragma unroll
-        for (int k = 0; k < TILE / 32; ++k) {
-#pragma unroll
-          for (int mb = 0; mb < CB; ++mb)
-            umma_e4m3_warp(tmem + 2 * N + mb * N, sdesc<CW>(v + mb * (TILE * CW) + k * 32 * CW, 0),
-                           N == 16 ? sdesc<16>(pp + k * 32 * N, 8 * 16) : sdesc<N < 32 ? 32 : N>(pp + k * 32 * N, 0), ID_PV,
-                           t > t0 || k > 0);
+        if (++kslot == NSK) {
+          kslot = 0;
+          kturn ^= 1u;
         }
-        tc::umma_commit_warp(&vempty[slot]);
-        tc::umma_commit_warp(&pdone[pb]);
       };
-      qk(t0);
-      for (int j = 0; j < p.n; ++j) {
-        if (j + 1 < p.n) qk(t0 + j + 1);
-        pv(t0 + j);
+      qk(tile);
+      for (int j = 0; j < p.n; ++j, ++tile) {
+        if (j + 1 < p.n) qk(tile + 1);
+        const uint32_t pb = tile & 1;
+        wait_bar(&vfull[vslot], vturn, abort);
+        wait_bar(&pfull[pb], (tile >> 1) & 1u, abort);
+        __syncwarp();
+        tc::fence_after();
+#pragma unroll
+        for (int mb = 0; mb < CB; ++mb)
+          umma_e4m3_warp<4, 32 * CW / 16, 32 * N / 16>(tmem + 2 * N + mb * N, {dV.lo + (vslot * C::SLOT + mb * (TILE * CW)) / 16, dV.hi},
+                                                       {dP.lo + pb * C::PB / 16, dP.hi}, ID_PV, j > 0);
+        tc::umma_commit_warp(&vempty[vslot]);
+        tc::umma_commit_warp(&pdone[pb]);
+        if (++vslot == NSV) {
+          vslot = 0;
+          vturn ^= 1u;
+        }
       }
-      tile = t0 + p.n;
     }
   } else {
-    // ---------------- softmax: thread = key of the tile, RW rows
+    // ---------------- softmax: thread = key of the tile, RW rows. Row r of the unit is column
+    // (r / RW)·2RW + r % RW of the products (hi), and RW columns further (lo): a warpgroup's are together.
     const int wg = warp >> 2, wq = warp & 3, key_in = wq * 32 + lane, r0 = wg * RW, bar = 1 + wg;
-    const uint32_t tlane = tmem + ((uint32_t)(wq * 32) << 16);
+    const uint32_t tlane = tmem + ((uint32_t)(wq * 32) << 16) + wg * (2 * RW);
     const int my_row = r0 + row_of<RW>(lane);
     const bool reducer = lane % (32 / RW) == 0;    // its lane of a row's reduction
-    uint32_t tile = 0;
-    while (next_piece(L, n_rg, R, w, p)) {
-      const int row0 = p.rg * R, nrows = min(R, rows_total - row0);
-      const int base = base_of(p.b);
-      const int key0 = p.j0 * TILE + key_in;
+    const Scratch ws = scratch(L, gridDim.x, R);
+    uint32_t tile = 0, piece = 0, eslot = 0, vslot = 0, vturn = 0;
 
-      // stage Q: a warp per row, hi at row r and lo at row R + r of the swizzled tile
-      constexpr int ROWS = R / (4 * NWG);
-      float x[ROWS][EPL];
+    // Q of a piece: a warp per row
+    constexpr int ROWS = R / (4 * NWG);
+    auto load_q = [&](const Piece& q, float (&x)[ROWS][EPL]) {
 #pragma unroll
       for (int i = 0; i < ROWS; ++i) {
-        const int r = warp + i * 4 * NWG;
-        if (r < nrows) {
-          const int rr = row0 + r, t = rr / nrep, hq = p.g * nrep + rr - t * nrep;
+        const int rr = q.rg * R + warp + i * 4 * NWG;
+        if (rr < rows_total) {
+          const int t = rr / nrep, hq = q.g * nrep + rr - t * nrep;
           load_row<__nv_bfloat16, EPL>(
-              static_cast<const __nv_bfloat16*>(L.q_buf) + (((int64_t)p.b * L.tokens + t) * L.n_heads + hq) * HD, lane, true, x[i]);
+              static_cast<const __nv_bfloat16*>(L.q_buf) + (((int64_t)q.b * L.tokens + t) * L.n_heads + hq) * HD, lane, true, x[i]);
         } else {
 #pragma unroll
           for (int k = 0; k < EPL; ++k) x[i][k] = 0.f;
         }
       }
+    };
+    auto stage_q = [&](uint32_t n, const float (&x)[ROWS][EPL]) {   // for the n-th piece
 #pragma unroll
       for (int i = 0; i < ROWS; ++i) {
-        const int r = warp + i * 4 * NWG;
+        const int r = warp + i * 4 * NWG, row = r / RW * (2 * RW) + r % RW;
         float amax = 0.f;
         bool fine = true;
 #pragma unroll
@@ -417,64 +486,74 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
           lo[k / 4] |= (uint32_t)to_e4m3x2((a - f.x) * 16.f, (z - f.y) * 16.f) << (k % 4 * 8);
         }
         const int byte = lane * EPL, cb = byte / CW, in = byte % CW;
-        store_bytes<EPL>(sQ + cb * (N * CW) + swz<CW>(r, in / 16) + in % 16, hi[0], hi[1]);
-        store_bytes<EPL>(sQ + cb * (N * CW) + swz<CW>(R + r, in / 16) + in % 16, lo[0], lo[1]);
-        if (lane == 0) {
-          qs[r] = fine ? exp2i(e) * (L.scale * LOG2E) : NAN;
-          mcur[r] = NOTHING;
-        }
+        store_bytes<EPL>(sQ + cb * (N * CW) + swz<CW>(row, in / 16) + in % 16, hi[0], hi[1]);
+        store_bytes<EPL>(sQ + cb * (N * CW) + swz<CW>(row + RW, in / 16) + in % 16, lo[0], lo[1]);
+        if (lane == 0) qs[(n & 1) * R + r] = fine ? exp2i(e) * (L.scale * LOG2E) : NAN;
       }
       tc::fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(qfull);
-      asm volatile("barrier.cta.sync 15, %0;" ::"n"(C::SOFTMAX) : "memory");   // qs and mcur of all rows are written
+    };
 
-      float m[RW], l[RW], qr[RW == 8 ? 8 : 1];
+    bool more = next_piece(L, n_rg, R, w, p);
+    if (more) {
+      float x[ROWS][EPL];
+      load_q(p, x);
+      stage_q(0, x);
+    }
+    while (more) {
+      const int row0 = p.rg * R + r0;   // this warpgroup's first row
+      const int base = base_of(p.b);
+      const float* q_scale = qs + (piece & 1) * R + r0;
+      // token and head (in the group) of the first row; later rows follow by counting
+      const int t_first = row0 / nrep, h_first = row0 - t_first * nrep;
+      int key = p.j0 * TILE + key_in;
+
+      float m[RW], l[RW];
 #pragma unroll
       for (int i = 0; i < RW; ++i) {
         m[i] = NOTHING;
         l[i] = 0.f;
-        if (RW == 8) qr[i] = qs[r0 + i];
       }
-      auto q_scale = [&](int i) { return RW == 8 ? qr[i] : qs[r0 + i]; };   // 16 rows: registers are short
-      // last key that the first of all rows of this warpgroup sees
-      const int seen_by_all = base + (row0 + r0) / nrep;
-
-      for (int j = 0; j < p.n; ++j, ++tile) {
+      for (int j = 0; j < p.n; ++j, ++tile, key += TILE) {
         const uint32_t sb = tile & 1, ph = (tile >> 1) & 1;
-        const int key = key0 + j * TILE;
-        wait(&sfull[sb], ph);
+        wait_bar(&sfull[sb], ph, abort);
+        __syncwarp();
         tc::fence_after();
-        uint32_t ev = sE[tile % C::NSE * TILE + key_in];
+        uint32_t sc[2 * RW];
+        tm_ld<2 * RW>(tlane + sb * N, sc);
+        uint32_t ev = sE[eslot * TILE + key_in];
+        if (++eslot == C::NSE) eslot = 0;
         const bool mine = ev != MISSING;   // the key exists
         if (!mine) ev = 127u << 8 | 127u;
         const float ks = __uint_as_float((ev & 0xffu) << 23);
         const float ve = (float)(int)(ev >> 8) - (127.f - BIAS), ivs = exp2i(127 - max((int)(ev >> 8), 1));
         // rows that may see this key: all, but for missing keys and the tiles of the new tokens
         uint32_t sees = mine ? 0xffffffffu : 0u;
-        if (mine && key > seen_by_all) {
+        if (mine && key > base + t_first) {
+          sees = 0;
+          int t = base + t_first, h = h_first;
 #pragma unroll
-          for (int i = 1; i < RW; ++i)
-            if (key > base + (row0 + r0 + i) / nrep) sees &= ~(1u << i);
-          sees &= ~1u;
+          for (int i = 0; i < RW; ++i) {
+            if (key <= t) sees |= 1u << i;
+            if (++h == nrep) {
+              h = 0;
+              ++t;
+            }
+          }
         }
-        uint32_t sh[RW], sl[RW];
-        tm_ld<RW>(tlane + sb * N + r0, sh);
-        tm_ld<RW>(tlane + sb * N + R + r0, sl);
+        const bool all = sees == 0xffffffffu;
         tm_wait_ld();
-        tc::fence_before();
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&sempty[sb]);
 
-        // d: exponents of the weights; scores times qr·ks are in log2 units
+        // d: exponents of the weights; scores times q_scale·ks are in log2 units
         float x[RW], d[RW];
         float top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < RW; ++i) {
-          x[i] = fmaf(__uint_as_float(sl[i]), 0.0625f, __uint_as_float(sh[i]));
-          d[i] = fmaf(x[i], q_scale(i) * ks, ve - m[i]);
+          x[i] = fmaf(__uint_as_float(sc[RW + i]), 0.0625f, __uint_as_float(sc[i]));
+          d[i] = fmaf(x[i], q_scale[i] * ks, ve - m[i]);
         }
-        if (sees != 0xffffffffu) {
+        if (!all) {
 #pragma unroll
           for (int i = 0; i < RW; ++i)
             if (!(sees >> i & 1)) d[i] = -INFINITY;
@@ -485,7 +564,7 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
           // raise the maxima to what they are, rescale l and O
           float y[RW];
 #pragma unroll
-          for (int i = 0; i < RW; ++i) y[i] = sees >> i & 1 ? fmaf(x[i], q_scale(i) * ks, ve - BIAS) : -INFINITY;
+          for (int i = 0; i < RW; ++i) y[i] = sees >> i & 1 ? fmaf(x[i], q_scale[i] * ks, ve - BIAS) : -INFINITY;
           const float best = warp_transpose_reduce<RW, true>(y, lane);
           if (reducer) red[wg * 4 * RW + row_of<RW>(lane) * 4 + wq] = best;
           bar_sync(bar);
@@ -501,27 +580,27 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
           for (int i = 0; i < RW; ++i) {
             m[i] = mcur[r0 + i];
             l[i] *= aux[r0 + i];
-            d[i] = sees >> i & 1 ? fmaf(x[i], q_scale(i) * ks, ve - m[i]) : -INFINITY;
+            d[i] = sees >> i & 1 ? fmaf(x[i], q_scale[i] * ks, ve - m[i]) : -INFINITY;
           }
           if (j > 0) {
-            const uint32_t t1 = tile - 1;
-            wait(&pdone[t1 & 1], (t1 >> 1) & 1);
+            wait_bar(&pdone[sb ^ 1], ((tile - 1) >> 1) & 1, abort);
+            __syncwarp();
             tc::fence_after();
 #pragma unroll 1
-            for (int c = 0; c < CB * 2; ++c) {
-              uint32_t o[RW];
-              const uint32_t where = tlane + 2 * N + (c >> 1) * N + (c & 1) * R + r0;
-              tm_ld<RW>(where, o);
+            for (int mb = 0; mb < CB; ++mb) {
+              uint32_t o[2 * RW];
+              tm_ld<2 * RW>(tlane + 2 * N + mb * N, o);
               tm_wait_ld();
 #pragma unroll
-              for (int i = 0; i < RW; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * aux[r0 + i]);
-              tm_st<RW>(where, o);
+              for (int i = 0; i < 2 * RW; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * aux[r0 + i % RW]);
+              tm_st<2 * RW>(tlane + 2 * N + mb * N, o);
             }
             tm_wait_st();
             tc::fence_before();
           }
         }
-        // weights, as two e4m3 values each
+        // weights, as two e4m3 values each. (The buffer's previous product, of tile - 2, was issued before QK of
+        // this tile and so is done.)
         uint32_t hi[RW / 4], lo[RW / 4];
 #pragma unroll
         for (int i = 0; i < RW; i += 2) {
@@ -539,74 +618,101 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
             lo[i / 4] |= (uint32_t)q << 16;
           }
         }
-        // (the buffer's previous product, of tile - 2, was issued before QK of this tile and so is done)
         uint8_t* pr = sP + sb * C::PB;
-        if constexpr (R == 8) {
-          *reinterpret_cast<uint4*>(pr + key_in * 16) = make_uint4(hi[0], hi[1], lo[0], lo[1]);
-        } else if constexpr (RW == 8) {
-          *reinterpret_cast<uint2*>(pr + swz<N>(key_in, r0 / 16) + r0 % 16) = make_uint2(hi[0], hi[1]);
-          *reinterpret_cast<uint2*>(pr + swz<N>(key_in, (R + r0) / 16) + r0 % 16) = make_uint2(lo[0], lo[1]);
+        constexpr int PW = N < 16 ? 16 : N;
+        if constexpr (RW == 8) {
+          *reinterpret_cast<uint4*>(pr + swz<PW>(key_in, wg)) = make_uint4(hi[0], hi[1], lo[0], lo[1]);
         } else {
-          *reinterpret_cast<uint4*>(pr + swz<N>(key_in, r0 / 16)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          *reinterpret_cast<uint4*>(pr + swz<N>(key_in, (R + r0) / 16)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          *reinterpret_cast<uint4*>(pr + swz<PW>(key_in, 2 * wg)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          *reinterpret_cast<uint4*>(pr + swz<PW>(key_in, 2 * wg + 1)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
         if (!mine && wg == 0) {
           // a key that is not there: its value row is whatever lies in the slot, and 0·NaN is NaN
-          wait(&vfull[tile % NSV], (tile / NSV) & 1u);
-          uint8_t* v = sV + tile % NSV * C::SLOT + key_in * CW;
+          wait_bar(&vfull[vslot], vturn, abort);
+          uint8_t* v = sV + vslot * C::SLOT + key_in * CW;
 #pragma unroll
           for (int cb = 0; cb < CB; ++cb)
 #pragma unroll
             for (int k = 0; k < CW / 16; ++k) *reinterpret_cast<uint4*>(v + cb * (TILE * CW) + k * 16) = make_uint4(0, 0, 0, 0);
         }
+        if (++vslot == NSV) {
+          vslot = 0;
+          vturn ^= 1u;
+        }
+        tc::fence_before();
         tc::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(&pfull[sb]);
       }
 
-      // ---- the piece is done: l over the keys, O out of TMEM (thread = head dim)
+      // ---- the piece is done. The scores of its last tile are here, so Q is free for the next piece, whose first
+      // product then runs beside the rest: l over the keys, O out of TMEM (thread = head dim).
+      Piece next;
+      more = next_piece(L, n_rg, R, w, next);
+      float x[ROWS][EPL];
+      if (more) load_q(next, x);
+      const bool whole = p.whole();
       const float s = warp_transpose_reduce<RW, false>(l, lane);
       if (reducer) red[wg * 4 * RW + row_of<RW>(lane) * 4 + wq] = s;
-      const uint32_t t1 = tile - 1;
-      wait(&pdone[t1 & 1], (t1 >> 1) & 1);
-      tc::fence_after();
+      if (more) stage_q(piece + 1, x);
       bar_sync(bar);
-      const bool whole = p.whole();
       if (wq == 0 && reducer) {
         const float4 v4 = *reinterpret_cast<const float4*>(red + wg * 4 * RW + row_of<RW>(lane) * 4);
         const float v = (v4.x + v4.y) + (v4.z + v4.w);
         aux[my_row] = v == 0.f ? 0.f : 1.f / v;
         if (!whole) ws.ml[(int64_t)p.slot() * R + my_row] = make_float2(v == 0.f ? -INFINITY : mcur[my_row], v);
+        mcur[my_row] = NOTHING;
       }
+      wait_bar(&pdone[(tile - 1) & 1], ((tile - 1) >> 1) & 1, abort);
+      tc::fence_after();
       bar_sync(bar);
 #pragma unroll 1
       for (int mb = 0; mb < CB; ++mb) {
-        uint32_t oh[RW], ol[RW];
-        tm_ld<RW>(tlane + 2 * N + mb * N + r0, oh);
-        tm_ld<RW>(tlane + 2 * N + mb * N + R + r0, ol);
-        tm_wait_ld();
         const int dim = mb * 128 + key_in;
-        if (dim < HD) {
-          if (whole) {
+        uint32_t o[2 * RW];
+        tm_ld<2 * RW>(tlane + 2 * N + mb * N, o);
+        if (whole) {
+          float gate[RW];
+          const int64_t m0 = (int64_t)p.b * L.tokens + t_first;
+          int64_t mrow = m0;
+          int h = h_first;
 #pragma unroll
-            for (int i = 0; i < RW; ++i) {
-              if (r0 + i < nrows) {
-                const int rr = row0 + r0 + i, t = rr / nrep, hq = p.g * nrep + rr - t * nrep;
-                const int64_t mrow = (int64_t)p.b * L.tokens + t;
-                const float gate = __bfloat162float(static_cast<const __nv_bfloat16*>(L.qkv)[mrow * L.ld_qkv + (int64_t)hq * 2 * HD + HD + dim]);
-                const float o = fmaf(__uint_as_float(ol[i]), 0.0625f, __uint_as_float(oh[i])) * aux[r0 + i];
-                static_cast<__nv_bfloat16*>(L.out)[mrow * L.ld_out + (int64_t)hq * HD + dim] = __float2bfloat16_rn(o * sigmoidf_(gate));
-              }
+          for (int i = 0; i < RW; ++i) {
+            gate[i] = 0.f;
+            if (row0 + i < rows_total && dim < HD)
+              gate[i] = __bfloat162float(
+                  static_cast<const __nv_bfloat16*>(L.qkv)[mrow * L.ld_qkv + (int64_t)(p.g * nrep + h) * 2 * HD + HD + dim]);
+            if (++h == nrep) {
+              h = 0;
+              ++mrow;
             }
-          } else {
-            float* o = ws.o + ((int64_t)p.slot() * R + r0) * HD + dim;
+          }
+          tm_wait_ld();
+          mrow = m0;
+          h = h_first;
 #pragma unroll
-            for (int i = 0; i < RW; ++i) o[i * HD] = fmaf(__uint_as_float(ol[i]), 0.0625f, __uint_as_float(oh[i]));
+          for (int i = 0; i < RW; ++i) {
+            const float v = fmaf(__uint_as_float(o[RW + i]), 0.0625f, __uint_as_float(o[i])) * aux[r0 + i];
+            if (row0 + i < rows_total && dim < HD)
+              static_cast<__nv_bfloat16*>(L.out)[mrow * L.ld_out + (int64_t)(p.g * nrep + h) * HD + dim] = __float2bfloat16_rn(v * sigmoidf_(gate[i]));
+            if (++h == nrep) {
+              h = 0;
+              ++mrow;
+            }
+          }
+        } else {
+          tm_wait_ld();
+          float* to = ws.o + ((int64_t)p.slot() * R + r0) * HD + dim;
+          if (dim < HD) {
+#pragma unroll
+            for (int i = 0; i < RW; ++i) to[i * HD] = fmaf(__uint_as_float(o[RW + i]), 0.0625f, __uint_as_float(o[i]));
           }
         }
       }
       tc::fence_before();   // the next piece's products overwrite O after its pfull
-      asm volatile("barrier.cta.sync 15, %0;" ::"n"(C::SOFTMAX) : "memory");   // qs, mcur, aux are written again
+      bar_sync(bar);        // aux and red are written again
+      ++piece;
+      if (more) p = next;
     }
     if (tid == 0) put_meta(ws, w, p);
   }
