@@ -361,86 +361,125 @@ static int launch_simt(const qsp_attn_kv8_layer& L, int G, cudaStream_t st) {
 }
 
 // ------------------------------------------------------------------ merge of divided units
-// CTA (c, y): rows 4y..4y+3 of the divided unit whose first tile attention CTA c had, if there is one; two
-// warps a row. Each warp weights its half of the partials with 2^(m_p − M) and adds them in their order,
-// a lane HD/32 columns; the halves are added, divided by l and gated. Latency-bound: eight partials
-// are in flight at a time.
-constexpr int MERGE_ROWS = 4;
+// CTA (u, y): the u-th divided unit, 8 rows of it with a warp each, or (WIDE, for few units of many parts) one
+// row with its partials dealt out to 8 warps. A warp weights its partials with 2^(m_p − M) and adds them in
+// their order, a lane HD/32 columns, four in flight at a time; WIDE adds the warps' sums in order. Then
+// / l and the gate. Bound by latency: four dependent reads and the launch.
+constexpr int MERGE_WARPS = 8;
 
-template <typename T, int HD>
-__global__ void __launch_bounds__(64 * MERGE_ROWS) merge_kernel(const qsp_attn_kv8_layer L, int G, int R) {
+template <typename T, int HD, bool WIDE>
+__global__ void __launch_bounds__(32 * MERGE_WARPS, 4) merge_kernel(const qsp_attn_kv8_layer L, int G, int R) {
   pdl_trigger();
   pdl_wait();
-  constexpr int EPL = HD / 32, DEPTH = 8;
-  __shared__ float half[MERGE_ROWS][HD + 1];
+  constexpr int EPL = HD / 32, DEPTH = 4;
+  __shared__ float part[WIDE ? MERGE_WARPS : 1][HD + 1];
+  __shared__ int found, counts[32];
   const Scratch ws = scratch(L, G, R);
-  const int4 meta = ws.meta[blockIdx.x];
-  const int np = meta.w;
-  if (np == 0) return;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = warp >> 1, h = warp & 1;
-  const int r = blockIdx.y * MERGE_ROWS + row;
-  const int nrep = L.n_heads / L.n_kv_heads, rr = meta.y * R + r;
-  const bool live = r < R && rr < nrep * L.tokens;
-  const int c = blockIdx.x, first = 2 * c + (meta.z >> 30), mid = (np + 1) / 2;
-  auto slot = [&](int q) { return (int64_t)(q == 0 ? first : 2 * (c + q)) * R + r; };
-  float acc[EPL], den = 0.f;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // the attention CTA that has the first tile of the u-th divided unit: thread i looks at CTAs i, i + 256, ..
+  constexpr int MAX_SCAN = 4;
+  bool has[MAX_SCAN];
+  uint32_t mask[MAX_SCAN];
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) acc[i] = 0.f;
-  if (live) {
-    float M = -INFINITY;
-    for (int q = lane; q < np; q += 32) M = fmaxf(M, ws.ml[slot(q)].x);
-    M = warp_max(M);
-    const float ref = M == -INFINITY ? 0.f : M;
-    const int q1 = h ? np : mid;
-    for (int q0 = h ? mid : 0; q0 < q1; q0 += DEPTH) {
-      float v[DEPTH][EPL];
-      float2 ml[DEPTH];
+  for (int k = 0; k < MAX_SCAN; ++k) {
+    const int i = k * 32 * MERGE_WARPS + threadIdx.x;
+    has[k] = i < G && ws.meta[i].w != 0;
+  }
+  if (threadIdx.x == 0) found = -1;
 #pragma unroll
-      for (int u = 0; u < DEPTH; ++u) {
-        if (q0 + u < q1) {
-          ml[u] = ws.ml[slot(q0 + u)];
-          load_row<float, EPL>(ws.o + slot(q0 + u) * HD, lane, true, v[u]);
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < DEPTH; ++u) {
-        if (q0 + u < q1 && ml[u].y != 0.f) {   // else a part of which the row saw nothing
-          const float f = exp2f(ml[u].x - ref);
-          den = fmaf(f, ml[u].y, den);
-#pragma unroll
-          for (int i = 0; i < EPL; ++i) acc[i] = fmaf(f, v[u][i], acc[i]);
-        }
-      }
-    }
-    if (h) {
-#pragma unroll
-      for (int i = 0; i < EPL; ++i) half[row][lane * EPL + i] = acc[i];
-      if (lane == 0) half[row][HD] = den;
-    }
+  for (int k = 0; k < MAX_SCAN; ++k) {
+    mask[k] = __ballot_sync(0xffffffffu, has[k]);
+    if (lane == 0) counts[k * MERGE_WARPS + warp] = __popc(mask[k]);
   }
   __syncthreads();
-  if (!live || h) return;
-  den += half[row][HD];
+#pragma unroll
+  for (int k = 0; k < MAX_SCAN; ++k) {
+    const int w = k * MERGE_WARPS + warp;
+    const int before = __reduce_add_sync(0xffffffffu, lane < w ? counts[lane] : 0);
+    if (has[k] && before + __popc(mask[k] & ((1u << lane) - 1)) == (int)blockIdx.x)
+      found = k * 32 * MERGE_WARPS + threadIdx.x;
+  }
+  __syncthreads();
+  const int c = found;
+  if (c < 0) return;
+  const int4 meta = ws.meta[c];
+  const int np = meta.w, r = WIDE ? blockIdx.y : blockIdx.y * MERGE_WARPS + warp;
+  const int nrep = L.n_heads / L.n_kv_heads, rr = meta.y * R + r;
+  const bool live = r < R && rr < nrep * L.tokens;   // the same for the whole CTA if WIDE
+  if (!live) return;
+  const int first = 2 * c + (meta.z >> 30);
+  auto slot = [&](int q) { return (int64_t)(q == 0 ? first : 2 * (c + q)) * R + r; };
   const int t = rr / nrep, hq = (meta.z & ((1 << 30) - 1)) * nrep + rr - t * nrep;
   const int64_t m = (int64_t)meta.x * L.tokens + t;
-  const T* gate = static_cast<const T*>(L.qkv) + m * L.ld_qkv + (int64_t)hq * 2 * HD + HD + lane * EPL;
-  T* out = static_cast<T*>(L.out) + m * L.ld_out + (int64_t)hq * HD + lane * EPL;
+  const T* gate_p = static_cast<const T*>(L.qkv) + m * L.ld_qkv + (int64_t)hq * 2 * HD + HD + lane * EPL;
+  float gate[EPL], acc[EPL], den = 0.f, M = -INFINITY;
 #pragma unroll
   for (int i = 0; i < EPL; ++i) {
-    const float v = den == 0.f ? 0.f : (acc[i] + half[row][lane * EPL + i]) / den;
-    out[i] = dt<T>::from_f(v * sigmoidf_(dt<T>::to_f(gate[i])));
+    gate[i] = dt<T>::to_f(gate_p[i]);
+    acc[i] = 0.f;
   }
+  for (int q = lane; q < np; q += 32) M = fmaxf(M, ws.ml[slot(q)].x);
+  M = warp_max(M);
+  const float ref = M == -INFINITY ? 0.f : M;
+  const int per = WIDE ? (np + MERGE_WARPS - 1) / MERGE_WARPS : np;
+  const int q_begin = WIDE ? warp * per : 0, q_end = min(np, q_begin + per);
+  for (int q0 = q_begin; q0 < q_end; q0 += DEPTH) {
+    float v[DEPTH][EPL];
+    float2 ml[DEPTH];
+#pragma unroll
+    for (int u = 0; u < DEPTH; ++u) {
+      if (q0 + u < q_end) {
+        ml[u] = ws.ml[slot(q0 + u)];
+        load_row<float, EPL>(ws.o + slot(q0 + u) * HD, lane, true, v[u]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < DEPTH; ++u) {
+      if (q0 + u < q_end && ml[u].y != 0.f) {   // else a part of which the row saw nothing
+        const float f = exp2f(ml[u].x - ref);
+        den = fmaf(f, ml[u].y, den);
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) acc[i] = fmaf(f, v[u][i], acc[i]);
+      }
+    }
+  }
+  T* out = static_cast<T*>(L.out) + m * L.ld_out + (int64_t)hq * HD + lane * EPL;
+  if constexpr (WIDE) {
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) part[warp][lane * EPL + i] = acc[i];
+    if (lane == 0) part[warp][HD] = den;
+    __syncthreads();
+    if (warp != 0) return;
+    for (int w = 1; w < MERGE_WARPS; ++w) {
+      den += part[w][HD];
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) acc[i] += part[w][lane * EPL + i];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) out[i] = dt<T>::from_f((den == 0.f ? 0.f : acc[i] / den) * sigmoidf_(gate[i]));
+}
+
+template <typename T, int HD>
+static int launch_merge_hd(const qsp_attn_kv8_layer& L, int G, int R, cudaStream_t st) {
+  const int rows = L.n_heads / L.n_kv_heads * L.tokens;
+  const int64_t units = (int64_t)L.batch * L.n_kv_heads * ((rows + R - 1) / R);
+  const int divided = (int)std::min<int64_t>(units, G);
+  // few units of many parts each: a CTA a row (one sequence of 32k keys, hd 256: 74 parts)
+  if (units * MERGE_WARPS <= G)
+    return launch_pdl("qsp_attn_kv8_verify(merge)", merge_kernel<T, HD, true>, dim3(divided, std::min(R, rows)), dim3(32 * MERGE_WARPS), 0,
+                      st, L, G, R);
+  return launch_pdl("qsp_attn_kv8_verify(merge)", merge_kernel<T, HD, false>,
+                    dim3(divided, (std::min(R, rows) + MERGE_WARPS - 1) / MERGE_WARPS), dim3(32 * MERGE_WARPS), 0, st, L, G, R);
 }
 
 template <typename T>
 static int launch_merge_t(const qsp_attn_kv8_layer& L, int G, int R, cudaStream_t st) {
-  const int rows = std::min(R, L.n_heads / L.n_kv_heads * L.tokens);
-  const dim3 grid(G, (rows + MERGE_ROWS - 1) / MERGE_ROWS), block(64 * MERGE_ROWS);
   switch (L.head_dim) {
-    case 32: return launch_pdl("qsp_attn_kv8_verify(merge)", merge_kernel<T, 32>, grid, block, 0, st, L, G, R);
-    case 64: return launch_pdl("qsp_attn_kv8_verify(merge)", merge_kernel<T, 64>, grid, block, 0, st, L, G, R);
-    case 128: return launch_pdl("qsp_attn_kv8_verify(merge)", merge_kernel<T, 128>, grid, block, 0, st, L, G, R);
-    default: return launch_pdl("qsp_attn_kv8_verify(merge)", merge_kernel<T, 256>, grid, block, 0, st, L, G, R);
+    case 32: return launch_merge_hd<T, 32>(L, G, R, st);
+    case 64: return launch_merge_hd<T, 64>(L, G, R, st);
+    case 128: return launch_merge_hd<T, 128>(L, G, R, st);
+    default: return launch_merge_hd<T, 256>(L, G, R, st);
   }
 }
 
