@@ -43,6 +43,14 @@ constexpr float SLACK = 4.f;         // log2 units the running maximum may lag b
 constexpr float BIAS = 4.f;          // weights are held times 2^BIAS: at most 2^(SLACK + BIAS) = 256 <= 448
 constexpr float NOTHING = -1e30f;    // maximum of a row that has seen nothing
 
+// A piece of work as the scales' warp hands it to the others, which run up to 4 tiles behind it (and the
+// slowest of them 3 pieces more): 8 slots.
+constexpr int NDESC = 8;
+struct Desc {
+  int b, row0, g, j0;         // sequence, first row of the unit, kv head, first tile
+  int n, base, slot, whole;   // tiles (0: no more pieces), sequence length, partial's slot, whole unit
+};
+
 template <int HD, int R_>
 struct Cfg {
   static constexpr int R = R_, N = 2 * R;                   // query rows, columns (hi | lo)
@@ -52,19 +60,25 @@ struct Cfg {
   static constexpr int SLOT = TILE * HD;                    // bytes of a K or V tile
   static constexpr int QB = N * HD, PB = TILE * N;
   static constexpr int OCC = HD == 256 || R >= 32 ? 1 : 2;  // CTAs per SM
-  static constexpr int BUDGET = OCC == 1 ? 232448 : 115712;
+  static constexpr size_t BUDGET = OCC == 1 ? 232448 : 115712;
   // barriers, row scales, row maxima, reduction buffer
-  // barriers, row scales (of two pieces), maxima and factors, reduction buffer
-  static constexpr int SMALL = 8 * 26 + 4 * (2 * R + 2 * R + 4 * R) + 16;
-  static constexpr int FIT = (BUDGET - SMALL - 6 * 2 * TILE - QB - 2 * PB) / SLOT;
-  static constexpr int NS = FIT < 8 ? FIT : 8;              // ring slots
-  static constexpr int NSV = (NS + 1) / 2, NSK = NS - NSV;  // a V tile waits for its weights, a K tile does not
-  static constexpr int NSE = NSK + 2;                       // slots of scale exponents
-  static constexpr size_t BYTES = (size_t)NS * SLOT + QB + 2 * PB + SMALL + NSE * 2 * TILE;
+  // barriers, piece descriptors, row scales (of two pieces), maxima and factors, reduction buffer
+  static constexpr int SMALL = 8 * 34 + NDESC * 32 + 4 * (2 * R + 2 * R + 4 * R) + 16;
+  // slots of scale exponents: two more than of K
+  static constexpr size_t bytes(int ns) { return (size_t)ns * SLOT + QB + 2 * PB + SMALL + (ns / 2 + 2) * 2 * TILE; }
+  static constexpr int slots() {
+    int ns = 8;
+    while (bytes(ns) > BUDGET) --ns;
+    return ns;
+  }
+  static constexpr int NS = slots();                        // ring slots
+  static constexpr int NSK = NS / 2, NSV = NS - NSK;        // a V tile waits for its weights, a K tile does not
+  static constexpr int NSE = NSK + 2;
+  static constexpr size_t BYTES = bytes(NS);
   static constexpr int SOFTMAX = 128 * NWG, THREADS = SOFTMAX + 128;
   static constexpr int COLS_USED = 2 * N + CB * N;
   static constexpr int COLS = COLS_USED <= 64 ? 64 : COLS_USED <= 128 ? 128 : COLS_USED <= 256 ? 256 : 512;
-  static_assert(NSK >= 2 && NSK <= 4, "ring too short, or too long for the exponents' slots");
+  static_assert(NSK >= 2 && NSK <= 4, "ring too short, or too long for the descriptors' slots");
   static_assert(2 * PB >= 36 * 4, "the weights' buffers first hold share()'s 36 ints");
 };
 
@@ -142,36 +156,44 @@ __device__ __forceinline__ void wait_bar(uint64_t* bar, uint32_t parity, volatil
     if ((++n & 255u) == 0 && give_up(n, abort)) return;
 }
 
-// ---------------------------------------------------------------- TMEM, n columns of this warp's 32 lanes
-template <int N>
-__device__ __forceinline__ void tm_ld(uint32_t t, uint32_t* r) {
-  if constexpr (N == 32) {
-    tm_ld<16>(t, r);
-    tm_ld<16>(t + 16, r + 16);
-  } else if constexpr (N == 16) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(t));
+// EPL bf16 of a row at p + lane·EPL, as they are
+template <int EPL>
+__device__ __forceinline__ void load_raw(const __nv_bfloat16* p, int lane, uint32_t (&r)[EPL > 1 ? EPL / 2 : 1]) {
+  const __nv_bfloat16* src = p + lane * EPL;
+  if constexpr (EPL == 8) {
+    const uint4 u = *reinterpret_cast<const uint4*>(src);
+    r[0] = u.x, r[1] = u.y, r[2] = u.z, r[3] = u.w;
+  } else if constexpr (EPL == 4) {
+    const uint2 u = *reinterpret_cast<const uint2*>(src);
+    r[0] = u.x, r[1] = u.y;
+  } else if constexpr (EPL == 2) {
+    r[0] = *reinterpret_cast<const uint32_t*>(src);
   } else {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-                 : "r"(t));
+    r[0] = *reinterpret_cast<const uint16_t*>(src);
   }
 }
-template <int N>
-__device__ __forceinline__ void tm_st(uint32_t t, const uint32_t* r) {
-  if constexpr (N > 8) {
-    tm_st<N / 2>(t, r);
-    tm_st<N / 2>(t + N / 2, r + N / 2);
-  } else {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(t), "r"(r[0]), "r"(r[1]),
-                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-                 : "memory");
-  }
+
+// ---------------------------------------------------------------- TMEM, 8 columns of this warp's 32 lanes
+__device__ __forceinline__ void tm_ld8(uint32_t t, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(t));
 }
-__device__ __forceinline__ void tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tm_st8(uint32_t t, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(t), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+// the registers are operands, so that nothing reads them before the wait
+__device__ __forceinline__ void tm_wait_ld8(uint32_t (&r)[8]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])::"memory");
+}
+__device__ __forceinline__ void tm_wait_ld8(uint32_t (&r)[8], uint32_t (&s)[8]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(s[0]), "+r"(s[1]),
+                 "+r"(s[2]), "+r"(s[3]), "+r"(s[4]), "+r"(s[5]), "+r"(s[6]), "+r"(s[7])::"memory");
+}
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -239,9 +261,11 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
   uint64_t* sfull = vempty + NSV;  // scores of a tile are in TMEM
   uint64_t* pfull = sfull + 2;     // weights of a tile are in shared memory (and its scores have been read)
   uint64_t* pdone = pfull + 2;     // ... and their product with V is done
-  uint64_t* qfull = pdone + 2;     // 2·8 + 7 barriers at most
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kfull + 25);
-  float* qs = reinterpret_cast<float*>(kfull + 26);   // [2][R] scale of a row's scores, in log2 units, by piece
+  uint64_t* qfull = pdone + 2;     // Q of a piece is in shared memory
+  uint64_t* dfull = qfull + 1;     // [NDESC] a piece's descriptor is there; 2·8 + 7 + 8 barriers at most
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kfull + 33);
+  Desc* desc = reinterpret_cast<Desc*>(kfull + 34);
+  float* qs = reinterpret_cast<float*>(desc + NDESC);   // [2][R] scale of a row's scores, in log2 units, by piece
   float* mcur = qs + 2 * R;                           // [R] running maximum
   float* aux = mcur + R;                              // [R] rescaling factor; 1 / l at the end
   float* red = aux + R;                               // [NWG][RW][4]
@@ -259,6 +283,7 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
       tc::mbar_init(&pdone[i], 1);
     }
     tc::mbar_init(qfull, 4 * NWG);
+    for (int i = 0; i < NDESC; ++i) tc::mbar_init(&dfull[i], 1);
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -273,10 +298,12 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
   tc::fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
   const int cap = L.max_pages * L.page_size;
-  auto base_of = [&](int b) { return min(L.seq_lens[b], cap); };
   auto kv_end_of = [&](int base) { return min(base + L.tokens, cap); };   // keys that can have a page
-  Piece p;
-  p.n = 0;
+  auto piece_at = [&](uint32_t i) -> Desc {   // the i-th piece of this CTA
+    wait_bar(&dfull[i % NDESC], i / NDESC & 1u, abort);
+    __syncwarp();
+    return desc[i % NDESC];
+  };
 
   if (warp == W_K || warp == W_V) {
     // ---------------- loads of K and of V: boxes of box_rows keys x a column block; lane i looks up the page
@@ -290,8 +317,10 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
     const int chunks = TILE / box_rows, pages_step = TILE / L.page_size, slot_step = TILE % L.page_size;
     int slot = 0;
     uint32_t turn = 1;   // parity of "empty" for this turn of the ring
-    while (next_piece(L, n_rg, R, w, p)) {
-      const int kv_end = kv_end_of(base_of(p.b));
+    for (uint32_t piece = 0;; ++piece) {
+      const Desc p = piece_at(piece);
+      if (p.n == 0) break;
+      const int kv_end = kv_end_of(p.base);
       const int32_t* pages = L.page_table + (int64_t)p.b * L.max_pages;
       int key = lane < chunks ? p.j0 * TILE + lane * box_rows : INT_MAX - 2 * TILE;   // this lane's first key of the tile
       int lp = key / L.page_size, in = key - lp * L.page_size;
@@ -316,7 +345,11 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
           const int r = __shfl_sync(0xffffffffu, row, i);
           if (r >= 0) {
 #pragma unroll
-            for (int cb = 0; cb < CB; ++cb) tc::tma_load_2d_warp(dst + cb * (TILE * CW), map, &full[slot], cb * CW, r);
+            for (int cb = 0; cb < CB; ++cb) {
+              // read once: kept out of the way of queries, page tables and partials in L2
+              if (n_rg == 1) tc::tma_load_2d_evict_first_warp(dst + cb * (TILE * CW), map, &full[slot], cb * CW, r);
+              else tc::tma_load_2d_warp(dst + cb * (TILE * CW), map, &full[slot], cb * CW, r);
+            }
           }
         }
         if (++slot == slots) {
@@ -328,13 +361,23 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
   } else if (warp == W_E) {
     // ---------------- scale exponents of a tile's keys, 4 a lane, in step with the K ring: pages are loaded two
     // tiles ahead, scales one. A slot is free when QK of the tile NSK before this one is done: that product was
-    // issued after the scores of the tile NSE before, and so its scales, had been read.
+    // issued after the scores of the tile NSE before, and so its scales, had been read. This warp also walks
+    // through the CTA's share of the work and describes its pieces to the others.
     const int nb = L.page_size / L.scale_block, sb_log = __ffs(L.scale_block) - 1;
     const int pages_step = TILE / L.page_size, slot_step = TILE % L.page_size;
     int slot = 0, eslot = 0;
     uint32_t turn = 1;
-    while (next_piece(L, n_rg, R, w, p)) {
-      const int kv_end = kv_end_of(base_of(p.b));
+    Piece p;
+    p.n = 0;
+    for (uint32_t piece = 0;; ++piece) {
+      const bool more = next_piece(L, n_rg, R, w, p);
+      const int base = more ? min(L.seq_lens[p.b], cap) : 0;
+      if (lane == 0) {
+        desc[piece % NDESC] = {p.b, p.rg * R, p.g, p.j0, more ? p.n : 0, base, p.slot(), p.whole()};
+        tc::mbar_arrive(&dfull[piece % NDESC]);
+      }
+      if (!more) break;
+      const int kv_end = kv_end_of(base);
       const int32_t* pages = L.page_table + (int64_t)p.b * L.max_pages;
       int page[4], blk[4], lp[4], in[4];   // of tile j + 1, then j + 2
       float ks[4], vs[4];                  // of tile j
@@ -388,6 +431,7 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
         pages_at(j + 2);
       }
     }
+    if (lane == 0) put_meta(scratch(L, gridDim.x, R), w, p);
   } else if (warp == W_MMA) {
     // ---------------- products, in the order QK(0) QK(1) PV(0) QK(2) PV(1) ... of each piece. QK(t) overwrites the
     // scores of t - 2, which had been read when pfull(t - 2) came, before PV(t - 2) and so before QK(t).
@@ -395,9 +439,10 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
     const Sdesc dK = sdesc<CW>(sK, 16), dV = sdesc<CW>(sV, 0), dQ = sdesc<CW>(sQ, 16);
     const Sdesc dP = N == 16 ? sdesc<16>(sP, 8 * 16) : sdesc<N < 32 ? 32 : N>(sP, 0);
     uint32_t tile = 0, piece = 0, kslot = 0, kturn = 0, vslot = 0, vturn = 0;
-    while (next_piece(L, n_rg, R, w, p)) {
+    for (;; ++piece) {
+      const int n = piece_at(piece).n;
+      if (n == 0) break;
       wait_bar(qfull, piece & 1u, abort);
-      ++piece;
       auto qk = [&](uint32_t t) {
         const uint32_t sb = t & 1;
         wait_bar(&kfull[kslot], kturn, abort);
@@ -415,8 +460,8 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
         }
       };
       qk(tile);
-      for (int j = 0; j < p.n; ++j, ++tile) {
-        if (j + 1 < p.n) qk(tile + 1);
+      for (int j = 0; j < n; ++j, ++tile) {
+        if (j + 1 < n) qk(tile + 1);
         const uint32_t pb = tile & 1;
         wait_bar(&vfull[vslot], vturn, abort);
         wait_bar(&pfull[pb], (tile >> 1) & 1u, abort);
@@ -444,32 +489,34 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
     const Scratch ws = scratch(L, gridDim.x, R);
     uint32_t tile = 0, piece = 0, eslot = 0, vslot = 0, vturn = 0;
 
-    // Q of a piece: a warp per row
+    // Q of a piece: a warp per row, loaded one tile before it is staged (4 rows: when it is; registers are short)
     constexpr int ROWS = R / (4 * NWG);
-    auto load_q = [&](const Piece& q, float (&x)[ROWS][EPL]) {
+    constexpr bool AHEAD = ROWS <= 2;
+    uint32_t q_raw[ROWS][EPL > 1 ? EPL / 2 : 1];
+    auto load_q = [&](const Desc& q) {
 #pragma unroll
       for (int i = 0; i < ROWS; ++i) {
-        const int rr = q.rg * R + warp + i * 4 * NWG;
+        const int rr = q.row0 + warp + i * 4 * NWG;
         if (rr < rows_total) {
           const int t = rr / nrep, hq = q.g * nrep + rr - t * nrep;
-          load_row<__nv_bfloat16, EPL>(
-              static_cast<const __nv_bfloat16*>(L.q_buf) + (((int64_t)q.b * L.tokens + t) * L.n_heads + hq) * HD, lane, true, x[i]);
+          load_raw<EPL>(static_cast<const __nv_bfloat16*>(L.q_buf) + (((int64_t)q.b * L.tokens + t) * L.n_heads + hq) * HD, lane, q_raw[i]);
         } else {
 #pragma unroll
-          for (int k = 0; k < EPL; ++k) x[i][k] = 0.f;
+          for (int k = 0; k < (EPL > 1 ? EPL / 2 : 1); ++k) q_raw[i][k] = 0;
         }
       }
     };
-    auto stage_q = [&](uint32_t n, const float (&x)[ROWS][EPL]) {   // for the n-th piece
+    auto stage_q = [&](uint32_t n) {   // for the n-th piece
 #pragma unroll
       for (int i = 0; i < ROWS; ++i) {
         const int r = warp + i * 4 * NWG, row = r / RW * (2 * RW) + r % RW;
-        float amax = 0.f;
+        float x[EPL], amax = 0.f;
         bool fine = true;
 #pragma unroll
         for (int k = 0; k < EPL; ++k) {
-          amax = fmaxf(amax, fabsf(x[i][k]));
-          fine = fine && isfinite(x[i][k]);
+          x[k] = __uint_as_float(k & 1 ? q_raw[i][k / 2] & 0xffff0000u : q_raw[i][k / 2] << 16);
+          amax = fmaxf(amax, fabsf(x[k]));
+          fine = fine && isfinite(x[k]);
         }
         amax = warp_max(amax);
         fine = __all_sync(0xffffffffu, fine);
@@ -479,7 +526,7 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
         uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
 #pragma unroll
         for (int k = 0; k < EPL; k += 2) {
-          const float a = fine ? x[i][k] * inv : 0.f, z = fine && EPL > 1 ? x[i][EPL > 1 ? k + 1 : 0] * inv : 0.f;
+          const float a = fine ? x[k] * inv : 0.f, z = fine && EPL > 1 ? x[EPL > 1 ? k + 1 : 0] * inv : 0.f;
           const uint16_t h = to_e4m3x2(a, z);
           const float2 f = from_e4m3x2(h);
           hi[k / 4] |= (uint32_t)h << (k % 4 * 8);
@@ -495,33 +542,33 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
       if (lane == 0) tc::mbar_arrive(qfull);
     };
 
-    bool more = next_piece(L, n_rg, R, w, p);
-    if (more) {
-      float x[ROWS][EPL];
-      load_q(p, x);
-      stage_q(0, x);
+    Desc p = piece_at(0);
+    if (p.n > 0) {
+      load_q(p);
+      stage_q(0);
     }
-    while (more) {
-      const int row0 = p.rg * R + r0;   // this warpgroup's first row
-      const int base = base_of(p.b);
+    while (p.n > 0) {
+      const int row0 = p.row0 + r0;   // this warpgroup's first row
       const float* q_scale = qs + (piece & 1) * R + r0;
+      const float* m = mcur + r0;     // shared memory: registers are short
       // token and head (in the group) of the first row; later rows follow by counting
       const int t_first = row0 / nrep, h_first = row0 - t_first * nrep;
       int key = p.j0 * TILE + key_in;
+      bool more = false;
 
-      float m[RW], l[RW];
+      float l[RW];
 #pragma unroll
-      for (int i = 0; i < RW; ++i) {
-        m[i] = NOTHING;
-        l[i] = 0.f;
-      }
+      for (int i = 0; i < RW; ++i) l[i] = 0.f;
       for (int j = 0; j < p.n; ++j, ++tile, key += TILE) {
         const uint32_t sb = tile & 1, ph = (tile >> 1) & 1;
+        if (j == p.n - 1) {
+          const Desc next = piece_at(piece + 1);
+          more = next.n > 0;
+          if (AHEAD && more) load_q(next);
+        }
         wait_bar(&sfull[sb], ph, abort);
         __syncwarp();
         tc::fence_after();
-        uint32_t sc[2 * RW];
-        tm_ld<2 * RW>(tlane + sb * N, sc);
         uint32_t ev = sE[eslot * TILE + key_in];
         if (++eslot == C::NSE) eslot = 0;
         const bool mine = ev != MISSING;   // the key exists
@@ -530,9 +577,9 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
         const float ve = (float)(int)(ev >> 8) - (127.f - BIAS), ivs = exp2i(127 - max((int)(ev >> 8), 1));
         // rows that may see this key: all, but for missing keys and the tiles of the new tokens
         uint32_t sees = mine ? 0xffffffffu : 0u;
-        if (mine && key > base + t_first) {
+        if (mine && key > p.base + t_first) {
           sees = 0;
-          int t = base + t_first, h = h_first;
+          int t = p.base + t_first, h = h_first;
 #pragma unroll
           for (int i = 0; i < RW; ++i) {
             if (key <= t) sees |= 1u << i;
@@ -543,29 +590,40 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
           }
         }
         const bool all = sees == 0xffffffffu;
-        tm_wait_ld();
 
         // d: exponents of the weights; scores times q_scale·ks are in log2 units
-        float x[RW], d[RW];
-        float top = -INFINITY;
+        auto exponents = [&](float (&d)[RW], bool over_max) {   // relative to the running maximum, or as they are
 #pragma unroll
-        for (int i = 0; i < RW; ++i) {
-          x[i] = fmaf(__uint_as_float(sc[RW + i]), 0.0625f, __uint_as_float(sc[i]));
-          d[i] = fmaf(x[i], q_scale[i] * ks, ve - m[i]);
-        }
-        if (!all) {
+          for (int i = 0; i < RW; i += 8) {
+            uint32_t hi[8], lo[8];
+            tm_ld8(tlane + sb * N + i, hi);
+            tm_ld8(tlane + sb * N + RW + i, lo);
+            tm_wait_ld8(hi, lo);
 #pragma unroll
-          for (int i = 0; i < RW; ++i)
-            if (!(sees >> i & 1)) d[i] = -INFINITY;
-        }
+            for (int k = 0; k < 8; k += 4) {
+              const float4 q = *reinterpret_cast<const float4*>(q_scale + i + k), mm = *reinterpret_cast<const float4*>(m + i + k);
+              const float qq[4] = {q.x, q.y, q.z, q.w}, m4[4] = {mm.x, mm.y, mm.z, mm.w};
+#pragma unroll
+              for (int u = 0; u < 4; ++u) {
+                const float x = fmaf(__uint_as_float(lo[k + u]), 0.0625f, __uint_as_float(hi[k + u]));
+                d[i + k + u] = fmaf(x, qq[u] * ks, over_max ? ve - m4[u] : ve - BIAS);
+              }
+            }
+          }
+          if (!all) {
+#pragma unroll
+            for (int i = 0; i < RW; ++i)
+              if (!(sees >> i & 1)) d[i] = -INFINITY;
+          }
+        };
+        float d[RW], top = -INFINITY;
+        exponents(d, true);
 #pragma unroll
         for (int i = 0; i < RW; ++i) top = fmaxf(top, d[i]);
         if (bar_any(bar, top > SLACK + BIAS)) {
-          // raise the maxima to what they are, rescale l and O
-          float y[RW];
-#pragma unroll
-          for (int i = 0; i < RW; ++i) y[i] = sees >> i & 1 ? fmaf(x[i], q_scale[i] * ks, ve - BIAS) : -INFINITY;
-          const float best = warp_transpose_reduce<RW, true>(y, lane);
+          // raise the maxima to what they are, rescale l and O. (The scores are still in TMEM: until pfull.)
+          exponents(d, false);
+          const float best = warp_transpose_reduce<RW, true>(d, lane);
           if (reducer) red[wg * 4 * RW + row_of<RW>(lane) * 4 + wq] = best;
           bar_sync(bar);
           if (wq == 0 && reducer) {
@@ -576,24 +634,23 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
             aux[my_row] = ex2(was - now);
           }
           bar_sync(bar);
+          exponents(d, true);
 #pragma unroll
-          for (int i = 0; i < RW; ++i) {
-            m[i] = mcur[r0 + i];
-            l[i] *= aux[r0 + i];
-            d[i] = sees >> i & 1 ? fmaf(x[i], q_scale[i] * ks, ve - m[i]) : -INFINITY;
-          }
+          for (int i = 0; i < RW; ++i) l[i] *= aux[r0 + i];
           if (j > 0) {
             wait_bar(&pdone[sb ^ 1], ((tile - 1) >> 1) & 1, abort);
             __syncwarp();
             tc::fence_after();
 #pragma unroll 1
-            for (int mb = 0; mb < CB; ++mb) {
-              uint32_t o[2 * RW];
-              tm_ld<2 * RW>(tlane + 2 * N + mb * N, o);
-              tm_wait_ld();
+            for (int c = 0; c < CB * (RW / 4); ++c) {   // 8 columns
+              const int mb = c / (RW / 4), i0 = c % (RW / 4) * 8;
+              uint32_t o[8];
+              const uint32_t where = tlane + 2 * N + mb * N + i0;
+              tm_ld8(where, o);
+              tm_wait_ld8(o);
 #pragma unroll
-              for (int i = 0; i < 2 * RW; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * aux[r0 + i % RW]);
-              tm_st<2 * RW>(tlane + 2 * N + mb * N, o);
+              for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * aux[r0 + i0 % RW + i]);
+              tm_st8(where, o);
             }
             tm_wait_st();
             tc::fence_before();
@@ -647,39 +704,37 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
 
       // ---- the piece is done. The scores of its last tile are here, so Q is free for the next piece, whose first
       // product then runs beside the rest: l over the keys, O out of TMEM (thread = head dim).
-      Piece next;
-      more = next_piece(L, n_rg, R, w, next);
-      float x[ROWS][EPL];
-      if (more) load_q(next, x);
-      const bool whole = p.whole();
+      if (!AHEAD && more) load_q(piece_at(piece + 1));
+      if (more) stage_q(piece + 1);
       const float s = warp_transpose_reduce<RW, false>(l, lane);
       if (reducer) red[wg * 4 * RW + row_of<RW>(lane) * 4 + wq] = s;
-      if (more) stage_q(piece + 1, x);
       bar_sync(bar);
       if (wq == 0 && reducer) {
         const float4 v4 = *reinterpret_cast<const float4*>(red + wg * 4 * RW + row_of<RW>(lane) * 4);
         const float v = (v4.x + v4.y) + (v4.z + v4.w);
         aux[my_row] = v == 0.f ? 0.f : 1.f / v;
-        if (!whole) ws.ml[(int64_t)p.slot() * R + my_row] = make_float2(v == 0.f ? -INFINITY : mcur[my_row], v);
+        if (!p.whole) ws.ml[(int64_t)p.slot * R + my_row] = make_float2(v == 0.f ? -INFINITY : mcur[my_row], v);
         mcur[my_row] = NOTHING;
       }
       wait_bar(&pdone[(tile - 1) & 1], ((tile - 1) >> 1) & 1, abort);
       tc::fence_after();
       bar_sync(bar);
 #pragma unroll 1
-      for (int mb = 0; mb < CB; ++mb) {
-        const int dim = mb * 128 + key_in;
-        uint32_t o[2 * RW];
-        tm_ld<2 * RW>(tlane + 2 * N + mb * N, o);
-        if (whole) {
-          float gate[RW];
-          const int64_t m0 = (int64_t)p.b * L.tokens + t_first;
+      for (int c = 0; c < CB * (RW / 8); ++c) {   // 8 rows of 128 head dims
+        const int mb = c / (RW / 8), i0 = c % (RW / 8) * 8, dim = mb * 128 + key_in;
+        uint32_t oh[8], ol[8];
+        tm_ld8(tlane + 2 * N + mb * N + i0, oh);
+        tm_ld8(tlane + 2 * N + mb * N + RW + i0, ol);
+        if (p.whole) {
+          const int first = row0 + i0, t0 = first / nrep, h0 = first - t0 * nrep;
+          const int64_t m0 = (int64_t)p.b * L.tokens + t0;
+          float gate[8];
           int64_t mrow = m0;
-          int h = h_first;
+          int h = h0;
 #pragma unroll
-          for (int i = 0; i < RW; ++i) {
+          for (int i = 0; i < 8; ++i) {
             gate[i] = 0.f;
-            if (row0 + i < rows_total && dim < HD)
+            if (first + i < rows_total && dim < HD)
               gate[i] = __bfloat162float(
                   static_cast<const __nv_bfloat16*>(L.qkv)[mrow * L.ld_qkv + (int64_t)(p.g * nrep + h) * 2 * HD + HD + dim]);
             if (++h == nrep) {
@@ -687,13 +742,13 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
               ++mrow;
             }
           }
-          tm_wait_ld();
+          tm_wait_ld8(oh, ol);
           mrow = m0;
-          h = h_first;
+          h = h0;
 #pragma unroll
-          for (int i = 0; i < RW; ++i) {
-            const float v = fmaf(__uint_as_float(o[RW + i]), 0.0625f, __uint_as_float(o[i])) * aux[r0 + i];
-            if (row0 + i < rows_total && dim < HD)
+          for (int i = 0; i < 8; ++i) {
+            const float v = fmaf(__uint_as_float(ol[i]), 0.0625f, __uint_as_float(oh[i])) * aux[r0 + i0 + i];
+            if (first + i < rows_total && dim < HD)
               static_cast<__nv_bfloat16*>(L.out)[mrow * L.ld_out + (int64_t)(p.g * nrep + h) * HD + dim] = __float2bfloat16_rn(v * sigmoidf_(gate[i]));
             if (++h == nrep) {
               h = 0;
@@ -701,20 +756,19 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
             }
           }
         } else {
-          tm_wait_ld();
-          float* to = ws.o + ((int64_t)p.slot() * R + r0) * HD + dim;
+          tm_wait_ld8(oh, ol);
+          float* to = ws.o + ((int64_t)p.slot * R + r0 + i0) * HD + dim;
           if (dim < HD) {
 #pragma unroll
-            for (int i = 0; i < RW; ++i) to[i * HD] = fmaf(__uint_as_float(o[RW + i]), 0.0625f, __uint_as_float(o[i]));
+            for (int i = 0; i < 8; ++i) to[i * HD] = fmaf(__uint_as_float(ol[i]), 0.0625f, __uint_as_float(oh[i]));
           }
         }
       }
       tc::fence_before();   // the next piece's products overwrite O after its pfull
       bar_sync(bar);        // aux and red are written again
       ++piece;
-      if (more) p = next;
+      p = piece_at(piece);
     }
-    if (tid == 0) put_meta(ws, w, p);
   }
   __syncthreads();
   if (*abort) {   // a wait ran out: give copies and products in flight time to land before the memory is given back
