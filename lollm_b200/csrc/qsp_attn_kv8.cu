@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(PREP_THREADS) prep_kernel(const qsp_attn_kv8_l
   if (lane == 0) red[warp] = amax;
   __syncthreads();
   amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  const int e = min(max(scale_exp(amax), e_old), MAX_EXP);
+  const int e = min(max(scale_exp(__float_as_uint(amax)), e_old), MAX_EXP);
   if (threadIdx.x == 0) *scale = exp2i(e);
   if (e_old < e && n_old > 0) {   // earlier tokens of the block take the larger scale
     const float f = ldexpf(1.f, e_old - e);
@@ -246,7 +246,7 @@ __global__ void __launch_bounds__(SIMT_THREADS) simt_kernel(const qsp_attn_kv8_l
   p.n = 0;
   while (next_piece(L, n_rg, SIMT_R, w, p)) {
     const int row0 = p.rg * SIMT_R, nrows = min(SIMT_R, rows_total - row0);
-    const long long base = L.seq_lens[p.b];
+    const long long base = p.len;
     const long long kv_end = min(base + L.tokens, (long long)L.max_pages * L.page_size);
     __syncthreads();   // the previous piece's q has been read
     for (int e = tid; e < nrows * HD; e += SIMT_THREADS) {

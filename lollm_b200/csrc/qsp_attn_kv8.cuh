@@ -76,11 +76,10 @@ __device__ __forceinline__ void store_bytes(uint8_t* dst, uint32_t a, uint32_t b
 }
 
 // ---------------------------------------------------------------- scales
-// least e in [MIN_EXP, MAX_EXP] with amax <= 448·2^e (448 = 0.875·2^9), amax finite and >= 0
-__device__ __forceinline__ int scale_exp(float amax) {
-  int x;
-  const float m = frexpf(amax, &x);
-  const int e = amax > 0.f ? x - 9 + (m > 0.875f ? 1 : 0) : MIN_EXP;
+// least e in [MIN_EXP, MAX_EXP] with amax <= 448·2^e, amax finite and >= 0 given by its bits:
+// 448 = 1.75·2^8, so e is amax's exponent - 8, and one more where its mantissa is over 1.75
+__device__ __forceinline__ int scale_exp(uint32_t amax_bits) {
+  const int e = (int)(amax_bits >> 23) - (127 + 8) + ((amax_bits & 0x7fffffu) > 0x600000u ? 1 : 0);
   return min(max(e, MIN_EXP), MAX_EXP);
 }
 __device__ __forceinline__ float exp2i(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
@@ -95,10 +94,11 @@ __device__ __forceinline__ int exp_of(float scale) { return ((__float_as_int(sca
 // written out by its CTA; the others leave a partial (o, m, l) in the workspace: slot 2c for the
 // first piece of CTA c, 2c + 1 for its last. The CTA that has the first tile of a divided unit
 // describes it in meta[c] for the merge kernel.
-constexpr int UNIT_COST = 2;
+constexpr int UNIT_COST = 3;
 
 struct Piece {
   int b, rg, g;
+  int len;          // cached tokens of the sequence
   int j0, n;        // first tile and tiles of this piece
   int unit_tiles;   // tiles of the unit
   bool first;       // the CTA's first piece
@@ -106,10 +106,10 @@ struct Piece {
   __device__ __forceinline__ int slot() const { return 2 * (int)blockIdx.x + (first ? 0 : 1); }
 };
 
-__device__ __forceinline__ int unit_tiles(const qsp_attn_kv8_layer& L, int b, int rg, int n_rg, int R) {
+__device__ __forceinline__ int unit_tiles(const qsp_attn_kv8_layer& L, int len, int rg, int n_rg, int R) {
   const int t_last = rg == n_rg - 1 ? L.tokens - 1 : ((rg + 1) * R - 1) / (L.n_heads / L.n_kv_heads);
   const int cap = L.max_pages * L.page_size;
-  const int kv = min(min(L.seq_lens[b], cap) + t_last + 1, cap);
+  const int kv = min(min(len, cap) + t_last + 1, cap);
   return kv <= TILE ? 1 : (kv + TILE - 1) / TILE;   // a unit without keys has a tile too: it writes zeros
 }
 
@@ -119,6 +119,7 @@ struct Walk {
   int at;             // position in that unit
   int pos, end;       // the same position among all, and the end of this CTA's share
   int total, parts;   // of all units, and the CTAs that share them
+  int len, next_len;  // cached tokens of sequence b and (loaded ahead) of b + 1
   bool first;
 };
 __device__ __forceinline__ int share_begin(int c, int total, int parts) {
@@ -134,40 +135,40 @@ __device__ __forceinline__ int share_owner(int pos, int total, int parts) {
 // a __syncthreads.
 __device__ __forceinline__ Walk share(const qsp_attn_kv8_layer& L, int n_rg, int R, int* sh) {
   const int n = L.batch * n_rg, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
+  const int per = (n + blockDim.x - 1) / blockDim.x;   // (b, rg) pairs of a thread: consecutive ones
   auto cost = [&](int i) {
     const int b = n_rg == 1 ? i : i / n_rg;
-    return UNIT_COST + unit_tiles(L, b, i - b * n_rg, n_rg, R);
+    return UNIT_COST + unit_tiles(L, L.seq_lens[b], i - b * n_rg, n_rg, R);
   };
-  int s = 0;
-  for (int i = tid; i < n; i += blockDim.x) s += cost(i);
-  s = __reduce_add_sync(0xffffffffu, s);
-  if (lane == 0) sh[warp] = s;
+  int mine = 0;
+  for (int k = 0; k < per; ++k)
+    if (tid * per + k < n) mine += cost(tid * per + k);
+  int incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) sh[warp] = incl;
   __syncthreads();
-  int total = lane < nw ? sh[lane] : 0;
-  total = __reduce_add_sync(0xffffffffu, total) * L.n_kv_heads;
+  const int of_warp = lane < nw ? sh[lane] : 0;
+  const int total = __reduce_add_sync(0xffffffffu, of_warp) * L.n_kv_heads;
+  const int before = __reduce_add_sync(0xffffffffu, lane < warp ? of_warp : 0) + incl - mine;
   const int parts = min((int)gridDim.x, total);   // no more CTAs than tiles: every one of them has some
   const int c = min((int)blockIdx.x, parts);
   const int begin = share_begin(c, total, parts), end = share_begin(min(c + 1, parts), total, parts);
-  if (warp == 0) {
-    int before = 0;   // positions of the units before i0
-    for (int i0 = 0; i0 < n; i0 += 32) {
-      const int i = i0 + lane;
-      const int mine = i < n ? cost(i) : 0;
-      int incl = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += v;
+  int a = before * L.n_kv_heads;
+  if (a <= begin && begin < a + mine * L.n_kv_heads) {   // one thread's
+    for (int k = 0; k < per; ++k) {
+      const int one = cost(tid * per + k), all = one * L.n_kv_heads;
+      if (begin < a + all) {
+        sh[32] = tid * per + k;
+        sh[33] = (begin - a) / one;
+        sh[34] = (begin - a) % one;
+        sh[35] = L.seq_lens[sh[32] / n_rg];
+        break;
       }
-      const int a = before + (incl - mine) * L.n_kv_heads, z = before + incl * L.n_kv_heads;
-      const bool here = mine > 0 && a <= begin && begin < z;
-      if (here) {
-        sh[32] = i;
-        sh[33] = (begin - a) / mine;
-        sh[34] = (begin - a) % mine;
-      }
-      if (__any_sync(0xffffffffu, here)) break;
-      before += __shfl_sync(0xffffffffu, incl, 31) * L.n_kv_heads;
+      a += all;
     }
   }
   __syncthreads();
@@ -181,6 +182,8 @@ __device__ __forceinline__ Walk share(const qsp_attn_kv8_layer& L, int n_rg, int
   w.total = total;
   w.parts = parts;
   w.first = true;
+  w.len = sh[35];
+  w.next_len = begin < end && w.b + 1 < L.batch ? L.seq_lens[w.b + 1] : 0;
   return w;
 }
 
@@ -189,7 +192,8 @@ __device__ __forceinline__ bool next_piece(const qsp_attn_kv8_layer& L, int n_rg
     p.b = w.b;
     p.rg = w.rg;
     p.g = w.g;
-    p.unit_tiles = unit_tiles(L, w.b, w.rg, n_rg, R);
+    p.len = w.len;
+    p.unit_tiles = unit_tiles(L, w.len, w.rg, n_rg, R);
     const int step = min(UNIT_COST + p.unit_tiles - w.at, w.end - w.pos);
     p.j0 = max(w.at - UNIT_COST, 0);
     p.n = max(w.at + step - UNIT_COST, 0) - p.j0;
@@ -200,6 +204,8 @@ __device__ __forceinline__ bool next_piece(const qsp_attn_kv8_layer& L, int n_rg
       if (++w.rg == n_rg) {
         w.rg = 0;
         ++w.b;
+        w.len = w.next_len;
+        w.next_len = w.b + 1 < L.batch ? L.seq_lens[w.b + 1] : 0;
       }
     }
     if (p.n > 0) {

@@ -288,6 +288,8 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (tid < R) mcur[tid] = NOTHING;
+  if (lane == 0 && (warp == W_K || warp == W_V))
+    asm volatile("prefetch.tensormap [%0];" ::"l"(warp == W_K ? &tmK : &tmV) : "memory");
   if (warp == W_MMA) {
     tc::tmem_alloc(tmem_slot, C::COLS);
     tc::fence_before();
@@ -371,7 +373,7 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
     p.n = 0;
     for (uint32_t piece = 0;; ++piece) {
       const bool more = next_piece(L, n_rg, R, w, p);
-      const int base = more ? min(L.seq_lens[p.b], cap) : 0;
+      const int base = more ? min(p.len, cap) : 0;
       if (lane == 0) {
         desc[piece % NDESC] = {p.b, p.rg * R, p.g, p.j0, more ? p.n : 0, base, p.slot(), p.whole()};
         tc::mbar_arrive(&dfull[piece % NDESC]);
@@ -510,17 +512,17 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
 #pragma unroll
       for (int i = 0; i < ROWS; ++i) {
         const int r = warp + i * 4 * NWG, row = r / RW * (2 * RW) + r % RW;
-        float x[EPL], amax = 0.f;
-        bool fine = true;
+        float x[EPL];
+        uint32_t top = 0;   // magnitudes compare as their bits do
 #pragma unroll
         for (int k = 0; k < EPL; ++k) {
-          x[k] = __uint_as_float(k & 1 ? q_raw[i][k / 2] & 0xffff0000u : q_raw[i][k / 2] << 16);
-          amax = fmaxf(amax, fabsf(x[k]));
-          fine = fine && isfinite(x[k]);
+          const uint32_t bits = k & 1 ? q_raw[i][k / 2] & 0xffff0000u : q_raw[i][k / 2] << 16;
+          x[k] = __uint_as_float(bits);
+          top = max(top, bits & 0x7fffffffu);
         }
-        amax = warp_max(amax);
-        fine = __all_sync(0xffffffffu, fine);
-        const int e = fine ? scale_exp(amax) : 0;
+        top = __reduce_max_sync(0xffffffffu, top);
+        const bool fine = top < 0x7f800000u;   // no infinity or NaN
+        const int e = fine ? scale_exp(top) : 0;
         const float inv = exp2i(-e);
         // pairs of codes, packed to the lane's EPL bytes
         uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
