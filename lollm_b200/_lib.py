@@ -167,8 +167,11 @@ def ptr(t) -> int:
 
 
 def stream_handle(stream=None) -> int:
-    s = torch.cuda.current_stream() if stream is None else stream
-    return s.cuda_stream
+    """cudaStream_t of `stream`, or of the current stream of the current device (asked for without
+    building a Stream object: 0.2 µs instead of 3.2 on every call)."""
+    if stream is not None:
+        return stream.cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def require_cuda(t: torch.Tensor, name: str):

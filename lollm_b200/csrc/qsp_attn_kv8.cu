@@ -10,16 +10,16 @@ namespace qsp {
 namespace kv8 {
 
 // ------------------------------------------------------------------ prep
-// Two kinds of CTA (128 threads) in one launch. The first n_kv_jobs quantise: one (sequence, touched
-// block of tokens, kv head, K or V) each, so that the block's largest magnitude is reduced and its
-// scale and earlier codes are rewritten by one CTA, without atomics. The others norm and rotate q,
-// a warp per (token row, head). A few µs of latency bound the small calls; the chunk of a prompt is
-// bound by its bytes, 9/10 of them q in and out.
+// Two kinds of CTA (8 warps) in one launch. The first n_kv_jobs quantise: one (sequence, touched block
+// of tokens, kv head, K or V) each, so that the block's largest magnitude is reduced and its scale
+// and earlier codes are rewritten by one CTA, without atomics. The others norm and rotate q, two token
+// rows each, a warp four heads at a time (8 KB a row in flight). A lane holds HD/32 consecutive dims of
+// a row; the rotation's other half is the same element of another lane.
 //
 // k is normed and rotated in fp64: with 3 mantissa bits a value next to a rounding border would
 // otherwise fall to either side with the order of the sum, and a cached code lives as long as its
 // sequence. There are 1/8 as many k as q heads, and B200 runs fp64 at half the fp32 rate.
-constexpr int PREP_THREADS = 128;
+constexpr int PREP_WARPS = 8, PREP_ROWS = 2, PREP_HEADS = 4;
 
 // EPL codes of a lane, EPL bytes at dst + lane·EPL
 template <int EPL>
@@ -31,91 +31,104 @@ __device__ __forceinline__ void store_codes(uint8_t* dst, int lane, const float 
   store_bytes<EPL>(dst + lane * EPL, c[0], c[1]);
 }
 
-// one head's row in F (float for q, double for k): norm, times 1 + w, rotate the first rd dims
-template <typename T, int HD, typename F>
-__device__ __forceinline__ void norm_rotate(const qsp_attn_kv8_layer& L, const float (&x)[HD / 32], const T* w, int pos, int lane,
-                                            F* xs, F (&y)[HD / 32]) {
-  constexpr int EPL = HD / 32;
+// a lane's elements of a row, 16-byte aligned or by themselves
+template <typename T, int EPL>
+__device__ __forceinline__ void store_row(T* p, int lane, const float (&y)[EPL]) {
+  T* dst = p + lane * EPL;
+  if constexpr (sizeof(T) == 4) {
+    if constexpr (EPL % 4 == 0) {
+#pragma unroll
+      for (int i = 0; i < EPL; i += 4) *reinterpret_cast<float4*>(dst + i) = make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) dst[i] = dt<T>::from_f(y[i]);
+    }
+  } else {
+    uint32_t o[EPL > 1 ? EPL / 2 : 1];
+#pragma unroll
+    for (int i = 0; i < EPL; i += 2) {
+      const __nv_bfloat162 v = __floats2bfloat162_rn(y[i], EPL > 1 ? y[EPL > 1 ? i + 1 : 0] : 0.f);
+      o[i / 2] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+    if constexpr (EPL == 8) *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+    else if constexpr (EPL == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(o[0], o[1]);
+    else if constexpr (EPL == 2) *reinterpret_cast<uint32_t*>(dst) = o[0];
+    else *dst = dt<T>::from_f(y[0]);
+  }
+}
+
+// x -> RMS-normed times 1 + w, in F (float for q, double for k)
+template <typename T, int EPL, typename F>
+__device__ __forceinline__ void norm_row(const Row<T, EPL>& x, const Row<T, EPL>& w, float eps, F (&y)[EPL]) {
   F ss = 0;
 #pragma unroll
   for (int i = 0; i < EPL; ++i) ss += (F)x[i] * (F)x[i];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  const F inv = rsqrt(ss / (F)HD + (F)L.eps);
-  const int rd = L.rotary_dim, half = rd / 2;
-  __syncwarp();   // the warp's previous row has been read
+  const F inv = rsqrt(ss / (F)(32 * EPL) + (F)eps);
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    const int d = lane * EPL + i;
-    y[i] = (F)x[i] * inv * ((F)dt<T>::to_f(w[d]) + (F)1);
-    if (d < rd) xs[d] = y[i];
-  }
-  __syncwarp();
-  if (lane * EPL < rd) {
-    const T* cosr = static_cast<const T*>(L.rope_cos) + (int64_t)pos * rd;
-    const T* sinr = static_cast<const T*>(L.rope_sin) + (int64_t)pos * rd;
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) {
-      const int d = lane * EPL + i;
-      if (d < rd) {
-        const F r = d < half ? -xs[d + half] : xs[d - half];
-        y[i] = y[i] * (F)dt<T>::to_f(cosr[d]) + r * (F)dt<T>::to_f(sinr[d]);
-      }
-    }
-  }
+  for (int i = 0; i < EPL; ++i) y[i] = (F)x[i] * inv * ((F)w[i] + (F)1);
 }
 
-template <int EPL>
-__device__ __forceinline__ bool warp_finite(const float (&x)[EPL]) {
-  bool ok = true;
+// the first rd dims rotated: y[d] <- y[d]·cos[d] + (d < half ? -y[d + half] : y[d - half])·sin[d]; half is a
+// whole number of lanes. cs, sn: a lane's entries of the position's table row.
+template <typename T, int EPL, typename F>
+__device__ __forceinline__ void rotate_row(F (&y)[EPL], const Row<T, EPL>& cs, const Row<T, EPL>& sn, int rd, int lane) {
+  const int lanes = rd / 2 / EPL, d = lane * EPL;
+  const bool low = d < rd / 2, in = d < rd;
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) ok = ok && isfinite(x[i]);
-  return __all_sync(0xffffffffu, ok);
+  for (int i = 0; i < EPL; ++i) {
+    const F other = __shfl_sync(0xffffffffu, y[i], low ? lane + lanes : lane - lanes);
+    if (in) y[i] = y[i] * (F)cs[i] + (low ? -other : other) * (F)sn[i];
+  }
 }
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(PREP_THREADS) prep_kernel(const qsp_attn_kv8_layer L, int n_kv_jobs, int most, bool vec) {
+__global__ void __launch_bounds__(32 * PREP_WARPS, HD == 256 ? 3 : 4)
+prep_kernel(const qsp_attn_kv8_layer L, int n_kv_jobs, int most, bool vec, bool vec_w, bool vec_rope) {
   pdl_trigger();
-  pdl_wait();
   constexpr int EPL = HD / 32;
-  __shared__ double xs[4][HD];
-  __shared__ float red[4];
+  __shared__ uint32_t red[PREP_WARPS];
   extern __shared__ float vals[];   // [scale_block][HD] of a quantising CTA
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int nh = L.n_heads, nkv = L.n_kv_heads;
+  const int nh = L.n_heads, nkv = L.n_kv_heads, rd = L.rotary_dim;
   const T* qkv = static_cast<const T*>(L.qkv);
+  const bool is_q = (int)blockIdx.x >= n_kv_jobs;
+  Row<T, EPL> w, cs, sn;   // weights do not change: read before the wait
+  w.load(static_cast<const T*>(is_q ? L.q_norm_w : L.k_norm_w), lane, vec_w);
+  pdl_wait();
+  auto load_rope = [&](int pos) {
+    if (lane * EPL < rd) {
+      cs.load(static_cast<const T*>(L.rope_cos) + (int64_t)pos * rd, lane, vec_rope);
+      sn.load(static_cast<const T*>(L.rope_sin) + (int64_t)pos * rd, lane, vec_rope);
+    }
+  };
 
-  if ((int)blockIdx.x >= n_kv_jobs) {
-    const int64_t idx = ((int64_t)blockIdx.x - n_kv_jobs) * 4 + warp;
-    if (idx >= (int64_t)L.batch * L.tokens * nh) return;
-    const int64_t m = idx / nh;
-    const int h = (int)(idx - m * nh);
-    const long long pos = (long long)L.seq_lens[m / L.tokens] + m % L.tokens;
-    float x[EPL], y[EPL];
-    load_row<T, EPL>(qkv + m * L.ld_qkv + (int64_t)h * 2 * HD, lane, vec, x);
-    // a position outside the table is flagged by the quantising CTAs; its q is rotated as position 0
-    norm_rotate<T, HD, float>(L, x, static_cast<const T*>(L.q_norm_w), pos >= 0 && pos < L.rope_rows ? (int)pos : 0, lane,
-                              reinterpret_cast<float*>(xs[warp]), y);
-    T* dst = static_cast<T*>(L.q_buf) + (m * nh + h) * HD + lane * EPL;
-    if constexpr (sizeof(T) == 4) {
-      if constexpr (EPL % 4 == 0) {
+  if (is_q) {
+    constexpr int WPR = PREP_WARPS / PREP_ROWS;   // warps of a row
+    const int64_t m = (int64_t)(blockIdx.x - n_kv_jobs) * PREP_ROWS + warp / WPR;
+    if (m >= (int64_t)L.batch * L.tokens) return;
+    const int b = (int)(m / L.tokens);
+    const int len = L.seq_lens[b];
+    for (int h0 = warp % WPR; h0 < nh; h0 += WPR * PREP_HEADS) {
+      Row<T, EPL> x[PREP_HEADS];
 #pragma unroll
-        for (int i = 0; i < EPL; i += 4) *reinterpret_cast<float4*>(dst + i) = make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < EPL; ++i) dst[i] = dt<T>::from_f(y[i]);
+      for (int i = 0; i < PREP_HEADS; ++i)
+        if (h0 + i * WPR < nh) x[i].load(qkv + m * L.ld_qkv + (int64_t)(h0 + i * WPR) * 2 * HD, lane, vec);
+      if (h0 < WPR) {
+        // a position outside the table is flagged by the quantising CTAs; its q is rotated as position 0
+        const long long at = (long long)len + (m - (int64_t)b * L.tokens);
+        load_rope(at >= 0 && at < L.rope_rows ? (int)at : 0);
       }
-    } else {
-      uint32_t o[EPL > 1 ? EPL / 2 : 1];
 #pragma unroll
-      for (int i = 0; i < EPL; i += 2) {
-        const __nv_bfloat162 v = __floats2bfloat162_rn(y[i], EPL > 1 ? y[EPL > 1 ? i + 1 : 0] : 0.f);
-        o[i / 2] = *reinterpret_cast<const uint32_t*>(&v);
+      for (int i = 0; i < PREP_HEADS; ++i) {
+        if (h0 + i * WPR < nh) {
+          float y[EPL];
+          norm_row<T, EPL, float>(x[i], w, L.eps, y);
+          rotate_row<T, EPL, float>(y, cs, sn, rd, lane);
+          store_row<T, EPL>(static_cast<T*>(L.q_buf) + (m * nh + h0 + i * WPR) * HD, lane, y);
+        }
       }
-      if constexpr (EPL == 8) *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
-      else if constexpr (EPL == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(o[0], o[1]);
-      else if constexpr (EPL == 2) *reinterpret_cast<uint32_t*>(dst) = o[0];
-      else *dst = dt<T>::from_f(y[0]);
     }
     return;
   }
@@ -131,66 +144,80 @@ __global__ void __launch_bounds__(PREP_THREADS) prep_kernel(const qsp_attn_kv8_l
   const long long p0 = max(base, 0ll);                   // a negative length: positions below 0 are left out
   const long long blk = p0 / sb + job % most;
   const long long lo = max(p0, blk * sb);
-  long long hi = min(base + L.tokens, (blk + 1) * sb);
+  const long long hi = min(base + L.tokens, (blk + 1) * sb);
   const bool any = lo < hi;
   const long long lp = lo / L.page_size;
   int page = -1;
   if (any && lo < L.rope_rows && lp < L.max_pages) page = L.page_table[(int64_t)b * L.max_pages + lp];
+  const int n_new = (int)(min(hi, (long long)L.rope_rows) - lo);
+  // a warp's first token while the page is looked up
+  Row<T, EPL> x, v;
+  auto load_token = [&](int j) {
+    const T* row = qkv + ((int64_t)b * L.tokens + (lo + j - base)) * L.ld_qkv + (int64_t)nh * 2 * HD + (int64_t)g * HD;
+    v.load(row + (int64_t)nkv * HD, lane, vec);
+    if (!is_v) {
+      x.load(row, lane, vec);
+      load_rope((int)lo + j);
+    }
+  };
+  if (warp < n_new) load_token(warp);
   const bool ok = page >= 0 && page < L.num_pages;
   if (threadIdx.x == 0 && L.bad_index != nullptr && (base < 0 || (any && (!ok || hi > L.rope_rows)))) *L.bad_index = 1;
   if (!ok) return;
-  hi = min(hi, (long long)L.rope_rows);
-  const int n_new = (int)(hi - lo), n_old = (int)(lo - blk * sb);
+  const int n_old = (int)(lo - blk * sb);
   const int slot0 = (int)(blk * sb % L.page_size);
   uint8_t* codes = static_cast<uint8_t*>(is_v ? L.v_pages : L.k_pages) + (((int64_t)page * nkv + g) * L.page_size + slot0) * HD;
   float* scale = (is_v ? L.v_scales : L.k_scales) + ((int64_t)page * nkv + g) * (L.page_size / sb) + slot0 / sb;
   const int e_old = n_old > 0 ? exp_of(*scale) : -128;
 
-  float amax = 0.f;
-  for (int j = warp; j < n_new; j += 4) {
-    const int pos = (int)lo + j;
-    const T* row = qkv + ((int64_t)b * L.tokens + (pos - base)) * L.ld_qkv + (int64_t)nh * 2 * HD + (int64_t)g * HD;
-    float v[EPL];
-    load_row<T, EPL>(row + (int64_t)nkv * HD, lane, vec, v);
-    bool fine = warp_finite(v);
+  uint32_t amax = 0;
+  for (int j = warp; j < n_new; j += PREP_WARPS) {
+    if (j != warp) load_token(j);
+    const bool v_fine = __reduce_max_sync(0xffffffffu, v.top()) < NOT_FINITE;
     float y[EPL];
     if (is_v) {
 #pragma unroll
-      for (int i = 0; i < EPL; ++i) y[i] = fine ? v[i] : 0.f;
+      for (int k = 0; k < EPL; ++k) y[k] = v_fine ? v[k] : 0.f;
     } else {
-      float x[EPL];
       double z[EPL];
-      load_row<T, EPL>(row, lane, vec, x);
-      norm_rotate<T, HD, double>(L, x, static_cast<const T*>(L.k_norm_w), pos, lane, xs[warp], z);
+      norm_row<T, EPL, double>(x, w, L.eps, z);
+      rotate_row<T, EPL, double>(z, cs, sn, rd, lane);
+      uint32_t top = 0;
 #pragma unroll
-      for (int i = 0; i < EPL; ++i) y[i] = (float)z[i];
-      fine = warp_finite(y) && fine;
+      for (int k = 0; k < EPL; ++k) {
+        y[k] = (float)z[k];
+        top = max(top, __float_as_uint(y[k]) & 0x7fffffffu);
+      }
+      const bool fine = __reduce_max_sync(0xffffffffu, top) < NOT_FINITE && v_fine;
 #pragma unroll
-      for (int i = 0; i < EPL; ++i) y[i] = fine ? y[i] : NAN;
+      for (int k = 0; k < EPL; ++k) y[k] = fine ? y[k] : NAN;
     }
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) {
-      vals[j * HD + lane * EPL + i] = y[i];
-      amax = fmaxf(amax, fabsf(y[i]));   // NaN is passed over
+    for (int k = 0; k < EPL; ++k) {
+      vals[j * HD + lane * EPL + k] = y[k];
+      const uint32_t bits = __float_as_uint(y[k]) & 0x7fffffffu;
+      amax = max(amax, bits < NOT_FINITE ? bits : 0u);   // NaN is passed over
     }
   }
-  amax = warp_max(amax);
+  amax = __reduce_max_sync(0xffffffffu, amax);
   if (lane == 0) red[warp] = amax;
   __syncthreads();
-  amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  const int e = min(max(scale_exp(__float_as_uint(amax)), e_old), MAX_EXP);
+  amax = red[0];
+#pragma unroll
+  for (int i = 1; i < PREP_WARPS; ++i) amax = max(amax, red[i]);
+  const int e = min(max(scale_exp(amax), e_old), MAX_EXP);
   if (threadIdx.x == 0) *scale = exp2i(e);
   if (e_old < e && n_old > 0) {   // earlier tokens of the block take the larger scale
     const float f = ldexpf(1.f, e_old - e);
     uint32_t* c4 = reinterpret_cast<uint32_t*>(codes);
-    for (int k = threadIdx.x; k < n_old * (HD / 4); k += PREP_THREADS) {
+    for (int k = threadIdx.x; k < n_old * (HD / 4); k += 32 * PREP_WARPS) {
       const uint32_t c = c4[k];
       const float2 a = from_e4m3x2((uint16_t)c), z = from_e4m3x2((uint16_t)(c >> 16));
       c4[k] = (uint32_t)to_e4m3x2(a.x * f, a.y * f) | (uint32_t)to_e4m3x2(z.x * f, z.y * f) << 16;
     }
   }
   const float inv = exp2i(-e);
-  for (int j = warp; j < n_new; j += 4) {   // a warp's own rows of vals
+  for (int j = warp; j < n_new; j += PREP_WARPS) {   // a warp's own rows of vals
     float y[EPL];
 #pragma unroll
     for (int i = 0; i < EPL; ++i) y[i] = vals[j * HD + lane * EPL + i];
@@ -203,18 +230,20 @@ static int launch_prep(const qsp_attn_kv8_layer& L, cudaStream_t st) {
   const int sb = L.scale_block;
   const int64_t most = (L.tokens + sb - 2) / sb + 1;    // blocks that T tokens can touch
   const int64_t jobs = 2 * most * L.n_kv_heads * L.batch;
-  const int64_t rows = ((int64_t)L.batch * L.tokens * L.n_heads + 3) / 4;
+  const int64_t rows = ((int64_t)L.batch * L.tokens + PREP_ROWS - 1) / PREP_ROWS;
   QSP_REQUIRE(jobs + rows < (1ll << 31), "qsp_attn_kv8_prep: too many tokens for one call");
   constexpr int A = std::min<int>(16, HD / 32 * sizeof(T));
   const bool vec = aligned(L.qkv, A) && (L.ld_qkv * (int64_t)sizeof(T)) % A == 0;
+  const bool vec_w = aligned(L.q_norm_w, A) && aligned(L.k_norm_w, A);
+  const bool vec_rope = aligned(L.rope_cos, A) && aligned(L.rope_sin, A) && (L.rotary_dim * (int64_t)sizeof(T)) % A == 0;
   const size_t smem = (size_t)sb * HD * sizeof(float);
   auto kern = prep_kernel<T, HD>;
-  if (smem > 32 * 1024) {   // with the static arrays past the 48 KB that need no leave
+  if (smem > 40 * 1024) {   // past the 48 KB that need no leave
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return set_error(QSP_ERR_CUDA, "qsp_attn_kv8_prep: %s", cudaGetErrorString(e));
   }
-  return launch_pdl("qsp_attn_kv8_prep", kern, dim3((unsigned)(jobs + rows)), dim3(PREP_THREADS), smem, st, L, (int)jobs,
-                    (int)most, vec);
+  return launch_pdl("qsp_attn_kv8_prep", kern, dim3((unsigned)(jobs + rows)), dim3(32 * PREP_WARPS), smem, st, L, (int)jobs,
+                    (int)most, vec, vec_w, vec_rope);
 }
 
 // ------------------------------------------------------------------ attention on CUDA cores
@@ -424,13 +453,13 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS, 4) merge_kernel(const qsp_at
   const int per = WIDE ? (np + MERGE_WARPS - 1) / MERGE_WARPS : np;
   const int q_begin = WIDE ? warp * per : 0, q_end = min(np, q_begin + per);
   for (int q0 = q_begin; q0 < q_end; q0 += DEPTH) {
-    float v[DEPTH][EPL];
+    Row<float, EPL> v[DEPTH];
     float2 ml[DEPTH];
 #pragma unroll
     for (int u = 0; u < DEPTH; ++u) {
       if (q0 + u < q_end) {
         ml[u] = ws.ml[slot(q0 + u)];
-        load_row<float, EPL>(ws.o + slot(q0 + u) * HD, lane, true, v[u]);
+        v[u].load(ws.o + slot(q0 + u) * HD, lane, true);
       }
     }
 #pragma unroll
@@ -517,7 +546,8 @@ static int validate(const char* what, const qsp_attn_kv8_layer* p, bool verify) 
   if (!verify) {
     QSP_REQUIRE(L.q_norm_w && L.k_norm_w && (L.rotary_dim == 0 || (L.rope_cos && L.rope_sin)) && L.rope_rows > 0,
                 "%s: null pointer or empty RoPE table", what);
-    QSP_REQUIRE(L.rotary_dim >= 0 && L.rotary_dim <= L.head_dim && L.rotary_dim % 2 == 0, "%s: bad rotary_dim", what);
+    QSP_REQUIRE(L.rotary_dim >= 0 && L.rotary_dim <= L.head_dim && L.rotary_dim % (L.head_dim / 16) == 0,
+                "%s: rotary_dim %d must be a multiple of head_dim / 16, head_dim at most", what, L.rotary_dim);
     return QSP_OK;
   }
   const size_t need = qsp_attn_kv8_workspace_bytes(L.batch, L.tokens, L.n_heads, L.n_kv_heads, L.head_dim, L.dtype);

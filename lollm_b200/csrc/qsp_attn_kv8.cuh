@@ -29,43 +29,55 @@ __device__ __forceinline__ __half2 e4m3x2_to_half2(uint16_t v) {
 __device__ __forceinline__ float2 from_e4m3x2(uint16_t v) { return __half22float2(e4m3x2_to_half2(v)); }
 
 // ---------------------------------------------------------------- a lane's elements of a row
-// EPL elements at p + lane·EPL; vec: that address is a multiple of min(16, EPL elements)
+// EPL elements at p + lane·EPL, kept as they are in memory (bf16: pairs, the low half first, each the upper
+// half of an fp32)
 template <typename T, int EPL>
-__device__ __forceinline__ void load_row(const T* p, int lane, bool vec, float (&x)[EPL]) {
-  const T* src = p + lane * EPL;
-  if constexpr (sizeof(T) == 4 && EPL % 4 == 0) {
-    if (vec) {
-#pragma unroll
-      for (int i = 0; i < EPL; i += 4) {
-        const float4 v = *reinterpret_cast<const float4*>(src + i);
-        x[i] = v.x, x[i + 1] = v.y, x[i + 2] = v.z, x[i + 3] = v.w;
-      }
-      return;
-    }
+struct Row {
+  static constexpr int W = EPL * (int)sizeof(T) >= 4 ? EPL * (int)sizeof(T) / 4 : 1;
+  uint32_t r[W];
+  __device__ __forceinline__ float operator[](int i) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(r[i]);
+    return __uint_as_float(i & 1 ? r[i / 2] & 0xffff0000u : r[i / 2] << 16);
   }
-  if constexpr (sizeof(T) == 2 && EPL > 1) {
-    if (vec) {
-      uint32_t v[EPL / 2];   // bf16 pairs: the low half first, each the upper half of an fp32
-      if constexpr (EPL == 8) {
-        const uint4 u = *reinterpret_cast<const uint4*>(src);
-        v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
-      } else if constexpr (EPL == 4) {
+  // vec: the address is a multiple of min(16 bytes, EPL elements)
+  __device__ __forceinline__ void load(const T* p, int lane, bool vec) {
+    const T* src = p + lane * EPL;
+    if (vec && W > 1) {
+      if constexpr (W % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < W; i += 4) {
+          const uint4 u = reinterpret_cast<const uint4*>(src)[i / 4];
+          r[i] = u.x, r[i + 1] = u.y, r[i + 2] = u.z, r[i + 3] = u.w;
+        }
+      } else if constexpr (W == 2) {
         const uint2 u = *reinterpret_cast<const uint2*>(src);
-        v[0] = u.x, v[1] = u.y;
-      } else {
-        v[0] = *reinterpret_cast<const uint32_t*>(src);
-      }
-#pragma unroll
-      for (int i = 0; i < EPL; i += 2) {
-        x[i] = __uint_as_float(v[i / 2] << 16);
-        x[i + 1] = __uint_as_float(v[i / 2] & 0xffff0000u);
+        r[0] = u.x, r[1] = u.y;
       }
       return;
     }
-  }
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) x[i] = dt<T>::to_f(src[i]);
-}
+      for (int i = 0; i < EPL; ++i) r[i] = __float_as_uint(src[i]);
+    } else {
+      const uint16_t* h = reinterpret_cast<const uint16_t*>(src);
+#pragma unroll
+      for (int i = 0; i < W; ++i) r[i] = h[2 * i] | (EPL > 1 ? (uint32_t)h[EPL > 1 ? 2 * i + 1 : 0] << 16 : 0u);
+    }
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < W; ++i) r[i] = 0;
+  }
+  // bits of the largest magnitude (they compare as the values do; 0x7f800000 and over: not finite)
+  __device__ __forceinline__ uint32_t top() const {
+    uint32_t t = 0;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) t = max(t, __float_as_uint((*this)[i]) & 0x7fffffffu);
+    return t;
+  }
+};
+constexpr uint32_t NOT_FINITE = 0x7f800000u;
+
 // N = 1, 2, 4 or 8 bytes, a first
 template <int N>
 __device__ __forceinline__ void store_bytes(uint8_t* dst, uint32_t a, uint32_t b) {

@@ -156,23 +156,6 @@ __device__ __forceinline__ void wait_bar(uint64_t* bar, uint32_t parity, volatil
     if ((++n & 255u) == 0 && give_up(n, abort)) return;
 }
 
-// EPL bf16 of a row at p + lane·EPL, as they are
-template <int EPL>
-__device__ __forceinline__ void load_raw(const __nv_bfloat16* p, int lane, uint32_t (&r)[EPL > 1 ? EPL / 2 : 1]) {
-  const __nv_bfloat16* src = p + lane * EPL;
-  if constexpr (EPL == 8) {
-    const uint4 u = *reinterpret_cast<const uint4*>(src);
-    r[0] = u.x, r[1] = u.y, r[2] = u.z, r[3] = u.w;
-  } else if constexpr (EPL == 4) {
-    const uint2 u = *reinterpret_cast<const uint2*>(src);
-    r[0] = u.x, r[1] = u.y;
-  } else if constexpr (EPL == 2) {
-    r[0] = *reinterpret_cast<const uint32_t*>(src);
-  } else {
-    r[0] = *reinterpret_cast<const uint16_t*>(src);
-  }
-}
-
 // ---------------------------------------------------------------- TMEM, 8 columns of this warp's 32 lanes
 __device__ __forceinline__ void tm_ld8(uint32_t t, uint32_t (&r)[8]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
@@ -494,17 +477,16 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
     // Q of a piece: a warp per row, loaded one tile before it is staged (4 rows: when it is; registers are short)
     constexpr int ROWS = R / (4 * NWG);
     constexpr bool AHEAD = ROWS <= 2;
-    uint32_t q_raw[ROWS][EPL > 1 ? EPL / 2 : 1];
+    Row<__nv_bfloat16, EPL> q_raw[ROWS];
     auto load_q = [&](const Desc& q) {
 #pragma unroll
       for (int i = 0; i < ROWS; ++i) {
         const int rr = q.row0 + warp + i * 4 * NWG;
         if (rr < rows_total) {
           const int t = rr / nrep, hq = q.g * nrep + rr - t * nrep;
-          load_raw<EPL>(static_cast<const __nv_bfloat16*>(L.q_buf) + (((int64_t)q.b * L.tokens + t) * L.n_heads + hq) * HD, lane, q_raw[i]);
+          q_raw[i].load(static_cast<const __nv_bfloat16*>(L.q_buf) + (((int64_t)q.b * L.tokens + t) * L.n_heads + hq) * HD, lane, true);
         } else {
-#pragma unroll
-          for (int k = 0; k < (EPL > 1 ? EPL / 2 : 1); ++k) q_raw[i][k] = 0;
+          q_raw[i].zero();
         }
       }
     };
@@ -512,23 +494,15 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
 #pragma unroll
       for (int i = 0; i < ROWS; ++i) {
         const int r = warp + i * 4 * NWG, row = r / RW * (2 * RW) + r % RW;
-        float x[EPL];
-        uint32_t top = 0;   // magnitudes compare as their bits do
-#pragma unroll
-        for (int k = 0; k < EPL; ++k) {
-          const uint32_t bits = k & 1 ? q_raw[i][k / 2] & 0xffff0000u : q_raw[i][k / 2] << 16;
-          x[k] = __uint_as_float(bits);
-          top = max(top, bits & 0x7fffffffu);
-        }
-        top = __reduce_max_sync(0xffffffffu, top);
-        const bool fine = top < 0x7f800000u;   // no infinity or NaN
+        const uint32_t top = __reduce_max_sync(0xffffffffu, q_raw[i].top());
+        const bool fine = top < NOT_FINITE;
         const int e = fine ? scale_exp(top) : 0;
         const float inv = exp2i(-e);
         // pairs of codes, packed to the lane's EPL bytes
         uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
 #pragma unroll
         for (int k = 0; k < EPL; k += 2) {
-          const float a = fine ? x[k] * inv : 0.f, z = fine && EPL > 1 ? x[EPL > 1 ? k + 1 : 0] * inv : 0.f;
+          const float a = fine ? q_raw[i][k] * inv : 0.f, z = fine && EPL > 1 ? q_raw[i][EPL > 1 ? k + 1 : 0] * inv : 0.f;
           const uint16_t h = to_e4m3x2(a, z);
           const float2 f = from_e4m3x2(h);
           hi[k / 4] |= (uint32_t)h << (k % 4 * 8);

@@ -42,7 +42,7 @@ def test_both_entry_points_refuse(field, value):
         assert fn(None, None) == L.QSP_ERR_INVALID
 
 
-@pytest.mark.parametrize("field,value", [("rotary_dim", 63), ("rotary_dim", 258), ("rope_rows", 0), ("rope_cos", 0), ("k_norm_w", 0)])
+@pytest.mark.parametrize("field,value", [("rotary_dim", 63), ("rotary_dim", 258), ("rotary_dim", 72), ("rope_rows", 0), ("rope_cos", 0), ("k_norm_w", 0)])
 def test_prep_refuses(field, value):
     d = _layer()
     setattr(d, field, value)
