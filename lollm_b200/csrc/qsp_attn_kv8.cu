@@ -10,9 +10,9 @@ namespace qsp {
 namespace kv8 {
 
 // ------------------------------------------------------------------ prep
-// Two kinds of CTA (8 warps) in one launch. The first n_kv_jobs quantise: one (sequence, touched block
-// of tokens, kv head, K or V) each, so that the block's largest magnitude is reduced and its scale
-// and earlier codes are rewritten by one CTA, without atomics. The others norm and rotate q, two token
+// Two kinds of CTA (8 warps) in one launch. The first n_kv_jobs quantise: K and V of one (sequence,
+// touched block of tokens, kv head) each, a warp a token, so that the block's largest magnitudes are
+// reduced and its scales and earlier codes are rewritten by one CTA, without atomics. The others norm and rotate q, two token
 // rows each, a warp four heads at a time (8 KB a row in flight). A lane holds HD/32 consecutive dims of
 // a row; the rotation's other half is the same element of another lane.
 //
@@ -84,12 +84,12 @@ __device__ __forceinline__ void rotate_row(F (&y)[EPL], const Row<T, EPL>& cs, c
 }
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(32 * PREP_WARPS, HD == 256 ? 3 : 4)
+__global__ void __launch_bounds__(32 * PREP_WARPS, 4)
 prep_kernel(const qsp_attn_kv8_layer L, int n_kv_jobs, int most, bool vec, bool vec_w, bool vec_rope) {
   pdl_trigger();
   constexpr int EPL = HD / 32;
-  __shared__ uint32_t red[PREP_WARPS];
-  extern __shared__ float vals[];   // [scale_block][HD] of a quantising CTA
+  __shared__ uint32_t red[2][PREP_WARPS];
+  extern __shared__ float keys[];   // [scale_block][HD] of a quantising CTA
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int nh = L.n_heads, nkv = L.n_kv_heads, rd = L.rotary_dim;
   const T* qkv = static_cast<const T*>(L.qkv);
@@ -135,8 +135,6 @@ prep_kernel(const qsp_attn_kv8_layer L, int n_kv_jobs, int most, bool vec, bool 
 
   // ---- quantise one block of one head
   int job = blockIdx.x;
-  const bool is_v = job & 1;
-  job >>= 1;
   const int g = job % nkv;
   job /= nkv;
   const int b = job / most, sb = L.scale_block;
@@ -150,78 +148,82 @@ prep_kernel(const qsp_attn_kv8_layer L, int n_kv_jobs, int most, bool vec, bool 
   int page = -1;
   if (any && lo < L.rope_rows && lp < L.max_pages) page = L.page_table[(int64_t)b * L.max_pages + lp];
   const int n_new = (int)(min(hi, (long long)L.rope_rows) - lo);
-  // a warp's first token while the page is looked up
   Row<T, EPL> x, v;
-  auto load_token = [&](int j) {
-    const T* row = qkv + ((int64_t)b * L.tokens + (lo + j - base)) * L.ld_qkv + (int64_t)nh * 2 * HD + (int64_t)g * HD;
-    v.load(row + (int64_t)nkv * HD, lane, vec);
-    if (!is_v) {
-      x.load(row, lane, vec);
-      load_rope((int)lo + j);
-    }
+  auto k_row = [&](int j) {
+    return qkv + ((int64_t)b * L.tokens + (lo + j - base)) * L.ld_qkv + (int64_t)nh * 2 * HD + (int64_t)g * HD;
   };
-  if (warp < n_new) load_token(warp);
+  auto load_token = [&](int j) {
+    x.load(k_row(j), lane, vec);
+    v.load(k_row(j) + (int64_t)nkv * HD, lane, vec);
+    load_rope((int)lo + j);
+  };
+  if (warp < n_new) load_token(warp);   // a warp's first token while the page is looked up
   const bool ok = page >= 0 && page < L.num_pages;
   if (threadIdx.x == 0 && L.bad_index != nullptr && (base < 0 || (any && (!ok || hi > L.rope_rows)))) *L.bad_index = 1;
   if (!ok) return;
   const int n_old = (int)(lo - blk * sb);
   const int slot0 = (int)(blk * sb % L.page_size);
-  uint8_t* codes = static_cast<uint8_t*>(is_v ? L.v_pages : L.k_pages) + (((int64_t)page * nkv + g) * L.page_size + slot0) * HD;
-  float* scale = (is_v ? L.v_scales : L.k_scales) + ((int64_t)page * nkv + g) * (L.page_size / sb) + slot0 / sb;
-  const int e_old = n_old > 0 ? exp_of(*scale) : -128;
+  const int64_t ph = (int64_t)page * nkv + g;
+  uint8_t* codes[2] = {static_cast<uint8_t*>(L.k_pages) + (ph * L.page_size + slot0) * HD,
+                       static_cast<uint8_t*>(L.v_pages) + (ph * L.page_size + slot0) * HD};
+  float* scale[2] = {L.k_scales + ph * (L.page_size / sb) + slot0 / sb, L.v_scales + ph * (L.page_size / sb) + slot0 / sb};
+  int e_old[2] = {-128, -128};
+  if (n_old > 0) e_old[0] = exp_of(*scale[0]), e_old[1] = exp_of(*scale[1]);
 
-  uint32_t amax = 0;
+  uint32_t k_max = 0, v_max = 0;
   for (int j = warp; j < n_new; j += PREP_WARPS) {
     if (j != warp) load_token(j);
-    const bool v_fine = __reduce_max_sync(0xffffffffu, v.top()) < NOT_FINITE;
+    const uint32_t v_top = __reduce_max_sync(0xffffffffu, v.top());
+    double z[EPL];
+    norm_row<T, EPL, double>(x, w, L.eps, z);
+    rotate_row<T, EPL, double>(z, cs, sn, rd, lane);
     float y[EPL];
-    if (is_v) {
-#pragma unroll
-      for (int k = 0; k < EPL; ++k) y[k] = v_fine ? v[k] : 0.f;
-    } else {
-      double z[EPL];
-      norm_row<T, EPL, double>(x, w, L.eps, z);
-      rotate_row<T, EPL, double>(z, cs, sn, rd, lane);
-      uint32_t top = 0;
-#pragma unroll
-      for (int k = 0; k < EPL; ++k) {
-        y[k] = (float)z[k];
-        top = max(top, __float_as_uint(y[k]) & 0x7fffffffu);
-      }
-      const bool fine = __reduce_max_sync(0xffffffffu, top) < NOT_FINITE && v_fine;
-#pragma unroll
-      for (int k = 0; k < EPL; ++k) y[k] = fine ? y[k] : NAN;
-    }
+    uint32_t k_top = 0;
 #pragma unroll
     for (int k = 0; k < EPL; ++k) {
-      vals[j * HD + lane * EPL + k] = y[k];
-      const uint32_t bits = __float_as_uint(y[k]) & 0x7fffffffu;
-      amax = max(amax, bits < NOT_FINITE ? bits : 0u);   // NaN is passed over
+      y[k] = (float)z[k];
+      k_top = max(k_top, __float_as_uint(y[k]) & 0x7fffffffu);
     }
-  }
-  amax = __reduce_max_sync(0xffffffffu, amax);
-  if (lane == 0) red[warp] = amax;
-  __syncthreads();
-  amax = red[0];
+    k_top = __reduce_max_sync(0xffffffffu, k_top);
+    const bool fine = k_top < NOT_FINITE && v_top < NOT_FINITE;
+    if (fine) k_max = max(k_max, k_top);
+    if (v_top < NOT_FINITE) v_max = max(v_max, v_top);
 #pragma unroll
-  for (int i = 1; i < PREP_WARPS; ++i) amax = max(amax, red[i]);
-  const int e = min(max(scale_exp(amax), e_old), MAX_EXP);
-  if (threadIdx.x == 0) *scale = exp2i(e);
-  if (e_old < e && n_old > 0) {   // earlier tokens of the block take the larger scale
-    const float f = ldexpf(1.f, e_old - e);
-    uint32_t* c4 = reinterpret_cast<uint32_t*>(codes);
-    for (int k = threadIdx.x; k < n_old * (HD / 4); k += 32 * PREP_WARPS) {
-      const uint32_t c = c4[k];
-      const float2 a = from_e4m3x2((uint16_t)c), z = from_e4m3x2((uint16_t)(c >> 16));
-      c4[k] = (uint32_t)to_e4m3x2(a.x * f, a.y * f) | (uint32_t)to_e4m3x2(z.x * f, z.y * f) << 16;
+    for (int k = 0; k < EPL; ++k) keys[j * HD + lane * EPL + k] = fine ? y[k] : NAN;
+  }
+  if (lane == 0) {
+    red[0][warp] = k_max;
+    red[1][warp] = v_max;
+  }
+  __syncthreads();
+  int e[2];
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv) {
+    uint32_t top = red[kv][0];
+#pragma unroll
+    for (int i = 1; i < PREP_WARPS; ++i) top = max(top, red[kv][i]);
+    e[kv] = min(max(scale_exp(top), e_old[kv]), MAX_EXP);
+    if (threadIdx.x == 0) *scale[kv] = exp2i(e[kv]);
+    if (e_old[kv] < e[kv] && n_old > 0) {   // earlier tokens of the block take the larger scale
+      const float f = ldexpf(1.f, e_old[kv] - e[kv]);
+      uint32_t* c4 = reinterpret_cast<uint32_t*>(codes[kv]);
+      for (int k = threadIdx.x; k < n_old * (HD / 4); k += 32 * PREP_WARPS) {
+        const uint32_t c = c4[k];
+        const float2 a = from_e4m3x2((uint16_t)c), z = from_e4m3x2((uint16_t)(c >> 16));
+        c4[k] = (uint32_t)to_e4m3x2(a.x * f, a.y * f) | (uint32_t)to_e4m3x2(z.x * f, z.y * f) << 16;
+      }
     }
   }
-  const float inv = exp2i(-e);
-  for (int j = warp; j < n_new; j += PREP_WARPS) {   // a warp's own rows of vals
+  for (int j = warp; j < n_new; j += PREP_WARPS) {   // a warp's own tokens again
     float y[EPL];
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) y[i] = vals[j * HD + lane * EPL + i];
-    store_codes<EPL>(codes + (int64_t)(n_old + j) * HD, lane, y, inv);
+    for (int i = 0; i < EPL; ++i) y[i] = keys[j * HD + lane * EPL + i];
+    store_codes<EPL>(codes[0] + (int64_t)(n_old + j) * HD, lane, y, exp2i(-e[0]));
+    if (n_new > PREP_WARPS) v.load(k_row(j) + (int64_t)nkv * HD, lane, vec);
+    const bool fine = __reduce_max_sync(0xffffffffu, v.top()) < NOT_FINITE;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) y[i] = fine ? v[i] : 0.f;
+    store_codes<EPL>(codes[1] + (int64_t)(n_old + j) * HD, lane, y, exp2i(-e[1]));
   }
 }
 
@@ -229,7 +231,7 @@ template <typename T, int HD>
 static int launch_prep(const qsp_attn_kv8_layer& L, cudaStream_t st) {
   const int sb = L.scale_block;
   const int64_t most = (L.tokens + sb - 2) / sb + 1;    // blocks that T tokens can touch
-  const int64_t jobs = 2 * most * L.n_kv_heads * L.batch;
+  const int64_t jobs = most * L.n_kv_heads * L.batch;
   const int64_t rows = ((int64_t)L.batch * L.tokens + PREP_ROWS - 1) / PREP_ROWS;
   QSP_REQUIRE(jobs + rows < (1ll << 31), "qsp_attn_kv8_prep: too many tokens for one call");
   constexpr int A = std::min<int>(16, HD / 32 * sizeof(T));
