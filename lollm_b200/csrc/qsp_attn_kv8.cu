@@ -250,129 +250,163 @@ static int launch_prep(const qsp_attn_kv8_layer& L, cudaStream_t st) {
 
 // ------------------------------------------------------------------ attention on CUDA cores
 // fp32 throughout: for fp32 models, and for bf16 shapes that the tensor-core kernel does not take.
-// A CTA of 4 warps runs its pieces (see Piece) with 16 query rows, 4 a warp; keys are staged 32 at a
-// time as fp32 values, lane j scores key j. Bound by its shared-memory reads (two per product).
-constexpr int SIMT_R = 16, SIMT_KT = 32, SIMT_THREADS = 128;
+// A CTA of 4 warps runs its pieces (see Piece) with 16 query rows, 4 a warp, and stages 32 keys at a time
+// as fp32 values, the next ones' codes in flight meanwhile. Scores: lane = key, a 16-byte read of K and of
+// each of the 4 queries for 16 products. Values: lane = HD/32 dims, the weights read back from shared memory.
+constexpr int SIMT_R = 16, SIMT_WARPS = 4, SIMT_RPW = SIMT_R / SIMT_WARPS;
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(SIMT_THREADS) simt_kernel(const qsp_attn_kv8_layer L, int n_rg) {
+struct SimtSmem {
+  float q[SIMT_R][HD];
+  float k[SIMT_TILE][HD + 4];   // lanes read 16 bytes a row: the rows' banks step by 4
+  float v[SIMT_TILE][HD];
+  float p[SIMT_WARPS][SIMT_RPW][SIMT_TILE];
+  int sh[36];
+};
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(32 * SIMT_WARPS) simt_kernel(const qsp_attn_kv8_layer L, int n_rg) {
   pdl_trigger();
   pdl_wait();
-  constexpr int DPL = HD / 32, RPW = SIMT_R / 4;
-  extern __shared__ float smem[];
-  __shared__ int sh[36];
-  float* Qs = smem;                       // [16][HD]
-  float* Ks = Qs + SIMT_R * HD;           // [32][HD + 1]
-  float* Vs = Ks + SIMT_KT * (HD + 1);    // [32][HD]
+  constexpr int DPL = HD / 32, RPW = SIMT_RPW, THREADS = 32 * SIMT_WARPS;
+  constexpr int TPK = THREADS / SIMT_TILE, CPT = HD / TPK;   // threads of a key, its codes of each
+  extern __shared__ __align__(16) uint8_t simt_raw[];
+  SimtSmem<T, HD>& sm = *reinterpret_cast<SimtSmem<T, HD>*>(simt_raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int nrep = L.n_heads / L.n_kv_heads, rows_total = nrep * L.tokens;
-  const T* qb = static_cast<const T*>(L.q_buf);
+  const int cap = L.max_pages * L.page_size, nb = L.page_size / L.scale_block;
   const uint8_t* kp = static_cast<const uint8_t*>(L.k_pages);
   const uint8_t* vp = static_cast<const uint8_t*>(L.v_pages);
   const Scratch ws = scratch(L, gridDim.x, SIMT_R);
   const float sl2 = L.scale * LOG2E;
+  const int my_key = tid / TPK, my_dim = tid % TPK * CPT;   // this thread's part of a staged tile
 
-  Walk w = share(L, n_rg, SIMT_R, sh);
+  Walk w = share<SIMT_TILE>(L, n_rg, SIMT_R, sm.sh);
   Piece p;
   p.n = 0;
-  while (next_piece(L, n_rg, SIMT_R, w, p)) {
+  while (next_piece<SIMT_TILE>(L, n_rg, SIMT_R, w, p)) {
     const int row0 = p.rg * SIMT_R, nrows = min(SIMT_R, rows_total - row0);
-    const long long base = p.len;
-    const long long kv_end = min(base + L.tokens, (long long)L.max_pages * L.page_size);
+    const int base = min(p.len, cap), kv_end = min(base + L.tokens, cap);
+    // codes and scales of a tile's key; a key without a page is zeros (and not seen)
+    uint32_t kc[CPT / 4], vc[CPT / 4];
+    float ks, vs;
+    bool mapped;
+    auto fetch = [&](int j) {
+      const int key = (p.j0 + j) * SIMT_TILE + my_key;
+      int page = -1;
+      if (j < p.n && key < kv_end) page = L.page_table[(int64_t)p.b * L.max_pages + key / L.page_size];
+      mapped = page >= 0 && page < L.num_pages;
+      ks = vs = 0.f;
+#pragma unroll
+      for (int i = 0; i < CPT / 4; ++i) kc[i] = vc[i] = 0;
+      if (mapped) {
+        const int slot = key % L.page_size;
+        const int64_t ph = (int64_t)page * L.n_kv_heads + p.g, off = (ph * L.page_size + slot) * HD + my_dim;
+        const int64_t so = ph * nb + slot / L.scale_block;
+        ks = L.k_scales[so];
+        vs = L.v_scales[so];
+#pragma unroll
+        for (int i = 0; i < CPT / 4; ++i) {
+          kc[i] = reinterpret_cast<const uint32_t*>(kp + off)[i];
+          vc[i] = reinterpret_cast<const uint32_t*>(vp + off)[i];
+        }
+      }
+    };
+    fetch(0);
     __syncthreads();   // the previous piece's q has been read
-    for (int e = tid; e < nrows * HD; e += SIMT_THREADS) {
+    for (int e = tid; e < nrows * HD; e += THREADS) {
       const int r = e / HD, d = e % HD, t = (row0 + r) / nrep, hq = p.g * nrep + (row0 + r) % nrep;
-      Qs[r * HD + d] = dt<T>::to_f(qb[(((int64_t)p.b * L.tokens + t) * L.n_heads + hq) * HD + d]);
+      sm.q[r][d] = dt<T>::to_f(static_cast<const T*>(L.q_buf)[(((int64_t)p.b * L.tokens + t) * L.n_heads + hq) * HD + d]);
     }
     float acc[RPW][DPL], mrow[RPW], lrow[RPW];
+    int last[RPW];   // last position the row sees
 #pragma unroll
     for (int i = 0; i < RPW; ++i) {
       mrow[i] = -INFINITY;
       lrow[i] = 0.f;
+      last[i] = base + (row0 + warp * RPW + i) / nrep;
 #pragma unroll
       for (int j = 0; j < DPL; ++j) acc[i][j] = 0.f;
     }
-    const long long k_begin = (long long)p.j0 * TILE, k_end = min(kv_end, k_begin + (long long)p.n * TILE);
-    for (long long k0 = k_begin; k0 < k_end; k0 += SIMT_KT) {
+    for (int j = 0; j < p.n; ++j) {
+      __syncthreads();   // the previous tile has been read
+#pragma unroll
+      for (int i = 0; i < CPT / 4; ++i) {
+        const float2 k01 = from_e4m3x2((uint16_t)kc[i]), k23 = from_e4m3x2((uint16_t)(kc[i] >> 16));
+        const float2 v01 = from_e4m3x2((uint16_t)vc[i]), v23 = from_e4m3x2((uint16_t)(vc[i] >> 16));
+        *reinterpret_cast<float4*>(&sm.k[my_key][my_dim + 4 * i]) = make_float4(k01.x * ks, k01.y * ks, k23.x * ks, k23.y * ks);
+        *reinterpret_cast<float4*>(&sm.v[my_key][my_dim + 4 * i]) = make_float4(v01.x * vs, v01.y * vs, v23.x * vs, v23.y * vs);
+      }
+      if (tid % TPK == 0) sm.p[0][0][my_key] = mapped ? 1.f : 0.f;   // for a moment: which keys there are
       __syncthreads();
-      bool mapped = false;   // key `lane` of this step has a page
-      for (int e = tid; e < SIMT_KT * HD / 4; e += SIMT_THREADS) {
-        const int j = e / (HD / 4), d = e % (HD / 4) * 4;
-        const long long pos = k0 + j;
-        float2 k01 = {0, 0}, k23 = {0, 0}, v01 = {0, 0}, v23 = {0, 0};
-        float ks = 0.f, vs = 0.f;
-        if (pos < k_end) {
-          const int page = L.page_table[(int64_t)p.b * L.max_pages + pos / L.page_size];
-          if (page >= 0 && page < L.num_pages) {
-            const int slot = (int)(pos % L.page_size);
-            const int64_t ph = (int64_t)page * L.n_kv_heads + p.g;
-            const int64_t off = (ph * L.page_size + slot) * HD + d;
-            const uint32_t kc = *reinterpret_cast<const uint32_t*>(kp + off), vc = *reinterpret_cast<const uint32_t*>(vp + off);
-            const int64_t so = ph * (L.page_size / L.scale_block) + slot / L.scale_block;
-            ks = L.k_scales[so];
-            vs = L.v_scales[so];
-            k01 = from_e4m3x2((uint16_t)kc), k23 = from_e4m3x2((uint16_t)(kc >> 16));
-            v01 = from_e4m3x2((uint16_t)vc), v23 = from_e4m3x2((uint16_t)(vc >> 16));
-          }
+      const bool here = sm.p[0][0][lane] != 0.f;
+      if (j + 1 < p.n) fetch(j + 1);
+      __syncthreads();   // p is written below
+      const int key = (p.j0 + j) * SIMT_TILE + lane;
+      float sc[RPW];
+#pragma unroll
+      for (int i = 0; i < RPW; ++i) sc[i] = 0.f;
+#pragma unroll 4
+      for (int d = 0; d < HD; d += 4) {
+        const float4 k = *reinterpret_cast<const float4*>(&sm.k[lane][d]);
+#pragma unroll
+        for (int i = 0; i < RPW; ++i) {
+          const float4 q = *reinterpret_cast<const float4*>(&sm.q[warp * RPW + i][d]);
+          sc[i] = fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, fmaf(q.w, k.w, sc[i]))));
         }
-        float* k = Ks + j * (HD + 1) + d;
-        k[0] = k01.x * ks, k[1] = k01.y * ks, k[2] = k23.x * ks, k[3] = k23.y * ks;
-        float* v = Vs + j * HD + d;
-        v[0] = v01.x * vs, v[1] = v01.y * vs, v[2] = v23.x * vs, v[3] = v23.y * vs;
       }
-      const long long kpos = k0 + lane;
-      if (kpos < k_end) {
-        const int page = L.page_table[(int64_t)p.b * L.max_pages + kpos / L.page_size];
-        mapped = page >= 0 && page < L.num_pages;
-      }
-      __syncthreads();
 #pragma unroll
       for (int i = 0; i < RPW; ++i) {
-        const int r = warp + 4 * i;
-        if (r >= nrows) break;
-        const float* q = Qs + r * HD;
-        const float* kr = Ks + lane * (HD + 1);
-        float sc = 0.f;
-#pragma unroll 8
-        for (int d = 0; d < HD; ++d) sc = fmaf(q[d], kr[d], sc);
-        const bool vis = mapped && kpos <= base + (row0 + r) / nrep;
-        sc = vis ? sc * sl2 : -INFINITY;
-        const float mnew = fmaxf(mrow[i], warp_max(sc));
+        const bool vis = here && key <= last[i];
+        const float s = vis ? sc[i] * sl2 : -INFINITY;
+        const float mnew = fmaxf(mrow[i], warp_max(s));
         const float mref = mnew == -INFINITY ? 0.f : mnew;   // nothing to see yet (a NaN score stays NaN below)
         const float alpha = exp2f(mrow[i] - mref);
-        const float pr = vis ? exp2f(sc - mref) : 0.f;
+        const float pr = vis ? exp2f(s - mref) : 0.f;
         lrow[i] = lrow[i] * alpha + warp_sum(pr);
         mrow[i] = mnew;
+        sm.p[warp][i][lane] = pr;
 #pragma unroll
-        for (int j = 0; j < DPL; ++j) acc[i][j] *= alpha;
-        for (int jj = 0; jj < SIMT_KT; ++jj) {
-          const float pj = __shfl_sync(0xffffffffu, pr, jj);
-          if (pj != 0.f) {
+        for (int d = 0; d < DPL; ++d) acc[i][d] *= alpha;
+      }
+      __syncwarp();
+#pragma unroll 2
+      for (int k0 = 0; k0 < SIMT_TILE; k0 += 4) {
+        float4 pr[RPW];
 #pragma unroll
-            for (int j = 0; j < DPL; ++j) acc[i][j] = fmaf(pj, Vs[jj * HD + lane + 32 * j], acc[i][j]);
+        for (int i = 0; i < RPW; ++i) pr[i] = *reinterpret_cast<const float4*>(&sm.p[warp][i][k0]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          Row<float, DPL> v;
+          v.load(sm.v[k0 + k], lane, true);
+#pragma unroll
+          for (int i = 0; i < RPW; ++i) {
+            const float pk = k == 0 ? pr[i].x : k == 1 ? pr[i].y : k == 2 ? pr[i].z : pr[i].w;
+#pragma unroll
+            for (int d = 0; d < DPL; ++d) acc[i][d] = fmaf(pk, v[d], acc[i][d]);
           }
         }
       }
+      __syncwarp();
     }
 #pragma unroll
     for (int i = 0; i < RPW; ++i) {
-      const int r = warp + 4 * i;
+      const int r = warp * RPW + i;
       if (r >= nrows) break;
       if (p.whole()) {
         const int t = (row0 + r) / nrep, hq = p.g * nrep + (row0 + r) % nrep;
         const int64_t m = (int64_t)p.b * L.tokens + t;
-        const T* gate = static_cast<const T*>(L.qkv) + m * L.ld_qkv + (int64_t)hq * 2 * HD + HD;
-        T* o = static_cast<T*>(L.out) + m * L.ld_out + (int64_t)hq * HD;
+        const T* gate = static_cast<const T*>(L.qkv) + m * L.ld_qkv + (int64_t)hq * 2 * HD + HD + lane * DPL;
+        T* o = static_cast<T*>(L.out) + m * L.ld_out + (int64_t)hq * HD + lane * DPL;
 #pragma unroll
-        for (int j = 0; j < DPL; ++j) {
-          const int d = lane + 32 * j;
-          const float v = lrow[i] == 0.f ? 0.f : acc[i][j] / lrow[i];
+        for (int d = 0; d < DPL; ++d) {
+          const float v = lrow[i] == 0.f ? 0.f : acc[i][d] / lrow[i];
           o[d] = dt<T>::from_f(v * sigmoidf_(dt<T>::to_f(gate[d])));
         }
       } else {
         const int64_t at = (int64_t)p.slot() * SIMT_R + r;
 #pragma unroll
-        for (int j = 0; j < DPL; ++j) ws.o[at * HD + lane + 32 * j] = acc[i][j];
+        for (int d = 0; d < DPL; ++d) ws.o[at * HD + lane * DPL + d] = acc[i][d];
         if (lane == 0) ws.ml[at] = make_float2(mrow[i], lrow[i]);
       }
     }
@@ -383,12 +417,12 @@ __global__ void __launch_bounds__(SIMT_THREADS) simt_kernel(const qsp_attn_kv8_l
 template <typename T, int HD>
 static int launch_simt(const qsp_attn_kv8_layer& L, int G, cudaStream_t st) {
   const int rows = L.n_heads / L.n_kv_heads * L.tokens, n_rg = (rows + SIMT_R - 1) / SIMT_R;
-  const size_t smem = (size_t)(SIMT_R * HD + SIMT_KT * (HD + 1) + SIMT_KT * HD) * sizeof(float);
+  const size_t smem = sizeof(SimtSmem<T, HD>);
   auto kern = simt_kernel<T, HD>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return set_error(QSP_ERR_CUDA, "qsp_attn_kv8_verify: %s", cudaGetErrorString(e));
-  const int rc = launch_pdl("qsp_attn_kv8_verify(simt)", kern, dim3(G), dim3(SIMT_THREADS), smem, st, L, n_rg);
-  return rc ? rc : launch_merge(L, G, SIMT_R, st);
+  const int rc = launch_pdl("qsp_attn_kv8_verify(simt)", kern, dim3(G), dim3(32 * SIMT_WARPS), smem, st, L, n_rg);
+  return rc ? rc : launch_merge(L, G, SIMT_R, SIMT_TILE, st);
 }
 
 // ------------------------------------------------------------------ merge of divided units
@@ -514,8 +548,8 @@ static int launch_merge_t(const qsp_attn_kv8_layer& L, int G, int R, cudaStream_
   }
 }
 
-int launch_merge(const qsp_attn_kv8_layer& L, int G, int R, cudaStream_t st) {
-  if ((int64_t)L.max_pages * L.page_size <= TILE) return QSP_OK;   // one tile a unit: none is divided
+int launch_merge(const qsp_attn_kv8_layer& L, int G, int R, int keys, cudaStream_t st) {
+  if ((int64_t)L.max_pages * L.page_size <= keys) return QSP_OK;   // one tile a unit: none is divided
   QSP_DISPATCH_DTYPE(L.dtype, T, { return launch_merge_t<T>(L, G, R, st); });
 }
 
@@ -539,7 +573,7 @@ static int validate(const char* what, const qsp_attn_kv8_layer* p, bool verify) 
                   L.page_size % L.scale_block == 0,
               "%s: scale_block %d must be a power of two up to 64 that divides the page size %d", what, L.scale_block, L.page_size);
   const int64_t q_rows = (int64_t)L.n_heads / L.n_kv_heads * L.tokens;
-  QSP_REQUIRE((double)L.batch * L.n_kv_heads * (q_rows / 8 + 1) * ((int64_t)L.max_pages * L.page_size / kv8::TILE + 4) < 2e9,
+  QSP_REQUIRE((double)L.batch * L.n_kv_heads * (q_rows / 8 + 1) * ((int64_t)L.max_pages * L.page_size / kv8::SIMT_TILE + 4) < 2e9,
               "%s: more than 2^31 tiles of keys", what);
   QSP_REQUIRE(aligned(L.k_pages, 16) && aligned(L.v_pages, 16) && aligned(L.q_buf, 16), "%s: pages and q_buf must be 16-byte aligned",
               what);

@@ -9,7 +9,8 @@
 namespace qsp {
 namespace kv8 {
 
-constexpr int TILE = 128;      // keys of a work tile
+constexpr int TILE = 128;      // keys of a tensor-core work tile
+constexpr int SIMT_TILE = 32;  // ... of one of the CUDA-core kernel
 constexpr int MIN_EXP = -40;   // least exponent of a scale
 constexpr int MAX_EXP = 120;   // 448·2^120 holds every fp32 value
 constexpr float LOG2E = 1.4426950408889634f;
@@ -99,7 +100,7 @@ __device__ __forceinline__ int exp_of(float scale) { return ((__float_as_int(sca
 
 // ---------------------------------------------------------------- work division
 // A unit is (sequence b, row group rg, kv head g): `R` query rows (t, q head of the group) against
-// the keys the last of them sees, cut into tiles of 128 keys. The tiles of all units, in the
+// the keys the last of them sees, cut into tiles of TILE keys. The tiles of all units, in the
 // order b, rg, g, are divided evenly over the CTAs, so a ragged batch, one long sequence and many
 // short ones all keep every SM equally busy. Beginning a unit counts as UNIT_COST tiles (queries in,
 // output out). A CTA's share is a run of pieces (parts of units). A piece that is a whole unit is
@@ -118,11 +119,12 @@ struct Piece {
   __device__ __forceinline__ int slot() const { return 2 * (int)blockIdx.x + (first ? 0 : 1); }
 };
 
+template <int KEYS>
 __device__ __forceinline__ int unit_tiles(const qsp_attn_kv8_layer& L, int len, int rg, int n_rg, int R) {
   const int t_last = rg == n_rg - 1 ? L.tokens - 1 : ((rg + 1) * R - 1) / (L.n_heads / L.n_kv_heads);
   const int cap = L.max_pages * L.page_size;
   const int kv = min(min(len, cap) + t_last + 1, cap);
-  return kv <= TILE ? 1 : (kv + TILE - 1) / TILE;   // a unit without keys has a tile too: it writes zeros
+  return kv <= KEYS ? 1 : (kv + KEYS - 1) / KEYS;   // a unit without keys has a tile too: it writes zeros
 }
 
 // Positions count UNIT_COST + tiles for each unit; the host has checked that all fit 31 bits.
@@ -145,12 +147,13 @@ __device__ __forceinline__ int share_owner(int pos, int total, int parts) {
 
 // This CTA's share, found by all threads of the CTA; `sh` holds 36 ints of shared memory. Ends with
 // a __syncthreads.
+template <int KEYS>
 __device__ __forceinline__ Walk share(const qsp_attn_kv8_layer& L, int n_rg, int R, int* sh) {
   const int n = L.batch * n_rg, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
   const int per = (n + blockDim.x - 1) / blockDim.x;   // (b, rg) pairs of a thread: consecutive ones
   auto cost = [&](int i) {
     const int b = n_rg == 1 ? i : i / n_rg;
-    return UNIT_COST + unit_tiles(L, L.seq_lens[b], i - b * n_rg, n_rg, R);
+    return UNIT_COST + unit_tiles<KEYS>(L, L.seq_lens[b], i - b * n_rg, n_rg, R);
   };
   int mine = 0;
   for (int k = 0; k < per; ++k)
@@ -199,13 +202,14 @@ __device__ __forceinline__ Walk share(const qsp_attn_kv8_layer& L, int n_rg, int
   return w;
 }
 
+template <int KEYS>
 __device__ __forceinline__ bool next_piece(const qsp_attn_kv8_layer& L, int n_rg, int R, Walk& w, Piece& p) {
   while (w.pos < w.end) {
     p.b = w.b;
     p.rg = w.rg;
     p.g = w.g;
     p.len = w.len;
-    p.unit_tiles = unit_tiles(L, w.len, w.rg, n_rg, R);
+    p.unit_tiles = unit_tiles<KEYS>(L, w.len, w.rg, n_rg, R);
     const int step = min(UNIT_COST + p.unit_tiles - w.at, w.end - w.pos);
     p.j0 = max(w.at - UNIT_COST, 0);
     p.n = max(w.at + step - UNIT_COST, 0) - p.j0;
@@ -255,7 +259,8 @@ __device__ __forceinline__ void put_meta(const Scratch& s, const Walk& w, const 
   s.meta[blockIdx.x] = m;
 }
 
-int launch_merge(const qsp_attn_kv8_layer& L, int G, int R, cudaStream_t st);
+// keys: of a work tile
+int launch_merge(const qsp_attn_kv8_layer& L, int G, int R, int keys, cudaStream_t st);
 // the tensor-core kernel; QSP_ERR_UNSUPPORTED when the shape is not one it takes
 int launch_tc(const qsp_attn_kv8_layer& L, cudaStream_t st);
 int tc_rows(int rows);            // its query rows per unit, for this many rows of a kv head

@@ -279,7 +279,7 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
   }
   pdl_wait();
   // the weights' buffers are not in use yet: room for share()'s 36 ints
-  Walk w = share(L, n_rg, R, reinterpret_cast<int*>(sP));
+  Walk w = share<TILE>(L, n_rg, R, reinterpret_cast<int*>(sP));
   tc::fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
   const int cap = L.max_pages * L.page_size;
@@ -355,7 +355,7 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
     Piece p;
     p.n = 0;
     for (uint32_t piece = 0;; ++piece) {
-      const bool more = next_piece(L, n_rg, R, w, p);
+      const bool more = next_piece<TILE>(L, n_rg, R, w, p);
       const int base = more ? min(p.len, cap) : 0;
       if (lane == 0) {
         desc[piece % NDESC] = {p.b, p.rg * R, p.g, p.j0, more ? p.n : 0, base, p.slot(), p.whole()};
@@ -787,7 +787,7 @@ static int launch_tc_t(const qsp_attn_kv8_layer& L, cudaStream_t st) {
   if (e != cudaSuccess) return set_error(QSP_ERR_CUDA, "qsp_attn_kv8_verify: %s", cudaGetErrorString(e));
   const int G = tc_grid(HD, R), n_rg = (L.n_heads / L.n_kv_heads * L.tokens + R - 1) / R;
   const int rc = launch_pdl("qsp_attn_kv8_verify", kern, dim3(G), dim3(C::THREADS), C::BYTES, st, mk, mv, L, n_rg, box_rows);
-  return rc ? rc : launch_merge(L, G, R, st);
+  return rc ? rc : launch_merge(L, G, R, TILE, st);
 }
 
 template <int HD>
