@@ -261,7 +261,7 @@ struct SimtSmem {
   float k[SIMT_TILE][HD + 4];   // lanes read 16 bytes a row: the rows' banks step by 4
   float v[SIMT_TILE][HD];
   float p[SIMT_WARPS][SIMT_RPW][SIMT_TILE];
-  int sh[36];
+  int sh[68];
 };
 
 template <typename T, int HD>
@@ -421,86 +421,95 @@ static int launch_simt(const qsp_attn_kv8_layer& L, int G, cudaStream_t st) {
   auto kern = simt_kernel<T, HD>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return set_error(QSP_ERR_CUDA, "qsp_attn_kv8_verify: %s", cudaGetErrorString(e));
+  G = grid_for(L, n_rg, SIMT_TILE, G);
   const int rc = launch_pdl("qsp_attn_kv8_verify(simt)", kern, dim3(G), dim3(32 * SIMT_WARPS), smem, st, L, n_rg);
   return rc ? rc : launch_merge(L, G, SIMT_R, SIMT_TILE, st);
 }
 
 // ------------------------------------------------------------------ merge of divided units
-// CTA (u, y): the u-th divided unit, 8 rows of it with a warp each, or (WIDE, for few units of many parts) one
-// row with its partials dealt out to 8 warps. A warp weights its partials with 2^(m_p − M) and adds them in
-// their order, a lane HD/32 columns, four in flight at a time; WIDE adds the warps' sums in order. Then
-// / l and the gate. Bound by latency: four dependent reads and the launch.
+// CTA (c, y): 8 rows, a warp each, of the divided unit whose first tile attention CTA c had, if there is one;
+// or (WIDE, for few units of many parts) CTA (u, r): row r of the u-th divided unit, its partials dealt out to 8
+// warps. A warp weights its partials with 2^(m_p − M) and adds them in their order, a lane HD/32 columns, four
+// in flight at a time; WIDE adds the warps' sums in order. Then / l and the gate. Bound by latency: the
+// launch and two dependent reads (meta; everything else).
 constexpr int MERGE_WARPS = 8;
 
 template <typename T, int HD, bool WIDE>
-__global__ void __launch_bounds__(32 * MERGE_WARPS, 4) merge_kernel(const qsp_attn_kv8_layer L, int G, int R) {
+__global__ void __launch_bounds__(32 * MERGE_WARPS, 3) merge_kernel(const qsp_attn_kv8_layer L, int G, int R) {
   pdl_trigger();
   pdl_wait();
   constexpr int EPL = HD / 32, DEPTH = 4;
   __shared__ float part[WIDE ? MERGE_WARPS : 1][HD + 1];
-  __shared__ int found, counts[32];
+  __shared__ float part_m[MERGE_WARPS];
   const Scratch ws = scratch(L, G, R);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  // the attention CTA that has the first tile of the u-th divided unit: thread i looks at CTAs i, i + 256, ..
-  constexpr int MAX_SCAN = 4;
-  bool has[MAX_SCAN];
-  uint32_t mask[MAX_SCAN];
+  int c = blockIdx.x;
+  if constexpr (WIDE) {
+    // the attention CTA that has the first tile of the u-th divided unit: thread i looks at CTAs i, i + 256, ..
+    constexpr int MAX_SCAN = 4;
+    __shared__ int found, counts[32];
+    bool has[MAX_SCAN];
+    uint32_t mask[MAX_SCAN];
 #pragma unroll
-  for (int k = 0; k < MAX_SCAN; ++k) {
-    const int i = k * 32 * MERGE_WARPS + threadIdx.x;
-    has[k] = i < G && ws.meta[i].w != 0;
-  }
-  if (threadIdx.x == 0) found = -1;
+    for (int k = 0; k < MAX_SCAN; ++k) {
+      const int i = k * 32 * MERGE_WARPS + threadIdx.x;
+      has[k] = i < G && ws.meta[i].w != 0;
+    }
+    if (threadIdx.x == 0) found = -1;
 #pragma unroll
-  for (int k = 0; k < MAX_SCAN; ++k) {
-    mask[k] = __ballot_sync(0xffffffffu, has[k]);
-    if (lane == 0) counts[k * MERGE_WARPS + warp] = __popc(mask[k]);
-  }
-  __syncthreads();
+    for (int k = 0; k < MAX_SCAN; ++k) {
+      mask[k] = __ballot_sync(0xffffffffu, has[k]);
+      if (lane == 0) counts[k * MERGE_WARPS + warp] = __popc(mask[k]);
+    }
+    __syncthreads();
 #pragma unroll
-  for (int k = 0; k < MAX_SCAN; ++k) {
-    const int w = k * MERGE_WARPS + warp;
-    const int before = __reduce_add_sync(0xffffffffu, lane < w ? counts[lane] : 0);
-    if (has[k] && before + __popc(mask[k] & ((1u << lane) - 1)) == (int)blockIdx.x)
-      found = k * 32 * MERGE_WARPS + threadIdx.x;
+    for (int k = 0; k < MAX_SCAN; ++k) {
+      const int w = k * MERGE_WARPS + warp;
+      const int before = __reduce_add_sync(0xffffffffu, lane < w ? counts[lane] : 0);
+      if (has[k] && before + __popc(mask[k] & ((1u << lane) - 1)) == (int)blockIdx.x) found = k * 32 * MERGE_WARPS + threadIdx.x;
+    }
+    __syncthreads();
+    c = found;
+    if (c < 0) return;
   }
-  __syncthreads();
-  const int c = found;
-  if (c < 0) return;
   const int4 meta = ws.meta[c];
   const int np = meta.w, r = WIDE ? blockIdx.y : blockIdx.y * MERGE_WARPS + warp;
   const int nrep = L.n_heads / L.n_kv_heads, rr = meta.y * R + r;
-  const bool live = r < R && rr < nrep * L.tokens;   // the same for the whole CTA if WIDE
-  if (!live) return;
+  if (np == 0 || r >= R || rr >= nrep * L.tokens) return;   // the same for the whole CTA if WIDE
   const int first = 2 * c + (meta.z >> 30);
   auto slot = [&](int q) { return (int64_t)(q == 0 ? first : 2 * (c + q)) * R + r; };
   const int t = rr / nrep, hq = (meta.z & ((1 << 30) - 1)) * nrep + rr - t * nrep;
   const int64_t m = (int64_t)meta.x * L.tokens + t;
-  const T* gate_p = static_cast<const T*>(L.qkv) + m * L.ld_qkv + (int64_t)hq * 2 * HD + HD + lane * EPL;
-  float gate[EPL], acc[EPL], den = 0.f, M = -INFINITY;
+  Row<T, EPL> gate;
+  gate.load(static_cast<const T*>(L.qkv) + m * L.ld_qkv + (int64_t)hq * 2 * HD + HD, lane, false);
+  float acc[EPL], den = 0.f, M = -INFINITY;   // sums relative to 2^M, the largest so far
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    gate[i] = dt<T>::to_f(gate_p[i]);
-    acc[i] = 0.f;
-  }
-  for (int q = lane; q < np; q += 32) M = fmaxf(M, ws.ml[slot(q)].x);
-  M = warp_max(M);
-  const float ref = M == -INFINITY ? 0.f : M;
+  for (int i = 0; i < EPL; ++i) acc[i] = 0.f;
   const int per = WIDE ? (np + MERGE_WARPS - 1) / MERGE_WARPS : np;
   const int q_begin = WIDE ? warp * per : 0, q_end = min(np, q_begin + per);
   for (int q0 = q_begin; q0 < q_end; q0 += DEPTH) {
     Row<float, EPL> v[DEPTH];
     float2 ml[DEPTH];
+    float top = M;
 #pragma unroll
     for (int u = 0; u < DEPTH; ++u) {
+      ml[u] = make_float2(-INFINITY, 0.f);
+      v[u].zero();
       if (q0 + u < q_end) {
         ml[u] = ws.ml[slot(q0 + u)];
         v[u].load(ws.o + slot(q0 + u) * HD, lane, true);
       }
     }
 #pragma unroll
+    for (int u = 0; u < DEPTH; ++u) top = fmaxf(top, ml[u].x);
+    const float ref = top == -INFINITY ? 0.f : top, old = exp2f(M - ref);
+    M = top;
+    den *= old;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) acc[i] *= old;
+#pragma unroll
     for (int u = 0; u < DEPTH; ++u) {
-      if (q0 + u < q_end && ml[u].y != 0.f) {   // else a part of which the row saw nothing
+      if (ml[u].y != 0.f) {   // else a part of which the row saw nothing
         const float f = exp2f(ml[u].x - ref);
         den = fmaf(f, ml[u].y, den);
 #pragma unroll
@@ -508,34 +517,46 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS, 4) merge_kernel(const qsp_at
       }
     }
   }
-  T* out = static_cast<T*>(L.out) + m * L.ld_out + (int64_t)hq * HD + lane * EPL;
   if constexpr (WIDE) {
 #pragma unroll
     for (int i = 0; i < EPL; ++i) part[warp][lane * EPL + i] = acc[i];
-    if (lane == 0) part[warp][HD] = den;
+    if (lane == 0) {
+      part[warp][HD] = den;
+      part_m[warp] = M;
+    }
     __syncthreads();
     if (warp != 0) return;
-    for (int w = 1; w < MERGE_WARPS; ++w) {
-      den += part[w][HD];
+    float top = M;
 #pragma unroll
-      for (int i = 0; i < EPL; ++i) acc[i] += part[w][lane * EPL + i];
+    for (int w = 1; w < MERGE_WARPS; ++w) top = fmaxf(top, part_m[w]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    den = 0.f;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) acc[i] = 0.f;
+#pragma unroll
+    for (int w = 0; w < MERGE_WARPS; ++w) {
+      const float f = exp2f(part_m[w] - ref);
+      den = fmaf(f, part[w][HD], den);
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) acc[i] = fmaf(f, part[w][lane * EPL + i], acc[i]);
     }
   }
+  T* out = static_cast<T*>(L.out) + m * L.ld_out + (int64_t)hq * HD + lane * EPL;
+  const float inv = den == 0.f ? 0.f : 1.f / den;
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) out[i] = dt<T>::from_f((den == 0.f ? 0.f : acc[i] / den) * sigmoidf_(gate[i]));
+  for (int i = 0; i < EPL; ++i) out[i] = dt<T>::from_f(acc[i] * inv * sigmoidf_(gate[i]));
 }
 
 template <typename T, int HD>
 static int launch_merge_hd(const qsp_attn_kv8_layer& L, int G, int R, cudaStream_t st) {
   const int rows = L.n_heads / L.n_kv_heads * L.tokens;
   const int64_t units = (int64_t)L.batch * L.n_kv_heads * ((rows + R - 1) / R);
-  const int divided = (int)std::min<int64_t>(units, G);
   // few units of many parts each: a CTA a row (one sequence of 32k keys, hd 256: 74 parts)
   if (units * MERGE_WARPS <= G)
-    return launch_pdl("qsp_attn_kv8_verify(merge)", merge_kernel<T, HD, true>, dim3(divided, std::min(R, rows)), dim3(32 * MERGE_WARPS), 0,
-                      st, L, G, R);
+    return launch_pdl("qsp_attn_kv8_verify(merge)", merge_kernel<T, HD, true>, dim3((unsigned)units, std::min(R, rows)),
+                      dim3(32 * MERGE_WARPS), 0, st, L, G, R);
   return launch_pdl("qsp_attn_kv8_verify(merge)", merge_kernel<T, HD, false>,
-                    dim3(divided, (std::min(R, rows) + MERGE_WARPS - 1) / MERGE_WARPS), dim3(32 * MERGE_WARPS), 0, st, L, G, R);
+                    dim3(G, (std::min(R, rows) + MERGE_WARPS - 1) / MERGE_WARPS), dim3(32 * MERGE_WARPS), 0, st, L, G, R);
 }
 
 template <typename T>

@@ -107,7 +107,10 @@ __device__ __forceinline__ int exp_of(float scale) { return ((__float_as_int(sca
 // written out by its CTA; the others leave a partial (o, m, l) in the workspace: slot 2c for the
 // first piece of CTA c, 2c + 1 for its last. The CTA that has the first tile of a divided unit
 // describes it in meta[c] for the merge kernel.
-constexpr int UNIT_COST = 3;
+// Dividing has a price: a second piece for most CTAs and the merge. Where no CTA would have more than
+// MERGE_COST tiles less to do for it, each unit goes whole to one CTA: 64 sequences of 2048 to 2560 keys,
+// 2 kv heads: 128 CTAs with at most 20 tiles each instead of 148 with 15.6 on average.
+constexpr int UNIT_COST = 3, MERGE_COST = 6;
 
 struct Piece {
   int b, rg, g;
@@ -145,7 +148,7 @@ __device__ __forceinline__ int share_owner(int pos, int total, int parts) {
   return pos < r * (q + 1) ? pos / (q + 1) : r + (pos - r * (q + 1)) / q;
 }
 
-// This CTA's share, found by all threads of the CTA; `sh` holds 36 ints of shared memory. Ends with
+// This CTA's share, found by all threads of the CTA; `sh` holds 68 ints of shared memory. Ends with
 // a __syncthreads.
 template <int KEYS>
 __device__ __forceinline__ Walk share(const qsp_attn_kv8_layer& L, int n_rg, int R, int* sh) {
@@ -155,20 +158,49 @@ __device__ __forceinline__ Walk share(const qsp_attn_kv8_layer& L, int n_rg, int
     const int b = n_rg == 1 ? i : i / n_rg;
     return UNIT_COST + unit_tiles<KEYS>(L, L.seq_lens[b], i - b * n_rg, n_rg, R);
   };
-  int mine = 0;
-  for (int k = 0; k < per; ++k)
-    if (tid * per + k < n) mine += cost(tid * per + k);
+  int mine = 0, most = 0;
+  for (int k = 0; k < per; ++k) {
+    if (tid * per + k < n) {
+      const int one = cost(tid * per + k);
+      mine += one;
+      most = max(most, one);
+    }
+  }
   int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int v = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += v;
   }
-  if (lane == 31) sh[warp] = incl;
+  most = __reduce_max_sync(0xffffffffu, most);
+  if (lane == 31) {
+    sh[warp] = incl;
+    sh[36 + warp] = most;
+  }
   __syncthreads();
   const int of_warp = lane < nw ? sh[lane] : 0;
+  most = __reduce_max_sync(0xffffffffu, lane < nw ? sh[36 + lane] : 0);
   const int total = __reduce_add_sync(0xffffffffu, of_warp) * L.n_kv_heads;
   const int before = __reduce_add_sync(0xffffffffu, lane < warp ? of_warp : 0) + incl - mine;
+  Walk w;
+  w.total = total;
+  w.first = true;
+  const int units = n * L.n_kv_heads;
+  if (units <= (int)gridDim.x && most <= total / (int)gridDim.x + MERGE_COST) {
+    // unit c to CTA c
+    const bool any = (int)blockIdx.x < units;
+    const int i = any ? blockIdx.x / L.n_kv_heads : 0;
+    w.b = i / n_rg;
+    w.rg = i - w.b * n_rg;
+    w.g = blockIdx.x - i * L.n_kv_heads;
+    w.at = w.pos = 0;
+    w.len = L.seq_lens[w.b];
+    w.next_len = 0;
+    w.end = any ? UNIT_COST + unit_tiles<KEYS>(L, w.len, w.rg, n_rg, R) : 0;
+    w.parts = 0;
+    __syncthreads();
+    return w;
+  }
   const int parts = min((int)gridDim.x, total);   // no more CTAs than tiles: every one of them has some
   const int c = min((int)blockIdx.x, parts);
   const int begin = share_begin(c, total, parts), end = share_begin(min(c + 1, parts), total, parts);
@@ -187,16 +219,13 @@ __device__ __forceinline__ Walk share(const qsp_attn_kv8_layer& L, int n_rg, int
     }
   }
   __syncthreads();
-  Walk w;
   w.b = sh[32] / n_rg;
   w.rg = sh[32] - w.b * n_rg;
   w.g = sh[33];
   w.at = sh[34];
   w.pos = begin;
   w.end = end;
-  w.total = total;
   w.parts = parts;
-  w.first = true;
   w.len = sh[35];
   w.next_len = begin < end && w.b + 1 < L.batch ? L.seq_lens[w.b + 1] : 0;
   return w;
@@ -259,6 +288,12 @@ __device__ __forceinline__ void put_meta(const Scratch& s, const Walk& w, const 
   s.meta[blockIdx.x] = m;
 }
 
+// CTAs of a launch: `most`, or as many as there can be positions
+inline int grid_for(const qsp_attn_kv8_layer& L, int n_rg, int keys, int most) {
+  const int64_t unit = UNIT_COST + ((int64_t)L.max_pages * L.page_size + keys - 1) / keys;
+  const int64_t all = (int64_t)L.batch * L.n_kv_heads * n_rg * unit;
+  return (int)(all < most ? all : most);
+}
 // keys: of a work tile
 int launch_merge(const qsp_attn_kv8_layer& L, int G, int R, int keys, cudaStream_t st);
 // the tensor-core kernel; QSP_ERR_UNSUPPORTED when the shape is not one it takes

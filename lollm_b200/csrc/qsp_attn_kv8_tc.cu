@@ -79,7 +79,7 @@ struct Cfg {
   static constexpr int COLS_USED = 2 * N + CB * N;
   static constexpr int COLS = COLS_USED <= 64 ? 64 : COLS_USED <= 128 ? 128 : COLS_USED <= 256 ? 256 : 512;
   static_assert(NSK >= 2 && NSK <= 4, "ring too short, or too long for the descriptors' slots");
-  static_assert(2 * PB >= 36 * 4, "the weights' buffers first hold share()'s 36 ints");
+  static_assert(2 * PB >= 68 * 4, "the weights' buffers first hold share()'s 68 ints");
 };
 
 // ---------------------------------------------------------------- descriptors
@@ -278,7 +278,7 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
     tc::fence_before();
   }
   pdl_wait();
-  // the weights' buffers are not in use yet: room for share()'s 36 ints
+  // the weights' buffers are not in use yet: room for share()'s 68 ints
   Walk w = share<TILE>(L, n_rg, R, reinterpret_cast<int*>(sP));
   tc::fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
@@ -785,7 +785,7 @@ static int launch_tc_t(const qsp_attn_kv8_layer& L, cudaStream_t st) {
   auto kern = tc_kernel<HD, R>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::BYTES);
   if (e != cudaSuccess) return set_error(QSP_ERR_CUDA, "qsp_attn_kv8_verify: %s", cudaGetErrorString(e));
-  const int G = tc_grid(HD, R), n_rg = (L.n_heads / L.n_kv_heads * L.tokens + R - 1) / R;
+  const int n_rg = (L.n_heads / L.n_kv_heads * L.tokens + R - 1) / R, G = grid_for(L, n_rg, TILE, tc_grid(HD, R));
   const int rc = launch_pdl("qsp_attn_kv8_verify", kern, dim3(G), dim3(C::THREADS), C::BYTES, st, mk, mv, L, n_rg, box_rows);
   return rc ? rc : launch_merge(L, G, R, TILE, st);
 }
