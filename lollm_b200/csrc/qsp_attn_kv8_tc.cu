@@ -287,7 +287,9 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
   auto piece_at = [&](uint32_t i) -> Desc {   // the i-th piece of this CTA
     wait_bar(&dfull[i % NDESC], i / NDESC & 1u, abort);
     __syncwarp();
-    return desc[i % NDESC];
+    Desc d = desc[i % NDESC];
+    if (__any_sync(0xffffffffu, *abort)) d.n = 0;   // a wait ran out: what is there may not be a descriptor
+    return d;
   };
 
   if (warp == W_K || warp == W_V) {
@@ -518,7 +520,14 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
       if (lane == 0) tc::mbar_arrive(qfull);
     };
 
-    Desc p = piece_at(0);
+    // the warps of a group meet at its barriers, so they have to agree on the next piece (they do, but for a
+    // wait that ran out in one of them)
+    auto agreed_piece_at = [&](uint32_t i) -> Desc {
+      Desc d = piece_at(i);
+      if (bar_any(bar, d.n == 0)) d.n = 0;
+      return d;
+    };
+    Desc p = agreed_piece_at(0);
     if (p.n > 0) {
       load_q(p);
       stage_q(0);
@@ -741,9 +750,8 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
         }
       }
       tc::fence_before();   // the next piece's products overwrite O after its pfull
-      bar_sync(bar);        // aux and red are written again
       ++piece;
-      p = piece_at(piece);
+      p = agreed_piece_at(piece);   // a barrier: aux and red are written again
     }
   }
   __syncthreads();

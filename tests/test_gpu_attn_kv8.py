@@ -243,7 +243,7 @@ ATTEND = [
     (H2B, 1, [0], 64, 16), (H2B, 1, [32, 127, 128, 300], 64, 16), (H2B, 4, [0, 700, 125, 126], 64, 16), (H2B, 2, [1500], 64, 16),
     (H2B, 9, [40, 250], 128, 64), (H2B, 40, [100], 16, 8), (HTINY, 5, [90, 201, 7], 32, 8), (HTINY, 33, [0, 130], 16, 1),
     (HMICRO, 3, [0, 2, 31, 513], 32, 32), (HMHA, 1, [400, 10], 32, 32), (HMHA, 17, [200], 64, 64), (HODD, 6, [5, 300], 8, 4),
-    (HODD, 6, [5, 150], 24, 8), (HTINY, 3, [140], 5, 1), ((8, 1, 256, 64), 16, [100], 64, 16), ((40, 2, 128, 32), 3, [70, 200], 64, 16),
+    (HODD, 6, [5, 150], 24, 8), (HTINY, 3, [140], 5, 1), (HTINY, 200, [0], 16, 8), (H2B, 131, [0, 70], 64, 16), (HMHA, 70, [0, 33], 256, 64), ((8, 1, 256, 64), 16, [100], 64, 16), ((40, 2, 128, 32), 3, [70, 200], 64, 16),
 ]
 
 
