@@ -232,7 +232,6 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
           int box_rows) {
   using C = Cfg<HD, R_>;
   constexpr int R = C::R, N = C::N, RW = C::RW, NWG = C::NWG, NSK = C::NSK, NSV = C::NSV, CW = C::CW, CB = C::CB, EPL = HD / 32;
-  pdl_trigger();
   extern __shared__ __align__(1024) uint8_t sK[];                // the swizzles go by address: 1024-byte tiles
   uint8_t* sV = sK + NSK * C::SLOT;
   uint8_t* sQ = sV + NSV * C::SLOT;
@@ -273,13 +272,16 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
   if (tid < R) mcur[tid] = NOTHING;
   if (lane == 0 && (warp == W_K || warp == W_V))
     asm volatile("prefetch.tensormap [%0];" ::"l"(warp == W_K ? &tmK : &tmV) : "memory");
+  pdl_wait();
+  // TMEM is asked for when the previous kernel has given its own back, and the next kernel may start when this
+  // grid has all of its: a CTA that waits for a grid never holds columns that the grid's CTAs still need
   if (warp == W_MMA) {
     tc::tmem_alloc(tmem_slot, C::COLS);
     tc::fence_before();
   }
-  pdl_wait();
   // the weights' buffers are not in use yet: room for share()'s 68 ints
   Walk w = share<TILE>(L, n_rg, R, reinterpret_cast<int*>(sP));
+  pdl_trigger();
   tc::fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
   const int cap = L.max_pages * L.page_size;
