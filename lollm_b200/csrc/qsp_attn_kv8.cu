@@ -660,7 +660,7 @@ size_t qsp_attn_kv8_workspace_bytes(int32_t batch, int32_t tokens, int32_t n_hea
     return 0;
   const size_t simt = kv8::scratch_bytes(kv8::simt_grid(), kv8::SIMT_R, head_dim);
   if (dtype == QSP_F32) return simt;
-  const int R = kv8::tc_rows(n_heads / n_kv_heads * std::min(tokens, 64));
+  const int R = kv8::tc_rows(n_heads / n_kv_heads * std::min(tokens, 128));
   return std::max(simt, kv8::scratch_bytes(kv8::tc_grid(head_dim, R), R, head_dim));
 }
 

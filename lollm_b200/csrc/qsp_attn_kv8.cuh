@@ -2,6 +2,7 @@
 // division of the attention's work over the CTAs.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_fp16.h>
 
 #include "qsp_common.cuh"
@@ -108,9 +109,10 @@ __device__ __forceinline__ int exp_of(float scale) { return ((__float_as_int(sca
 // first piece of CTA c, 2c + 1 for its last. The CTA that has the first tile of a divided unit
 // describes it in meta[c] for the merge kernel.
 // Dividing has a price: a second piece for most CTAs and the merge. Where no CTA would have more than
-// MERGE_COST tiles less to do for it, each unit goes whole to one CTA: 64 sequences of 2048 to 2560 keys,
+// merge_cost tiles less to do for it, each unit goes whole to one CTA: 64 sequences of 2048 to 2560 keys,
 // 2 kv heads: 128 CTAs with at most 20 tiles each instead of 148 with 15.6 on average.
-constexpr int UNIT_COST = 3, MERGE_COST = 6;
+constexpr int UNIT_COST = 3;
+__device__ __forceinline__ int merge_cost(int R) { return R > 64 ? 10 : 6; }
 
 struct Piece {
   int b, rg, g;
@@ -159,6 +161,7 @@ __device__ __forceinline__ Walk share(const qsp_attn_kv8_layer& L, int n_rg, int
     return UNIT_COST + unit_tiles<KEYS>(L, L.seq_lens[b], i - b * n_rg, n_rg, R);
   };
   int mine = 0, most = 0;
+#pragma unroll 1
   for (int k = 0; k < per; ++k) {
     if (tid * per + k < n) {
       const int one = cost(tid * per + k);
@@ -186,7 +189,7 @@ __device__ __forceinline__ Walk share(const qsp_attn_kv8_layer& L, int n_rg, int
   w.total = total;
   w.first = true;
   const int units = n * L.n_kv_heads;
-  if (units <= (int)gridDim.x && most <= total / (int)gridDim.x + MERGE_COST) {
+  if (units <= (int)gridDim.x && most <= total / (int)gridDim.x + merge_cost(R)) {
     // unit c to CTA c
     const bool any = (int)blockIdx.x < units;
     const int i = any ? blockIdx.x / L.n_kv_heads : 0;
@@ -206,6 +209,7 @@ __device__ __forceinline__ Walk share(const qsp_attn_kv8_layer& L, int n_rg, int
   const int begin = share_begin(c, total, parts), end = share_begin(min(c + 1, parts), total, parts);
   int a = before * L.n_kv_heads;
   if (a <= begin && begin < a + mine * L.n_kv_heads) {   // one thread's
+#pragma unroll 1
     for (int k = 0; k < per; ++k) {
       const int one = cost(tid * per + k), all = one * L.n_kv_heads;
       if (begin < a + all) {
@@ -296,11 +300,14 @@ inline int grid_for(const qsp_attn_kv8_layer& L, int n_rg, int keys, int most) {
 }
 // keys: of a work tile
 int launch_merge(const qsp_attn_kv8_layer& L, int G, int R, int keys, cudaStream_t st);
-// the tensor-core kernel; QSP_ERR_UNSUPPORTED when the shape is not one it takes
+// the tensor-core kernels; QSP_ERR_UNSUPPORTED when the shape is not one they take
 int launch_tc(const qsp_attn_kv8_layer& L, cudaStream_t st);
-int tc_rows(int rows);            // its query rows per unit, for this many rows of a kv head
-int tc_grid(int hd, int R);       // its CTAs
+int tc_rows(int rows);            // their query rows per unit, for this many rows of a kv head
+int tc_grid(int hd, int R);       // their CTAs
+// ... for units of 128 rows; the tensor maps of K and V, boxes of box_rows keys
+int launch_rows(const qsp_attn_kv8_layer& L, const CUtensorMap& mk, const CUtensorMap& mv, int box_rows, cudaStream_t st);
 int device_error(int reset);
+int rows_error(int reset);
 
 }  // namespace kv8
 }  // namespace qsp

@@ -26,30 +26,12 @@
 //
 // Bound by HBM: a tile of 128 keys at hd 256 is 64 KB, 2800 cycles of an SM's share of 6.5 TB/s; its
 // products take 520 cycles of the tensor cores at R = 32.
-#include "qsp_attn_kv8.cuh"
-#include "qsp_tc.cuh"
-
-#include <limits.h>
+#include "qsp_attn_kv8_tc.cuh"
 
 #include <algorithm>
 
 namespace qsp {
 namespace kv8 {
-
-__device__ int g_kv8_error = 0;
-
-constexpr int CODE_WAIT = 302;       // a bounded wait ran out
-constexpr float SLACK = 4.f;         // log2 units the running maximum may lag behind
-constexpr float BIAS = 4.f;          // weights are held times 2^BIAS: at most 2^(SLACK + BIAS) = 256 <= 448
-constexpr float NOTHING = -1e30f;    // maximum of a row that has seen nothing
-
-// A piece of work as the scales' warp hands it to the others, which run up to 4 tiles behind it (and the
-// slowest of them 3 pieces more): 8 slots.
-constexpr int NDESC = 8;
-struct Desc {
-  int b, row0, g, j0;         // sequence, first row of the unit, kv head, first tile
-  int n, base, slot, whole;   // tiles (0: no more pieces), sequence length, partial's slot, whole unit
-};
 
 template <int HD, int R_>
 struct Cfg {
@@ -82,124 +64,6 @@ struct Cfg {
   static_assert(2 * PB >= 68 * 4, "the weights' buffers first hold share()'s 68 ints");
 };
 
-// ---------------------------------------------------------------- descriptors
-// rows of W bytes (16, 32, 64 or 128), swizzled over W bytes, 8-row groups 8·W apart: the layout of
-// TMA boxes with inner extent W. K-major: rows are M/N, bytes along the row K. MN-major: the row is
-// M/N, rows are K; lead = distance of the next W elements along M/N (0: the same again).
-struct Sdesc {   // the address is in the low word; all offsets within shared memory are added there
-  uint32_t lo, hi;
-};
-template <int W>
-__device__ __forceinline__ Sdesc sdesc(const void* p, uint32_t lead) {
-  constexpr uint32_t type = W == 128 ? 2 : W == 64 ? 4 : W == 32 ? 6 : 0;
-  return {((tc::smem_u32(p) & 0x3FFFFu) >> 4) | (lead >> 4) << 16, (8 * W >> 4) | 1u << 14 | type << 29};
-}
-template <int W>
-__device__ __forceinline__ int swz(int row, int chunk) {   // byte offset of a 16-byte chunk of a row
-  constexpr int M = W / 16 - 1;
-  return row * W + ((chunk ^ (row * W / 128 & M)) << 4);
-}
-// kind::f8f6f4, D fp32, A and B e4m3
-__host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N, bool mn_major) {
-  return (1u << 4) | (mn_major ? 3u << 15 : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
-}
-// `STEPS` MMAs of K = 32 into the same accumulator, the operands' addresses a_step and b_step (in
-// 16-byte units) apart; the first accumulates iff acc != 0. Issued by a converged warp.
-template <int STEPS, int A_STEP, int B_STEP>
-__device__ __forceinline__ void umma_e4m3_warp(uint32_t d, Sdesc a, Sdesc b, uint32_t idesc, uint32_t acc) {
-  static_assert(STEPS == 1 || STEPS == 2 || STEPS == 4, "");
-  if constexpr (STEPS == 4) {
-    asm volatile(
-        "{\n\t.reg .pred e, p;\n\t.reg .b64 a, b;\n\t.reg .b32 x, y;\n\t"
-        "elect.sync _|e, 0xffffffff;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "mov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %5, p;\n\t"
-        "setp.eq.b32 p, %6, %6;\n\t"
-        "add.u32 x, %1, %7;\n\tadd.u32 y, %3, %8;\n\tmov.b64 a, {x, %2};\n\tmov.b64 b, {y, %4};\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %5, p;\n\t"
-        "add.u32 x, x, %7;\n\tadd.u32 y, y, %8;\n\tmov.b64 a, {x, %2};\n\tmov.b64 b, {y, %4};\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %5, p;\n\t"
-        "add.u32 x, x, %7;\n\tadd.u32 y, y, %8;\n\tmov.b64 a, {x, %2};\n\tmov.b64 b, {y, %4};\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %5, p;\n\t}" ::"r"(d),
-        "r"(a.lo), "r"(a.hi), "r"(b.lo), "r"(b.hi), "r"(idesc), "r"(acc), "n"(A_STEP), "n"(B_STEP)
-        : "memory");
-  } else {
-    asm volatile(
-        "{\n\t.reg .pred e, p;\n\t.reg .b64 a, b;\n\t"
-        "elect.sync _|e, 0xffffffff;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "mov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %5, p;\n\t}" ::"r"(d),
-        "r"(a.lo), "r"(a.hi), "r"(b.lo), "r"(b.hi), "r"(idesc), "r"(acc)
-        : "memory");
-    if constexpr (STEPS == 2)
-      umma_e4m3_warp<1, A_STEP, B_STEP>(d, {a.lo + A_STEP, a.hi}, {b.lo + B_STEP, b.hi}, idesc, 1);
-  }
-}
-
-// ---------------------------------------------------------------- waits
-// Bounded; the poll is kept small (five roles share an instruction cache), the rest is out of line.
-__device__ __noinline__ bool give_up(uint32_t polls, volatile int* abort) {
-  if (*abort) return true;
-  if (polls < tc::WAIT_LIMIT) {
-    __nanosleep(64);
-    return false;
-  }
-  atomicExch(&g_kv8_error, CODE_WAIT);
-  *abort = 1;
-  return true;
-}
-__device__ __forceinline__ void wait_bar(uint64_t* bar, uint32_t parity, volatile int* abort) {
-  uint32_t n = 0;
-  while (!tc::mbar_try_wait(bar, parity))
-    if ((++n & 255u) == 0 && give_up(n, abort)) return;
-}
-
-// ---------------------------------------------------------------- TMEM, 8 columns of this warp's 32 lanes
-__device__ __forceinline__ void tm_ld8(uint32_t t, uint32_t (&r)[8]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-               : "r"(t));
-}
-__device__ __forceinline__ void tm_st8(uint32_t t, const uint32_t (&r)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(t), "r"(r[0]), "r"(r[1]), "r"(r[2]),
-               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-               : "memory");
-}
-// the registers are operands, so that nothing reads them before the wait
-__device__ __forceinline__ void tm_wait_ld8(uint32_t (&r)[8]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])::"memory");
-}
-__device__ __forceinline__ void tm_wait_ld8(uint32_t (&r)[8], uint32_t (&s)[8]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(s[0]), "+r"(s[1]),
-                 "+r"(s[2]), "+r"(s[3]), "+r"(s[4]), "+r"(s[5]), "+r"(s[6]), "+r"(s[7])::"memory");
-}
-__device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint16_t half2_to_e4m3x2(__half2 v) {
-  uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(*reinterpret_cast<uint32_t*>(&v)));
-  return r;
-}
-__device__ __forceinline__ void bar_sync(int id) { asm volatile("barrier.cta.sync %0, 128;" ::"r"(id) : "memory"); }
-__device__ __forceinline__ bool bar_any(int id, bool p) {
-  uint32_t r;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %2, 0;\n\tbarrier.cta.red.or.pred q, %1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(r)
-      : "r"(id), "r"((uint32_t)p)
-      : "memory");
-  return r != 0;
-}
-
 // v[RW] per lane -> in lane i the reduction over the warp's lanes of row row_of(i)
 template <int RW, bool MAX>
 __device__ __forceinline__ float warp_transpose_reduce(float (&v)[RW], int lane) {
@@ -223,8 +87,6 @@ template <int RW>
 __device__ __forceinline__ int row_of(int lane) {
   return lane / (32 / RW);
 }
-
-constexpr uint32_t MISSING = 0xffffu;   // scale exponents of a key that has no page
 
 template <int HD, int R_>
 __global__ void __launch_bounds__(Cfg<HD, R_>::THREADS, Cfg<HD, R_>::OCC)
@@ -284,8 +146,6 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
   pdl_trigger();
   tc::fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
-  const int cap = L.max_pages * L.page_size;
-  auto kv_end_of = [&](int base) { return min(base + L.tokens, cap); };   // keys that can have a page
   auto piece_at = [&](uint32_t i) -> Desc {   // the i-th piece of this CTA
     wait_bar(&dfull[i % NDESC], i / NDESC & 1u, abort);
     __syncwarp();
@@ -295,131 +155,20 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
   };
 
   if (warp == W_K || warp == W_V) {
-    // ---------------- loads of K and of V: boxes of box_rows keys x a column block; lane i looks up the page
-    // of the tile's i-th box_rows keys, one tile ahead
     const bool is_v = warp == W_V;
-    const CUtensorMap* map = is_v ? &tmV : &tmK;
-    uint8_t* ring = is_v ? sV : sK;
-    uint64_t* full = is_v ? vfull : kfull;
-    uint64_t* empty = is_v ? vempty : kempty;
-    const int slots = is_v ? NSV : NSK;
-    const int chunks = TILE / box_rows, pages_step = TILE / L.page_size, slot_step = TILE % L.page_size;
-    int slot = 0;
-    uint32_t turn = 1;   // parity of "empty" for this turn of the ring
-    for (uint32_t piece = 0;; ++piece) {
-      const Desc p = piece_at(piece);
-      if (p.n == 0) break;
-      const int kv_end = kv_end_of(p.base);
-      const int32_t* pages = L.page_table + (int64_t)p.b * L.max_pages;
-      int key = lane < chunks ? p.j0 * TILE + lane * box_rows : INT_MAX - 2 * TILE;   // this lane's first key of the tile
-      int lp = key / L.page_size, in = key - lp * L.page_size;
-      int page = key < kv_end ? pages[lp] : -1;
-      for (int j = 0; j < p.n; ++j) {
-        // row of the pages' [pages·n_kv·page_size, hd] view, or -1
-        const int row = page >= 0 && page < L.num_pages ? (page * L.n_kv_heads + p.g) * L.page_size + in : -1;
-        if (lane < chunks) key += TILE;
-        lp += pages_step;
-        in += slot_step;
-        if (in >= L.page_size) {
-          in -= L.page_size;
-          ++lp;
-        }
-        page = j + 1 < p.n && key < kv_end ? pages[lp] : -1;
-        wait_bar(&empty[slot], turn, abort);
-        __syncwarp();
-        const uint32_t there = __ballot_sync(0xffffffffu, row >= 0);
-        tc::mbar_expect_tx_warp(&full[slot], __popc(there) * box_rows * HD);
-        uint8_t* dst = ring + slot * C::SLOT;
-        for (int i = 0; i < chunks; ++i, dst += box_rows * CW) {
-          const int r = __shfl_sync(0xffffffffu, row, i);
-          if (r >= 0) {
-#pragma unroll
-            for (int cb = 0; cb < CB; ++cb) {
-              // read once: kept out of the way of queries, page tables and partials in L2
-              if (n_rg == 1) tc::tma_load_2d_evict_first_warp(dst + cb * (TILE * CW), map, &full[slot], cb * CW, r);
-              else tc::tma_load_2d_warp(dst + cb * (TILE * CW), map, &full[slot], cb * CW, r);
-            }
-          }
-        }
-        if (++slot == slots) {
-          slot = 0;
-          turn ^= 1u;
-        }
-      }
-    }
+    load_tiles<HD, CW>(L, is_v ? &tmV : &tmK, is_v ? sV : sK, is_v ? vfull : kfull, is_v ? vempty : kempty, is_v ? NSV : NSK, box_rows,
+                       n_rg == 1, piece_at, abort);
   } else if (warp == W_E) {
-    // ---------------- scale exponents of a tile's keys, 4 a lane, in step with the K ring: pages are loaded two
-    // tiles ahead, scales one. A slot is free when QK of the tile NSK before this one is done: that product was
-    // issued after the scores of the tile NSE before, and so its scales, had been read. This warp also walks
-    // through the CTA's share of the work and describes its pieces to the others.
-    const int nb = L.page_size / L.scale_block, sb_log = __ffs(L.scale_block) - 1;
-    const int pages_step = TILE / L.page_size, slot_step = TILE % L.page_size;
-    int slot = 0, eslot = 0;
-    uint32_t turn = 1;
-    Piece p;
-    p.n = 0;
-    for (uint32_t piece = 0;; ++piece) {
-      const bool more = next_piece<TILE>(L, n_rg, R, w, p);
-      const int base = more ? min(p.len, cap) : 0;
-      if (lane == 0) {
-        desc[piece % NDESC] = {p.b, p.rg * R, p.g, p.j0, more ? p.n : 0, base, p.slot(), p.whole()};
-        tc::mbar_arrive(&dfull[piece % NDESC]);
-      }
-      if (!more) break;
-      const int kv_end = kv_end_of(base);
-      const int32_t* pages = L.page_table + (int64_t)p.b * L.max_pages;
-      int page[4], blk[4], lp[4], in[4];   // of tile j + 1, then j + 2
-      float ks[4], vs[4];                  // of tile j
-      bool here[4];
+    // ---------------- scale exponents of a tile's keys, 4 a lane
+    uint16_t* e = sE + lane;
+    const Piece p = walk_and_scales(L, n_rg, R, NSK, w, desc, dfull, kfull, kempty, abort, [&](const Scales& x) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = p.j0 * TILE + i * 32 + lane;
-        lp[i] = key / L.page_size;
-        in[i] = key - lp[i] * L.page_size;
-      }
-      auto pages_at = [&](int j) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          blk[i] = in[i] >> sb_log;
-          page[i] = j < p.n && (p.j0 + j) * TILE + i * 32 + lane < kv_end ? pages[lp[i]] : -1;
-          lp[i] += pages_step;
-          in[i] += slot_step;
-          if (in[i] >= L.page_size) {
-            in[i] -= L.page_size;
-            ++lp[i];
-          }
-        }
-      };
-      auto scales_at = [&]() {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          here[i] = page[i] >= 0 && page[i] < L.num_pages;
-          const int64_t at = here[i] ? ((int64_t)page[i] * L.n_kv_heads + p.g) * nb + blk[i] : 0;
-          ks[i] = L.k_scales[at];
-          vs[i] = L.v_scales[at];
-        }
-      };
-      pages_at(0);
-      scales_at();
-      pages_at(1);
-      for (int j = 0; j < p.n; ++j) {
-        wait_bar(&kempty[slot], turn, abort);
-        uint16_t* e = sE + eslot * TILE;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          e[i * 32 + lane] = here[i] ? (uint16_t)((__float_as_uint(ks[i]) >> 23 & 0xffu) | (__float_as_uint(vs[i]) >> 23 & 0xffu) << 8)
-                                     : (uint16_t)MISSING;
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&kfull[slot]);
-        if (++eslot == C::NSE) eslot = 0;
-        if (++slot == NSK) {
-          slot = 0;
-          turn ^= 1u;
-        }
-        scales_at();
-        pages_at(j + 2);
-      }
-    }
+      for (int i = 0; i < 4; ++i)
+        e[i * 32] = x.here[i] ? (uint16_t)((__float_as_uint(x.ks[i]) >> 23 & 0xffu) | (__float_as_uint(x.vs[i]) >> 23 & 0xffu) << 8)
+                              : (uint16_t)MISSING;
+      e += TILE;
+      if (e == sE + lane + C::NSE * TILE) e = sE + lane;
+    });
     if (lane == 0) put_meta(scratch(L, gridDim.x, R), w, p);
   } else if (warp == W_MMA) {
     // ---------------- products, in the order QK(0) QK(1) PV(0) QK(2) PV(1) ... of each piece. QK(t) overwrites the
@@ -736,7 +485,7 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
           for (int i = 0; i < 8; ++i) {
             const float v = fmaf(__uint_as_float(ol[i]), 0.0625f, __uint_as_float(oh[i])) * aux[r0 + i0 + i];
             if (first + i < rows_total && dim < HD)
-              static_cast<__nv_bfloat16*>(L.out)[mrow * L.ld_out + (int64_t)(p.g * nrep + h) * HD + dim] = __float2bfloat16_rn(v * sigmoidf_(gate[i]));
+              static_cast<__nv_bfloat16*>(L.out)[mrow * L.ld_out + (int64_t)(p.g * nrep + h) * HD + dim] = __float2bfloat16_rn(v * sigmoid_ex2(gate[i]));
             if (++h == nrep) {
               h = 0;
               ++mrow;
@@ -758,6 +507,7 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
   }
   __syncthreads();
   if (*abort) {   // a wait ran out: give copies and products in flight time to land before the memory is given back
+#pragma unroll 1
     for (int i = 0; i < 4096; ++i) __nanosleep(1000);
     __syncthreads();
   }
@@ -778,20 +528,16 @@ static bool make_map(CUtensorMap* m, const void* base, int64_t rows, int hd, int
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// CTAs: one an SM, or two where registers and shared memory have room
 int tc_grid(int hd, int R) { return tc::sm_count() * (hd == 256 || R >= 32 ? 1 : 2); }
 
-// the least R that holds all query rows of a kv head, so that each key is read once; 64 at most
-int tc_rows(int rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+// the least R that holds all query rows of a kv head, so that each key is read once; over 64 rows: units of 128, of
+// rows_kernel
+int tc_rows(int rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
 
 template <int HD, int R>
-static int launch_tc_t(const qsp_attn_kv8_layer& L, cudaStream_t st) {
+static int launch_tc_t(const qsp_attn_kv8_layer& L, const CUtensorMap& mk, const CUtensorMap& mv, int box_rows, cudaStream_t st) {
   using C = Cfg<HD, R>;
-  const int64_t rows = (int64_t)L.num_pages * L.n_kv_heads * L.page_size;
-  int box_rows = 8;
-  while (box_rows < TILE && L.page_size % (2 * box_rows) == 0) box_rows *= 2;
-  CUtensorMap mk, mv;
-  if (!make_map(&mk, L.k_pages, rows, HD, box_rows) || !make_map(&mv, L.v_pages, rows, HD, box_rows))
-    return set_error(QSP_ERR_CUDA, "qsp_attn_kv8_verify: no tensor map for the pages");
   auto kern = tc_kernel<HD, R>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::BYTES);
   if (e != cudaSuccess) return set_error(QSP_ERR_CUDA, "qsp_attn_kv8_verify: %s", cudaGetErrorString(e));
@@ -801,23 +547,32 @@ static int launch_tc_t(const qsp_attn_kv8_layer& L, cudaStream_t st) {
 }
 
 template <int HD>
-static int launch_tc_hd(const qsp_attn_kv8_layer& L, cudaStream_t st) {
-  switch (tc_rows(L.n_heads / L.n_kv_heads * L.tokens)) {
-    case 8: return launch_tc_t<HD, 8>(L, st);
-    case 16: return launch_tc_t<HD, 16>(L, st);
-    case 32: return launch_tc_t<HD, 32>(L, st);
-    default: return launch_tc_t<HD, 64>(L, st);
+static int launch_tc_hd(const qsp_attn_kv8_layer& L, int R, const CUtensorMap& mk, const CUtensorMap& mv, int box_rows,
+                        cudaStream_t st) {
+  switch (R) {
+    case 8: return launch_tc_t<HD, 8>(L, mk, mv, box_rows, st);
+    case 16: return launch_tc_t<HD, 16>(L, mk, mv, box_rows, st);
+    case 32: return launch_tc_t<HD, 32>(L, mk, mv, box_rows, st);
+    default: return launch_tc_t<HD, 64>(L, mk, mv, box_rows, st);
   }
 }
 
 int launch_tc(const qsp_attn_kv8_layer& L, cudaStream_t st) {
   // rows of the pages are 32-bit coordinates of the tensor map
-  if (L.page_size % 8 != 0 || (int64_t)L.num_pages * L.n_kv_heads * L.page_size >= (1ll << 31)) return QSP_ERR_UNSUPPORTED;
+  const int64_t rows = (int64_t)L.num_pages * L.n_kv_heads * L.page_size;
+  if (L.page_size % 8 != 0 || rows >= (1ll << 31)) return QSP_ERR_UNSUPPORTED;
+  int box_rows = 8;
+  while (box_rows < TILE && L.page_size % (2 * box_rows) == 0) box_rows *= 2;
+  CUtensorMap mk, mv;
+  if (!make_map(&mk, L.k_pages, rows, L.head_dim, box_rows) || !make_map(&mv, L.v_pages, rows, L.head_dim, box_rows))
+    return set_error(QSP_ERR_CUDA, "qsp_attn_kv8_verify: no tensor map for the pages");
+  const int R = tc_rows(L.n_heads / L.n_kv_heads * L.tokens);
+  if (R == 128 && L.scale_block >= 8) return launch_rows(L, mk, mv, box_rows, st);
   switch (L.head_dim) {
-    case 32: return launch_tc_hd<32>(L, st);
-    case 64: return launch_tc_hd<64>(L, st);
-    case 128: return launch_tc_hd<128>(L, st);
-    default: return launch_tc_hd<256>(L, st);
+    case 32: return launch_tc_hd<32>(L, R, mk, mv, box_rows, st);
+    case 64: return launch_tc_hd<64>(L, R, mk, mv, box_rows, st);
+    case 128: return launch_tc_hd<128>(L, R, mk, mv, box_rows, st);
+    default: return launch_tc_hd<256>(L, R, mk, mv, box_rows, st);
   }
 }
 
@@ -828,7 +583,8 @@ int device_error(int reset) {
     const int z = 0;
     cudaMemcpyToSymbol(g_kv8_error, &z, sizeof(int));
   }
-  return v;
+  const int rows = rows_error(reset);
+  return v ? v : rows;
 }
 
 }  // namespace kv8
