@@ -73,9 +73,14 @@ struct Row {
   // bits of the largest magnitude (they compare as the values do; 0x7f800000 and over: not finite)
   __device__ __forceinline__ uint32_t top() const {
     uint32_t t = 0;
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) t = max(t, __float_as_uint((*this)[i]) & 0x7fffffffu);
-    return t;
+      for (int i = 0; i < W; ++i) t = max(t, r[i] & 0x7fffffffu);
+      return t;
+    }
+#pragma unroll
+    for (int i = 0; i < W; ++i) t = __vmaxu2(t, r[i] & 0x7fff7fffu);   // two halves at a time
+    return max(t & 0xffff0000u, t << 16);
   }
 };
 constexpr uint32_t NOT_FINITE = 0x7f800000u;

@@ -290,7 +290,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
     const Scratch ws = scratch(L, gridDim.x, RR);
     uint32_t tile = 0, piece = 0, eslot = 0, vslot = 0, vturn = 0;
 
-    // Q of a piece: a warp per row, four rows while the next four are loaded. (A loop: as straight code it took three
+    // Q of a piece: a warp per row, four rows while the next eight are loaded. (A loop: as straight code it took three
     // times as long, for the fetching of instructions.)
     auto stage_q = [&](const Desc& q, uint32_t n) {
       int64_t at = -1;   // of row lane·8 + warp in q_buf
@@ -298,22 +298,25 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
         const int rr = q.row0 + lane * 8 + warp, t = rr / nrep;
         at = (((int64_t)q.b * L.tokens + t) * L.n_heads + q.g * nrep + rr - t * nrep) * HD;
       }
-      Row<__nv_bfloat16, EPL> x[4], y[4];
+      Row<__nv_bfloat16, EPL> x[4], y[4], z[4];
       auto load = [&](int i0) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int64_t from = __shfl_sync(0xffffffffu, at, i0 + i);
-          y[i].zero();
-          if (from >= 0) y[i].load(static_cast<const __nv_bfloat16*>(L.q_buf) + from, lane, true);
+          z[i].zero();
+          if (from >= 0) z[i].load(static_cast<const __nv_bfloat16*>(L.q_buf) + from, lane, true);
         }
       };
       const int byte = lane * EPL, in = byte % CW;
       load(0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = z[i];
+      load(4);
 #pragma unroll 1
       for (int i0 = 0; i0 < 16; i0 += 4) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = y[i];
-        if (i0 < 12) load(i0 + 4);
+        for (int i = 0; i < 4; ++i) x[i] = y[i], y[i] = z[i];
+        if (i0 < 8) load(i0 + 8);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int r = (i0 + i) * 8 + warp;
