@@ -551,8 +551,9 @@ template <typename T, int HD>
 static int launch_merge_hd(const qsp_attn_kv8_layer& L, int G, int R, cudaStream_t st) {
   const int rows = L.n_heads / L.n_kv_heads * L.tokens;
   const int64_t units = (int64_t)L.batch * L.n_kv_heads * ((rows + R - 1) / R);
-  // few units of many parts each: a CTA a row (one sequence of 32k keys, hd 256: 74 parts)
-  if (units * MERGE_WARPS <= G)
+  // few units of many parts each, and few rows: a CTA a row (one sequence of 32k keys, hd 256: 74 parts). Many rows fill the
+  // GPU by themselves.
+  if (units * MERGE_WARPS <= G && units * std::min(R, rows) <= 2 * tc::sm_count())
     return launch_pdl("qsp_attn_kv8_verify(merge)", merge_kernel<T, HD, true>, dim3((unsigned)units, std::min(R, rows)),
                       dim3(32 * MERGE_WARPS), 0, st, L, G, R);
   return launch_pdl("qsp_attn_kv8_verify(merge)", merge_kernel<T, HD, false>,
