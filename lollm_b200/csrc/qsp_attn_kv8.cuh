@@ -117,7 +117,7 @@ __device__ __forceinline__ int exp_of(float scale) { return ((__float_as_int(sca
 // merge_cost tiles less to do for it, each unit goes whole to one CTA: 64 sequences of 2048 to 2560 keys,
 // 2 kv heads: 128 CTAs with at most 20 tiles each instead of 148 with 15.6 on average.
 constexpr int UNIT_COST = 3;
-__device__ __forceinline__ int merge_cost(int R) { return R > 64 ? 10 : 6; }
+__device__ __forceinline__ int merge_cost(int R) { return R > 64 ? 12 : 6; }
 
 struct Piece {
   int b, rg, g;
