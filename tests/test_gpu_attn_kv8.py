@@ -442,3 +442,137 @@ def test_builder_refuses():
         c.layer(out=c.out[:, :-1])
     with pytest.raises(RuntimeError):
         K().attn_kv8_verify(c.layer(workspace=torch.empty(16, dtype=torch.uint8, device=DEV)))
+
+
+# more than 64 rows of query per kv head: chunks of prompts
+CHUNKS = [
+    (HMICRO, 40, [0, 100, 7], 32, 32), (HMICRO, 70, [300], 64, 8), (HODD, 30, [5, 300, 0], 24, 8), (HODD, 45, [130], 8, 8),
+    (HTINY, 17, [64, 60, 2], 16, 8), (HTINY, 32, [1000], 64, 64), (HMHA, 65, [129, 0], 32, 16), (H2B, 16, [2600], 64, 16),
+    (H2B, 17, [3, 900, 127], 128, 32), ((12, 2, 256, 0), 11, [0, 255], 64, 64), ((64, 1, 64, 32), 3, [250, 4], 16, 16),
+    (H2B, 20, [40, 250], 16, 4), (HTINY, 40, [70], 16, 2),
+]
+
+
+@pytest.mark.parametrize("heads,T,lens,ps,sb", CHUNKS)
+def test_attend_chunk(heads, T, lens, ps, sb):
+    c = Case(BF16, heads, T, lens, ps, sb)
+    c.check_out(*c.attend(c.set_q()))
+
+
+@pytest.mark.parametrize("q_scale", [1e-3, 12.0])
+def test_attend_chunk_flat_and_peaked(q_scale):
+    """Scores that hardly differ, and ones whose maximum keeps rising along the keys (O is rescaled often)."""
+    c = Case(BF16, H2B, 18, [700, 30], 64, 16, q_scale=q_scale)
+    c.check_out(*c.attend(c.set_q()))
+    for n in ("k", "v"):
+        s = c.c[n + "_scales"]
+        s.mul_(2.0 ** torch.randint(-12, 4, s.shape, generator=c.g).float())
+        for p in range(0, 700, 16):
+            s[c.table[0, p // 64], :, p % 64 // 16] = 2.0 ** (-13 + p / 90 // 1)
+        c.d[n + "_scales"].copy_(s)
+    c.check_out(*c.attend(c.set_q()))
+
+
+def test_attend_chunk_sink():
+    """One strong key and many weak ones that weigh the same: no rounding of weights may add up."""
+    T = 12
+    c = Case(BF16, H2B, T, [900], 64, 16)
+    _uniform_codes(c, 0.0)
+    q = torch.zeros(T, c.nh * c.hd, dtype=BF16)
+    q.view(T, c.nh, c.hd)[..., 0] = 16.0
+    c.q_buf.copy_(q)
+    page, j = c.table[0, 3], 0
+    sc = float(c.c["k_scales"][page, 0, j])
+    c.c["k_pages"].view(torch.uint8)[page, :, 5, 0] = torch.tensor(min(9.0 / sc, 448.0)).to(kv8.F8).view(torch.uint8)
+    c.d["k_pages"].view(torch.uint8).copy_(c.c["k_pages"].view(torch.uint8))
+    c.check_out(*c.attend(q))
+
+
+def test_attend_chunk_ignores_what_it_may_not_see():
+    """NaN codes past the sequences, in pages of nobody and in a page that the table does not name; a
+    negative length leaves the first queries without a key; a row of NaN and one of infinities."""
+    T = 20
+    c = Case(BF16, H2B, T, [3, 230, -7, 107], 64, 16, cap=320)
+    c.table[1, 1] = -1
+    c.table[3, 0] = 10 ** 6
+    c.c["table"] = c.table.tolist()
+    c.d["page_table"].copy_(c.table)
+    P = c.c["k_pages"].shape[0]
+    used = torch.zeros(P, 64, dtype=torch.bool)
+    for b, n in enumerate(c.lens):
+        for p in range(n + T):
+            if 0 <= c.table[b, p // 64] < P:
+                used[c.table[b, p // 64], p % 64] = True
+    for n in ("k_pages", "v_pages"):
+        raw = c.c[n].view(torch.uint8)
+        raw[~used[:, None].expand(-1, c.nkv, -1)] = 0x7f
+        c.d[n].view(torch.uint8).copy_(raw)
+    q = c.set_q()
+    c.check_out(*c.attend(q))
+    q[5, 3], q[T + 6, 256] = math.nan, math.inf
+    c.q_buf.copy_(q)
+    want, tol = c.attend(q)
+    assert torch.isnan(want).any() and torch.isfinite(want).any()
+    c.check_out(want, tol)
+
+
+def test_attend_chunk_past_the_capacity():
+    """Tokens behind the last page are not there: their rows see what there is."""
+    c = Case(BF16, H2B, 40, [100, 128, 300], 64, 16, cap=128, rows=400)
+    c.check_out(*c.attend(c.set_q()))
+
+
+def test_append_then_attend_chunk():
+    """A prompt in chunks as a forward runs them, rows strided and not aligned, outputs beside others; a stored
+    NaN key is seen by the rows at and behind it."""
+    T = 33
+    c = Case(BF16, H2B, T, [0, 70], 64, 16, cap=256)
+    wide = torch.zeros(c.qkv.shape[0], c.qkv.shape[1] + 3, dtype=BF16, device=DEV)
+    out = torch.full((2 * T + 2, c.nh * c.hd + 7), 3.0, dtype=BF16, device=DEV)
+    d = c.layer(wide[:, 3:], out=out[:, 2:2 + c.nh * c.hd])
+    for step in range(3):
+        c.new_inputs()
+        if step == 2:
+            kv8.split(c.qkv, c.nh, c.nkv, c.hd)[2][T + 9, 1, 5] = math.inf
+        wide[:, 3:].copy_(c.qkv)
+        c.append(d)
+        c.check_stored()
+        want, tol = c.attend(c.q_buf.cpu(), d)
+        c.out.copy_(out[:2 * T, 2:2 + c.nh * c.hd])
+        c.check_out(want, tol)
+        assert (out[2 * T:] == 3).all() and (out[:, :2] == 3).all() and (out[:, 2 + c.nh * c.hd:] == 3).all()
+        c.lens = c.c["lens"] = [n + T for n in c.lens]
+        c.d["seq_lens"].copy_(torch.tensor(c.lens, dtype=torch.int32))
+    assert torch.isnan(want).any() and torch.isfinite(want).any()
+
+
+def test_chunk_repeated_captured_and_two_at_once():
+    """Repeated calls give the same bits, two layers at once on two streams too; a captured graph replays on
+    new lengths and queries."""
+    a, b = Case(BF16, H2B, 17, [700, 90, 1300], 64, 16, seed=1), Case(BF16, HMHA, 70, [10, 1100], 64, 16, seed=2)
+    qa, qb = a.set_q(), b.set_q()
+    da, db = a.layer(), b.layer()
+    want = [a.attend(qa, da), b.attend(qb, db)]
+    torch.cuda.synchronize()
+    a0, b0 = a.out.clone(), b.out.clone()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(20):
+        with torch.cuda.stream(s1):
+            K().attn_kv8_verify(da)
+        with torch.cuda.stream(s2):
+            K().attn_kv8_verify(db)
+    torch.cuda.synchronize()
+    assert torch.equal(a.out, a0) and torch.equal(b.out, b0)
+    a.check_out(*want[0])
+    b.check_out(*want[1])
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s1):
+        K().attn_kv8_verify(da)
+    a.lens = a.c["lens"] = [4, 1290, 0]
+    a.d["seq_lens"].copy_(torch.tensor(a.lens, dtype=torch.int32))
+    qa = a.set_q()
+    g.replay()
+    torch.cuda.synchronize()
+    got = a.out.clone()
+    a.check_out(*a.attend(qa, da))
+    assert torch.equal(a.out, got)
