@@ -114,8 +114,11 @@ class Qwen3_5Cache:
         lens = self.seq_lens.long()
         if self.kv8:
             for j in range(t):
-                for pages, scales, x in ((self.k_pages[s], self.k_scales[s], k), (self.v_pages[s], self.v_scales[s], v)):
-                    self._append8(pages, scales, x[:, :, j].float(), lens + j)
+                kj, vj = k[:, :, j].float(), v[:, :, j].float()
+                v_fine = torch.isfinite(vj).all(-1, keepdim=True)
+                fine = v_fine & torch.isfinite(kj).all(-1, keepdim=True)
+                self._append8(self.k_pages[s], self.k_scales[s], torch.where(fine, kj, math.nan), lens + j)
+                self._append8(self.v_pages[s], self.v_scales[s], torch.where(v_fine, vj, 0.0), lens + j)
             self.seq_lens += t
             return self.read_kv(layer)
         for j in range(t):
@@ -130,11 +133,12 @@ class Qwen3_5Cache:
     def _append8(self, pages, scales, x, pos):
         """One token x (B, n_kv, hd) fp32 per sequence into 8-bit pages, by the rule of
         `qsp_attn_kv8_prep`: the block's scale is the least power of two that holds the token and
-        what the block has; earlier codes follow when it grows."""
+        what the block has; earlier codes follow when it grows. A head of NaN (a token that is not finite)
+        counts nothing."""
         page = self.page_table.long().gather(1, (pos // self.page_size)[:, None])[:, 0]
         slot, sb = pos % self.page_size, self.scale_block
         blk = slot // sb
-        m, e = torch.frexp(x.abs().amax(-1))                                   # (B, n_kv)
+        m, e = torch.frexp(x.abs().nan_to_num(nan=0.0).amax(-1))   # (B, n_kv)
         e = torch.where(m > 0, e - 9 + (m > 0.875).int(), -40).clamp_min(-40)
         was = torch.frexp(scales[page, :, blk])[1] - 1
         now = torch.where((slot % sb > 0)[:, None], torch.maximum(e, was), e)

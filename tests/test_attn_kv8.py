@@ -180,3 +180,24 @@ def test_cache_append_kv_matches_the_rule():
             assert torch.equal(got[1][b].double(), want.to(torch.bfloat16).double())
             assert torch.equal(got[0][b], -got[1][b])
     assert c.seen_tokens == 18
+
+
+def test_cache_append_kv_non_finite():
+    """As the kernel stores them: a token whose key or value is not finite in a kv head is a NaN key there, a value
+    that is not finite is zero, and neither counts in the block's scale."""
+    c, ref = (_cache(kv_dtype=kv8.F8, scale_block=8) for _ in range(2))
+    layer = c.cfg.attn_layers[0]
+    nkv, hd = c.cfg.num_key_value_heads, c.cfg.head_dim
+    g = torch.Generator().manual_seed(1)
+    k, v = torch.randn(2, 2, nkv, 6, hd, generator=g)
+    k0, v0 = k.clone(), v.clone()
+    k[0, 1, 2, 3], v[1, 0, 4, 1], v[1, 0, 4, 2] = float("inf"), float("nan"), float("-inf")
+    k0[0, 1, 2], k0[1, 0, 4], v0[1, 0, 4] = 0.0, 0.0, 0.0
+    c.append_kv(layer, k, v)
+    ref.append_kv(layer, k0, v0)
+    assert torch.equal(c.k_scales, ref.k_scales) and torch.equal(c.v_scales, ref.v_scales)
+    assert torch.equal(c.v_pages.view(torch.uint8), ref.v_pages.view(torch.uint8))
+    got = c.read_kv(layer)[0]
+    bad = torch.isnan(got)
+    assert bad[0, 1, 2].all() and bad[1, 0, 4].all() and int(bad.sum()) == 2 * hd
+    assert torch.equal(got[~bad], ref.read_kv(layer)[0][~bad])
