@@ -77,10 +77,11 @@ struct Row {
 #pragma unroll
       for (int i = 0; i < W; ++i) t = max(t, r[i] & 0x7fffffffu);
       return t;
-    }
+    } else {
 #pragma unroll
-    for (int i = 0; i < W; ++i) t = __vmaxu2(t, r[i] & 0x7fff7fffu);   // two halves at a time
-    return max(t & 0xffff0000u, t << 16);
+      for (int i = 0; i < W; ++i) t = __vmaxu2(t, r[i] & 0x7fff7fffu);   // two halves at a time
+      return max(t & 0xffff0000u, t << 16);
+    }
   }
 };
 constexpr uint32_t NOT_FINITE = 0x7f800000u;

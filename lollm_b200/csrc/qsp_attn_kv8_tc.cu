@@ -301,6 +301,15 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
           const Desc next = piece_at(piece + 1);
           more = next.n > 0;
           if (AHEAD && more) load_q(next);
+          if (p.whole && wq == 0) {   // gates of this group's rows into L2: a quarter of a row a lane
+#pragma unroll
+            for (int i = 0; i < RW; i += 8) {
+              const int rr = row0 + i + lane / 4, t = rr / nrep;
+              if (rr < rows_total)
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const __nv_bfloat16*>(L.qkv) + ((int64_t)p.b * L.tokens + t) * L.ld_qkv +
+                                                               (int64_t)(p.g * nrep + rr - t * nrep) * 2 * HD + HD + lane % 4 * (HD / 4)));
+            }
+          }
         }
         wait_bar(&sfull[sb], ph, abort);
         __syncwarp();
@@ -442,6 +451,28 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
       // product then runs beside the rest: l over the keys, O out of TMEM (thread = head dim).
       if (!AHEAD && more) load_q(piece_at(piece + 1));
       if (more) stage_q(piece + 1);
+      // gates, as they are in memory (whatever is done beside a load waits for it): they come in while the sums
+      // are added
+      uint16_t gates[CB * RW];
+      if (p.whole) {
+#pragma unroll
+        for (int mb = 0; mb < CB; ++mb) {
+          const int dim = mb * 128 + key_in;
+          int h = h_first;
+          const uint16_t* at = static_cast<const uint16_t*>(L.qkv) + ((int64_t)p.b * L.tokens + t_first) * L.ld_qkv +
+                               (int64_t)(p.g * nrep + h) * 2 * HD + HD + dim;
+#pragma unroll
+          for (int i = 0; i < RW; ++i) {
+            gates[mb * RW + i] = 0;
+            if (row0 + i < rows_total && dim < HD) gates[mb * RW + i] = *at;
+            at += 2 * HD;
+            if (++h == nrep) {
+              h = 0;
+              at += L.ld_qkv - (int64_t)nrep * 2 * HD;
+            }
+          }
+        }
+      }
       const float s = warp_transpose_reduce<RW, false>(l, lane);
       if (reducer) red[wg * 4 * RW + row_of<RW>(lane) * 4 + wq] = s;
       bar_sync(bar);
@@ -455,49 +486,35 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
       wait_bar(&pdone[(tile - 1) & 1], ((tile - 1) >> 1) & 1, abort);
       tc::fence_after();
       bar_sync(bar);
-#pragma unroll 1
-      for (int c = 0; c < CB * (RW / 8); ++c) {   // 8 rows of 128 head dims
-        const int mb = c / (RW / 8), i0 = c % (RW / 8) * 8, dim = mb * 128 + key_in;
-        uint32_t oh[8], ol[8];
-        tm_ld8(tlane + 2 * N + mb * N + i0, oh);
-        tm_ld8(tlane + 2 * N + mb * N + RW + i0, ol);
-        if (p.whole) {
-          const int first = row0 + i0, t0 = first / nrep, h0 = first - t0 * nrep;
-          const int64_t m0 = (int64_t)p.b * L.tokens + t0;
-          float gate[8];
-          int64_t mrow = m0;
-          int h = h0;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            gate[i] = 0.f;
-            if (first + i < rows_total && dim < HD)
-              gate[i] = __bfloat162float(
-                  static_cast<const __nv_bfloat16*>(L.qkv)[mrow * L.ld_qkv + (int64_t)(p.g * nrep + h) * 2 * HD + HD + dim]);
-            if (++h == nrep) {
-              h = 0;
-              ++mrow;
-            }
-          }
-          tm_wait_ld8(oh, ol);
-          mrow = m0;
-          h = h0;
+      for (int mb = 0; mb < CB; ++mb) {
+        const int dim = mb * 128 + key_in;
+        int h = h_first;
+        __nv_bfloat16* at = static_cast<__nv_bfloat16*>(L.out) + ((int64_t)p.b * L.tokens + t_first) * L.ld_out + (int64_t)(p.g * nrep + h) * HD + dim;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float v = fmaf(__uint_as_float(ol[i]), 0.0625f, __uint_as_float(oh[i])) * aux[r0 + i0 + i];
-            if (first + i < rows_total && dim < HD)
-              static_cast<__nv_bfloat16*>(L.out)[mrow * L.ld_out + (int64_t)(p.g * nrep + h) * HD + dim] = __float2bfloat16_rn(v * sigmoid_ex2(gate[i]));
-            if (++h == nrep) {
-              h = 0;
-              ++mrow;
-            }
-          }
-        } else {
+        for (int i0 = 0; i0 < RW; i0 += 8) {
+          uint32_t oh[8], ol[8];
+          tm_ld8(tlane + 2 * N + mb * N + i0, oh);
+          tm_ld8(tlane + 2 * N + mb * N + RW + i0, ol);
           tm_wait_ld8(oh, ol);
-          float* to = ws.o + ((int64_t)p.slot * R + r0 + i0) * HD + dim;
-          if (dim < HD) {
+          if (p.whole) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float g = __uint_as_float((uint32_t)gates[mb * RW + i0 + i] << 16);
+              const float v = fmaf(__uint_as_float(ol[i]), 0.0625f, __uint_as_float(oh[i])) * aux[r0 + i0 + i] * sigmoid_ex2(g);
+              if (row0 + i0 + i < rows_total && dim < HD) *at = __float2bfloat16_rn(v);
+              at += HD;
+              if (++h == nrep) {
+                h = 0;
+                at += L.ld_out - (int64_t)nrep * HD;
+              }
+            }
+          } else if (dim < HD) {
+            float* to = ws.o + ((int64_t)p.slot * R + r0 + i0) * HD + dim;
 #pragma unroll
             for (int i = 0; i < 8; ++i) to[i * HD] = fmaf(__uint_as_float(ol[i]), 0.0625f, __uint_as_float(oh[i]));
           }
+          __syncwarp();
         }
       }
       tc::fence_before();   // the next piece's products overwrite O after its pfull
