@@ -154,6 +154,15 @@ __device__ __forceinline__ bool bar_any(int id, bool p) {
 constexpr uint32_t MISSING = 0xffffu;   // scale exponents of a key that has no page
 
 // ---------------------------------------------------------------- the loading warps
+// a box at (x, row) under an L2 policy; issued by a converged warp
+__device__ __forceinline__ void load_box(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int row, uint64_t policy) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4}], [%2], %5;\n\t}" ::"r"(
+          tc::smem_u32(dst)),
+      "l"(map), "r"(tc::smem_u32(bar)), "r"(x), "r"(row), "l"(policy)
+      : "memory");
+}
 // K or V tiles of the CTA's pieces into a ring of `slots`, by TMA: boxes of box_rows keys x CW bytes; lane i looks
 // up the page of the tile's i-th box_rows keys, one tile ahead. once: no other CTA reads the tile.
 template <int HD, int CW, typename PieceAt>
@@ -164,6 +173,9 @@ __device__ __forceinline__ void load_tiles(const qsp_attn_kv8_layer& L, const CU
   const int chunks = TILE / box_rows, pages_step = TILE / L.page_size, slot_step = TILE % L.page_size;
   int slot = 0;
   uint32_t turn = 1;   // parity of "empty" for this turn of the ring
+  uint64_t policy;     // what is read once stays out of the way of queries, page tables and partials in L2
+  if (once) asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+  else asm("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy));
   for (uint32_t piece = 0;; ++piece) {
     const Desc p = piece_at(piece);
     if (p.n == 0) break;
@@ -192,11 +204,7 @@ __device__ __forceinline__ void load_tiles(const qsp_attn_kv8_layer& L, const CU
         const int r = __shfl_sync(0xffffffffu, row, i);
         if (r >= 0) {
 #pragma unroll
-          for (int cb = 0; cb < HD / CW; ++cb) {
-            // read once: kept out of the way of queries, page tables and partials in L2
-            if (once) tc::tma_load_2d_evict_first_warp(dst + cb * (TILE * CW), map, &full[slot], cb * CW, r);
-            else tc::tma_load_2d_warp(dst + cb * (TILE * CW), map, &full[slot], cb * CW, r);
-          }
+          for (int cb = 0; cb < HD / CW; ++cb) load_box(dst + cb * (TILE * CW), map, &full[slot], cb * CW, r, policy);
         }
       }
       if (++slot == slots) {
