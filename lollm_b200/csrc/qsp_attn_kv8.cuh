@@ -120,7 +120,7 @@ __device__ __forceinline__ int exp_of(float scale) { return ((__float_as_int(sca
 // Units of 128 rows leave partials of 128 KB (hd 256), so dividing costs more: 2 x 512 tokens over 8k keys took
 // 144 us with a bound of 10 tiles, which divides them, 124 us with 12.
 constexpr int UNIT_COST = 3;
-__device__ __forceinline__ int merge_cost(int R) { return R > 64 ? 12 : 6; }
+__host__ __device__ __forceinline__ int merge_cost(int R) { return R > 64 ? 12 : 6; }
 
 struct Piece {
   int b, rg, g;
