@@ -432,7 +432,7 @@ static int launch_simt(const qsp_attn_kv8_layer& L, int G, cudaStream_t st) {
 }
 
 // ------------------------------------------------------------------ merge of divided units
-// CTA (c, y): 8 rows, a warp each, of the divided unit whose first tile attention CTA c had, if there is one;
+// CTA (c, y): `each` times 8 rows, a warp each, of the divided unit whose first tile attention CTA c had, if there is one;
 // or (WIDE, for few units of many parts) CTA (u, r): row r of the u-th divided unit, its partials dealt out to 8
 // warps. A warp weights its partials with 2^(m_p − M) and adds them in their order, a lane HD/32 columns, four
 // in flight at a time; WIDE adds the warps' sums in order. Then / l and the gate. Bound by latency: the
@@ -440,7 +440,7 @@ static int launch_simt(const qsp_attn_kv8_layer& L, int G, cudaStream_t st) {
 constexpr int MERGE_WARPS = 8;
 
 template <typename T, int HD, bool WIDE>
-__global__ void __launch_bounds__(32 * MERGE_WARPS, 3) merge_kernel(const qsp_attn_kv8_layer L, int G, int R) {
+__global__ void __launch_bounds__(32 * MERGE_WARPS, 3) merge_kernel(const qsp_attn_kv8_layer L, int G, int R, int each, bool vec) {
   pdl_trigger();
   pdl_wait();
   constexpr int EPL = HD / 32, DEPTH = 4;
@@ -478,78 +478,87 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS, 3) merge_kernel(const qsp_at
     if (c < 0) return;
   }
   const int4 meta = ws.meta[c];
-  const int np = meta.w, r = WIDE ? blockIdx.y : blockIdx.y * MERGE_WARPS + warp;
-  const int nrep = L.n_heads / L.n_kv_heads, rr = meta.y * R + r;
-  if (np == 0 || r >= R || rr >= nrep * L.tokens) return;   // the same for the whole CTA if WIDE
-  const int first = 2 * c + (meta.z >> 30);
-  auto slot = [&](int q) { return (int64_t)(q == 0 ? first : 2 * (c + q)) * R + r; };
-  const int t = rr / nrep, hq = (meta.z & ((1 << 30) - 1)) * nrep + rr - t * nrep;
-  const int64_t m = (int64_t)meta.x * L.tokens + t;
-  Row<T, EPL> gate;
-  gate.load(static_cast<const T*>(L.qkv) + m * L.ld_qkv + (int64_t)hq * 2 * HD + HD, lane, false);
-  float acc[EPL], den = 0.f, M = -INFINITY;   // sums relative to 2^M, the largest so far
-#pragma unroll
-  for (int i = 0; i < EPL; ++i) acc[i] = 0.f;
-  const int per = WIDE ? (np + MERGE_WARPS - 1) / MERGE_WARPS : np;
-  const int q_begin = WIDE ? warp * per : 0, q_end = min(np, q_begin + per);
-  for (int q0 = q_begin; q0 < q_end; q0 += DEPTH) {
-    Row<float, EPL> v[DEPTH];
-    float2 ml[DEPTH];
-    float top = M;
-#pragma unroll
-    for (int u = 0; u < DEPTH; ++u) {
-      ml[u] = make_float2(-INFINITY, 0.f);
-      v[u].zero();
-      if (q0 + u < q_end) {
-        ml[u] = ws.ml[slot(q0 + u)];
-        v[u].load(ws.o + slot(q0 + u) * HD, lane, true);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < DEPTH; ++u) top = fmaxf(top, ml[u].x);
-    const float ref = top == -INFINITY ? 0.f : top, old = exp2f(M - ref);
-    M = top;
-    den *= old;
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) acc[i] *= old;
-#pragma unroll
-    for (int u = 0; u < DEPTH; ++u) {
-      if (ml[u].y != 0.f) {   // else a part of which the row saw nothing
-        const float f = exp2f(ml[u].x - ref);
-        den = fmaf(f, ml[u].y, den);
-#pragma unroll
-        for (int i = 0; i < EPL; ++i) acc[i] = fmaf(f, v[u][i], acc[i]);
-      }
-    }
-  }
-  if constexpr (WIDE) {
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) part[warp][lane * EPL + i] = acc[i];
-    if (lane == 0) {
-      part[warp][HD] = den;
-      part_m[warp] = M;
-    }
-    __syncthreads();
-    if (warp != 0) return;
-    float top = M;
-#pragma unroll
-    for (int w = 1; w < MERGE_WARPS; ++w) top = fmaxf(top, part_m[w]);
-    const float ref = top == -INFINITY ? 0.f : top;
-    den = 0.f;
+  const int np = meta.w, nrep = L.n_heads / L.n_kv_heads, first = 2 * c + (meta.z >> 30);
+  if (np == 0) return;
+#pragma unroll 1
+  for (int it = 0; it < each; ++it) {
+    const int r = WIDE ? blockIdx.y : (blockIdx.y * each + it) * MERGE_WARPS + warp, rr = meta.y * R + r;
+    if (r >= R || rr >= nrep * L.tokens) return;   // the same for the whole CTA if WIDE
+    auto slot = [&](int q) { return (int64_t)(q == 0 ? first : 2 * (c + q)) * R + r; };
+    const int t = rr / nrep, hq = (meta.z & ((1 << 30) - 1)) * nrep + rr - t * nrep;
+    const int64_t m = (int64_t)meta.x * L.tokens + t;
+    Row<T, EPL> gate;
+    gate.load(static_cast<const T*>(L.qkv) + m * L.ld_qkv + (int64_t)hq * 2 * HD + HD, lane, vec);
+    float acc[EPL], den = 0.f, M = -INFINITY;   // sums relative to 2^M, the largest so far
 #pragma unroll
     for (int i = 0; i < EPL; ++i) acc[i] = 0.f;
+    const int per = WIDE ? (np + MERGE_WARPS - 1) / MERGE_WARPS : np;
+    const int q_begin = WIDE ? warp * per : 0, q_end = min(np, q_begin + per);
+    for (int q0 = q_begin; q0 < q_end; q0 += DEPTH) {
+      Row<float, EPL> v[DEPTH];
+      float2 ml[DEPTH];
+      float top = M;
 #pragma unroll
-    for (int w = 0; w < MERGE_WARPS; ++w) {
-      const float f = exp2f(part_m[w] - ref);
-      den = fmaf(f, part[w][HD], den);
+      for (int u = 0; u < DEPTH; ++u) {
+        ml[u] = make_float2(-INFINITY, 0.f);
+        v[u].zero();
+        if (q0 + u < q_end) {
+          ml[u] = ws.ml[slot(q0 + u)];
+          v[u].load(ws.o + slot(q0 + u) * HD, lane, true);
+        }
+      }
 #pragma unroll
-      for (int i = 0; i < EPL; ++i) acc[i] = fmaf(f, part[w][lane * EPL + i], acc[i]);
+      for (int u = 0; u < DEPTH; ++u) top = fmaxf(top, ml[u].x);
+      const float ref = top == -INFINITY ? 0.f : top, old = exp2f(M - ref);
+      M = top;
+      den *= old;
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) acc[i] *= old;
+#pragma unroll
+      for (int u = 0; u < DEPTH; ++u) {
+        if (ml[u].y != 0.f) {   // else a part of which the row saw nothing
+          const float f = exp2f(ml[u].x - ref);
+          den = fmaf(f, ml[u].y, den);
+#pragma unroll
+          for (int i = 0; i < EPL; ++i) acc[i] = fmaf(f, v[u][i], acc[i]);
+        }
+      }
+    }
+    if constexpr (WIDE) {
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) part[warp][lane * EPL + i] = acc[i];
+      if (lane == 0) {
+        part[warp][HD] = den;
+        part_m[warp] = M;
+      }
+      __syncthreads();
+      if (warp != 0) return;
+      float top = M;
+#pragma unroll
+      for (int w = 1; w < MERGE_WARPS; ++w) top = fmaxf(top, part_m[w]);
+      const float ref = top == -INFINITY ? 0.f : top;
+      den = 0.f;
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) acc[i] = 0.f;
+#pragma unroll
+      for (int w = 0; w < MERGE_WARPS; ++w) {
+        const float f = exp2f(part_m[w] - ref);
+        den = fmaf(f, part[w][HD], den);
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) acc[i] = fmaf(f, part[w][lane * EPL + i], acc[i]);
+      }
+    }
+    T* out = static_cast<T*>(L.out) + m * L.ld_out + (int64_t)hq * HD;
+    const float inv = den == 0.f ? 0.f : 1.f / den;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) acc[i] = acc[i] * inv * sigmoidf_(gate[i]);
+    if (vec) {
+      store_row<T, EPL>(out, lane, acc);
+    } else {
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) out[lane * EPL + i] = dt<T>::from_f(acc[i]);
     }
   }
-  T* out = static_cast<T*>(L.out) + m * L.ld_out + (int64_t)hq * HD + lane * EPL;
-  const float inv = den == 0.f ? 0.f : 1.f / den;
-#pragma unroll
-  for (int i = 0; i < EPL; ++i) out[i] = dt<T>::from_f(acc[i] * inv * sigmoidf_(gate[i]));
 }
 
 template <typename T, int HD>
@@ -558,11 +567,16 @@ static int launch_merge_hd(const qsp_attn_kv8_layer& L, int G, int R, cudaStream
   const int64_t units = (int64_t)L.batch * L.n_kv_heads * ((rows + R - 1) / R);
   // few units of many parts each, and few rows: a CTA a row (one sequence of 32k keys, hd 256: 74 parts). Many rows fill the
   // GPU by themselves.
+  constexpr int A = std::min<int>(16, HD / 32 * sizeof(T));
+  const bool vec = aligned(L.qkv, A) && aligned(L.out, A) && (L.ld_qkv * (int64_t)sizeof(T)) % A == 0 && (L.ld_out * (int64_t)sizeof(T)) % A == 0;
   if (units * MERGE_WARPS <= G && units * std::min(R, rows) <= 2 * tc::sm_count())
     return launch_pdl("qsp_attn_kv8_verify(merge)", merge_kernel<T, HD, true>, dim3((unsigned)units, std::min(R, rows)),
-                      dim3(32 * MERGE_WARPS), 0, st, L, G, R);
+                      dim3(32 * MERGE_WARPS), 0, st, L, G, R, 1, vec);
+  // 128 rows of many units: fewer CTAs, most of which find nothing to do (8 x 127 tokens over 1-2k keys, all whole: 47.6 us
+  // with 1, 45.5 with 4); of few units: one row a warp (1 x 128 over 16k: 55.5 and 64.7)
+  const int each = R > 64 && 2 * units >= G ? 4 : 1;
   return launch_pdl("qsp_attn_kv8_verify(merge)", merge_kernel<T, HD, false>,
-                    dim3(G, (std::min(R, rows) + MERGE_WARPS - 1) / MERGE_WARPS), dim3(32 * MERGE_WARPS), 0, st, L, G, R);
+                    dim3(G, (std::min(R, rows) + each * MERGE_WARPS - 1) / (each * MERGE_WARPS)), dim3(32 * MERGE_WARPS), 0, st, L, G, R, each, vec);
 }
 
 template <typename T>
