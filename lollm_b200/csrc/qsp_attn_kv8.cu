@@ -12,18 +12,18 @@ namespace kv8 {
 // ------------------------------------------------------------------ prep
 // Two kinds of CTA (8 warps) in one launch. The first n_kv_jobs quantise: K and V of one (sequence,
 // touched block of tokens, kv head) each, a warp a token, so that the block's largest magnitudes are
-// reduced and its scales and earlier codes are rewritten by one CTA, without atomics. The others norm and rotate q, two token
-// rows each, a warp four heads at a time (8 KB a row in flight). A lane holds HD/32 consecutive dims of
-// a row; the rotation's other half is the same element of another lane.
+// reduced and its scales and earlier codes are rewritten by one CTA, without atomics. The others norm and
+// rotate q, two token rows each, a warp two or four heads at a time. A lane holds HD/32 consecutive dims
+// of a row; the rotation's other half is the same element of another lane.
 //
 // k is normed and rotated in fp64: with 3 mantissa bits a value next to a rounding border would
 // otherwise fall to either side with the order of the sum, and a cached code lives as long as its
 // sequence. There are 1/8 as many k as q heads, and B200 runs fp64 at half the fp32 rate.
 //
-// Bound by latency: one token 3.1 us on the device (length, then page and row, then the block's scale); 16 x 127
-// tokens of 16 + 2 x 2 heads of 256 13.5 us, 40 MB of which the q part alone takes 9. (16 or 4 warps a CTA, 3 or 6 CTAs
-// an SM: no faster.)
-constexpr int PREP_WARPS = 8, PREP_ROWS = 2, PREP_HEADS = 4;
+// Small calls are bound by latency: one token 3.3 us, 64 x 4 tokens 4.2 (length, then page and row, then the block's scale).
+// 16 x 127 tokens of 16 + 2 x 2 heads of 256: 13.2 us for 40 MB, bound by instructions (issued in 0.7 of the cycles:
+// 130 for a head of q, three times as many for one of k), of which the q part alone takes 9.
+constexpr int PREP_WARPS = 8, PREP_ROWS = 2;
 
 // EPL codes of a lane, EPL bytes at dst + lane·EPL
 template <int EPL>
@@ -87,11 +87,13 @@ __device__ __forceinline__ void rotate_row(F (&y)[EPL], const Row<T, EPL>& cs, c
   }
 }
 
-template <typename T, int HD>
-__global__ void __launch_bounds__(32 * PREP_WARPS, 4)
+// OCC: CTAs an SM. At 4 a thread has 64 registers and the fp64 part spills: calls whose CTAs fit three an SM take 3, and
+// four heads a warp in flight (64 x 4 tokens 5.2 -> 4.2 us); for more of them occupancy counts (16 x 127 13.8 us at 3, 13.1 at 4).
+template <typename T, int HD, int OCC>
+__global__ void __launch_bounds__(32 * PREP_WARPS, OCC)
 prep_kernel(const qsp_attn_kv8_layer L, int n_kv_jobs, int most, bool vec, bool vec_w, bool vec_rope) {
   pdl_trigger();
-  constexpr int EPL = HD / 32;
+  constexpr int EPL = HD / 32, PREP_HEADS = OCC == 3 ? 4 : 2;
   __shared__ uint32_t red[2][PREP_WARPS];
   extern __shared__ float keys[];   // [scale_block][HD] of a quantising CTA
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -114,6 +116,12 @@ prep_kernel(const qsp_attn_kv8_layer L, int n_kv_jobs, int most, bool vec, bool 
     if (m >= (int64_t)L.batch * L.tokens) return;
     const int b = (int)(m / L.tokens);
     const int len = L.seq_lens[b];
+    // what all heads share, as they use it: the kernel is bound by instructions
+    float w1[EPL];
+    const int half = rd / 2 / EPL;   // lanes
+    const bool low = lane < half, in = lane * EPL < rd;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) w1[i] = w[i] + 1.f;
     for (int h0 = warp % WPR; h0 < nh; h0 += WPR * PREP_HEADS) {
       Row<T, EPL> x[PREP_HEADS];
 #pragma unroll
@@ -123,13 +131,26 @@ prep_kernel(const qsp_attn_kv8_layer L, int n_kv_jobs, int most, bool vec, bool 
         // a position outside the table is flagged by the quantising CTAs; its q is rotated as position 0
         const long long at = (long long)len + (m - (int64_t)b * L.tokens);
         load_rope(at >= 0 && at < L.rope_rows ? (int)at : 0);
+        if (low) sn.negate();
       }
 #pragma unroll
       for (int i = 0; i < PREP_HEADS; ++i) {
         if (h0 + i * WPR < nh) {
-          float y[EPL];
-          norm_row<T, EPL, float>(x[i], w, L.eps, y);
-          rotate_row<T, EPL, float>(y, cs, sn, rd, lane);
+          float y[EPL], ss = 0.f;
+#pragma unroll
+          for (int k = 0; k < EPL; ++k) {
+            y[k] = x[i][k];
+            ss = fmaf(y[k], y[k], ss);
+          }
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          const float inv = rsqrtf(ss * (1.f / HD) + L.eps);
+#pragma unroll
+          for (int k = 0; k < EPL; ++k) {
+            y[k] = y[k] * inv * w1[k];
+            const float other = __shfl_sync(0xffffffffu, y[k], low ? lane + half : lane - half);
+            if (in) y[k] = fmaf(other, sn[k], y[k] * cs[k]);
+          }
           store_row<T, EPL>(static_cast<T*>(L.q_buf) + (m * nh + h0 + i * WPR) * HD, lane, y);
         }
       }
@@ -243,7 +264,7 @@ static int launch_prep(const qsp_attn_kv8_layer& L, cudaStream_t st) {
   const bool vec_w = aligned(L.q_norm_w, A) && aligned(L.k_norm_w, A);
   const bool vec_rope = aligned(L.rope_cos, A) && aligned(L.rope_sin, A) && (L.rotary_dim * (int64_t)sizeof(T)) % A == 0;
   const size_t smem = (size_t)sb * HD * sizeof(float);
-  auto kern = prep_kernel<T, HD>;
+  auto kern = jobs + rows <= 3 * tc::sm_count() ? prep_kernel<T, HD, 3> : prep_kernel<T, HD, 4>;
   if (smem > 40 * 1024) {   // past the 48 KB that need no leave
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return set_error(QSP_ERR_CUDA, "qsp_attn_kv8_prep: %s", cudaGetErrorString(e));

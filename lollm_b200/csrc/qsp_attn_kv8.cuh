@@ -70,6 +70,10 @@ struct Row {
 #pragma unroll
     for (int i = 0; i < W; ++i) r[i] = 0;
   }
+  __device__ __forceinline__ void negate() {
+#pragma unroll
+    for (int i = 0; i < W; ++i) r[i] ^= sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
+  }
   // bits of the largest magnitude (they compare as the values do; 0x7f800000 and over: not finite)
   __device__ __forceinline__ uint32_t top() const {
     uint32_t t = 0;
