@@ -21,8 +21,8 @@ namespace kv8 {
 // sequence. There are 1/8 as many k as q heads, and B200 runs fp64 at half the fp32 rate.
 //
 // Small calls are bound by latency: one token 3.3 us, 64 x 4 tokens 4.2 (length, then page and row, then the block's scale).
-// 16 x 127 tokens of 16 + 2 x 2 heads of 256: 13.2 us for 40 MB, bound by instructions (issued in 0.7 of the cycles:
-// 130 for a head of q, three times as many for one of k), of which the q part alone takes 9.
+// 16 x 127 tokens of 16 + 2 x 2 heads of 256: 13.2 us for 40 MB, bound by instructions (issued in 0.7 of the
+// cycles), of which the q part alone takes 9.
 constexpr int PREP_WARPS = 8, PREP_ROWS = 2;
 
 // EPL codes of a lane, EPL bytes at dst + lane·EPL
@@ -61,29 +61,29 @@ __device__ __forceinline__ void store_row(T* p, int lane, const float (&y)[EPL])
   }
 }
 
-// x -> RMS-normed times 1 + w, in F (float for q, double for k)
-template <typename T, int EPL, typename F>
-__device__ __forceinline__ void norm_row(const Row<T, EPL>& x, const Row<T, EPL>& w, float eps, F (&y)[EPL]) {
-  F ss = 0;
+// x -> RMS-normed times 1 + w, in 64 bits
+template <typename T, int EPL>
+__device__ __forceinline__ void norm_row(const Row<T, EPL>& x, const Row<T, EPL>& w, float eps, double (&y)[EPL]) {
+  double ss = 0;
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) ss += (F)x[i] * (F)x[i];
+  for (int i = 0; i < EPL; ++i) ss += (double)x[i] * (double)x[i];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  const F inv = rsqrt(ss / (F)(32 * EPL) + (F)eps);
+  const double inv = rsqrt(ss / (double)(32 * EPL) + (double)eps);
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) y[i] = (F)x[i] * inv * ((F)w[i] + (F)1);
+  for (int i = 0; i < EPL; ++i) y[i] = (double)x[i] * inv * ((double)w[i] + (double)1);
 }
 
 // the first rd dims rotated: y[d] <- y[d]·cos[d] + (d < half ? -y[d + half] : y[d - half])·sin[d]; half is a
 // whole number of lanes. cs, sn: a lane's entries of the position's table row.
-template <typename T, int EPL, typename F>
-__device__ __forceinline__ void rotate_row(F (&y)[EPL], const Row<T, EPL>& cs, const Row<T, EPL>& sn, int rd, int lane) {
+template <typename T, int EPL>
+__device__ __forceinline__ void rotate_row(double (&y)[EPL], const Row<T, EPL>& cs, const Row<T, EPL>& sn, int rd, int lane) {
   const int lanes = rd / 2 / EPL, d = lane * EPL;
   const bool low = d < rd / 2, in = d < rd;
 #pragma unroll
   for (int i = 0; i < EPL; ++i) {
-    const F other = __shfl_sync(0xffffffffu, y[i], low ? lane + lanes : lane - lanes);
-    if (in) y[i] = y[i] * (F)cs[i] + (low ? -other : other) * (F)sn[i];
+    const double other = __shfl_sync(0xffffffffu, y[i], low ? lane + lanes : lane - lanes);
+    if (in) y[i] = y[i] * (double)cs[i] + (low ? -other : other) * (double)sn[i];
   }
 }
 
@@ -200,8 +200,8 @@ prep_kernel(const qsp_attn_kv8_layer L, int n_kv_jobs, int most, bool vec, bool 
     if (j != warp) load_token(j);
     const uint32_t v_top = __reduce_max_sync(0xffffffffu, v.top());
     double z[EPL];
-    norm_row<T, EPL, double>(x, w, L.eps, z);
-    rotate_row<T, EPL, double>(z, cs, sn, rd, lane);
+    norm_row<T, EPL>(x, w, L.eps, z);
+    rotate_row<T, EPL>(z, cs, sn, rd, lane);
     float y[EPL];
     uint32_t k_top = 0;
 #pragma unroll
