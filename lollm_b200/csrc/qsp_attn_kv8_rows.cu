@@ -23,7 +23,7 @@
 // A tile takes 1024 + 900 cycles of the tensor cores at hd 256 (hi and lo) and 2100 of the softmax: 64
 // exponentials a thread at 16 an SM and cycle are half of that. They overlap but for the start of each; 2700
 // cycles were measured. Against 64 rows a unit (tc_kernel in groups): 8 sequences x 127 tokens over 1k to 2k keys, 2 kv
-// heads of 256, 84 -> 49 us; 64 x 16 over 2k 97 -> 54 us; 4 x 2048 from an empty cache 665 -> 302 us; 27 x 64
+// heads of 256, 84 -> 45 us; 64 x 16 over 2k 97 -> 54 us; 4 x 2048 from an empty cache 665 -> 302 us; 27 x 64
 // tokens of 1 x 2 heads over 4k to 9k 93 -> 71 us.
 #include "qsp_attn_kv8_tc.cuh"
 
