@@ -576,3 +576,27 @@ def test_chunk_repeated_captured_and_two_at_once():
     got = a.out.clone()
     a.check_out(*a.attend(qa, da))
     assert torch.equal(a.out, got)
+
+
+@pytest.mark.parametrize("heads,T,lens,sb", [(H2B, 1100, [37, 0, 2000], 16), (HMHA, 1500, [0, 900], 64), (HMICRO, 3000, [5], 8)])
+def test_attend_long_chunk(heads, T, lens, sb):
+    """Many row groups a sequence: some tokens of each against the definition (bound as in `_attend_bound`)."""
+    c = Case(BF16, heads, T, lens, 64, sb)
+    q = c.set_q().double().view(-1, c.nh, c.hd)
+    K().attn_kv8_verify(c.layer())
+    got = c.out.double().cpu().view(-1, c.nh, c.hd)
+    gate = torch.sigmoid(kv8.split(c.qkv, c.nh, c.nkv, c.hd)[1].double())
+    rep = c.nh // c.nkv
+    for b, n in enumerate(lens):
+        for t in (0, 1, 15, 16, 17, 63, 127, 128, T // 2, T - 2, T - 1):
+            m, row = n + t + 1, b * T + t
+            k, v, has = kv8.read(c.c, b, m)
+            assert has.all()
+            for g in range(c.nkv):
+                h = slice(g * rep, (g + 1) * rep)
+                s = q[row, h] @ k[g].T * c.hd ** -0.5
+                want = torch.softmax(s, -1) @ v[g] * gate[row, h]
+                A = (q[row, h].abs() @ k[g].abs().T).amax(-1, keepdim=True) * c.hd ** -0.5 + 1
+                tol = (2 * (c.hd + 2) * 2.0 ** -23 * A + 2 * m * 2.0 ** -23 + 2.0 ** -8 + m * 2.0 ** -18) * v[g].abs().max() * gate[row, h]
+                assert ((got[row, h] - want).abs() <= tol + (want.abs() + tol) * torch.finfo(BF16).eps / 2).all(), (b, t, g)
+    assert K().device_status() == 0
