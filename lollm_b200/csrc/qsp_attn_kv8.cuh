@@ -12,6 +12,7 @@ namespace kv8 {
 
 constexpr int TILE = 128;      // keys of a tensor-core work tile
 constexpr int SIMT_TILE = 32;  // ... of one of the CUDA-core kernel
+constexpr int GROUP = 8;       // keys that share their scales in rows_kernel: scale_block is a multiple
 constexpr int MIN_EXP = -40;   // least exponent of a scale
 constexpr int MAX_EXP = 120;   // 448·2^120 holds every fp32 value
 constexpr float LOG2E = 1.4426950408889634f;

@@ -1,5 +1,5 @@
 // Attention over the 8-bit KV cache for many query rows (chunks of prompts) on tcgen05 tensor cores: bf16
-// models, page sizes that are a multiple of 8, more than 64 rows (tokens x heads of the kv head).
+// models, page sizes and scale blocks that are a multiple of 8, more than 64 rows (tokens x heads of the kv head).
 //
 // A unit is 128 query rows, which are the rows of the products:
 //   S [128, 128 keys] = Q [128, hd] · K^T       A = Q from shared memory, B = K as it lies in the cache
@@ -33,7 +33,6 @@ namespace qsp {
 namespace kv8 {
 
 constexpr int RR = 128;    // rows of a unit
-constexpr int GROUP = 8;   // keys that share their scales: scale_block is a multiple
 
 template <int HD>
 struct RowsCfg {

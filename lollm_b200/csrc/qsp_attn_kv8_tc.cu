@@ -587,7 +587,9 @@ int launch_tc(const qsp_attn_kv8_layer& L, cudaStream_t st) {
   if (!make_map(&mk, L.k_pages, rows, L.head_dim, box_rows) || !make_map(&mv, L.v_pages, rows, L.head_dim, box_rows))
     return set_error(QSP_ERR_CUDA, "qsp_attn_kv8_verify: no tensor map for the pages");
   const int R = tc_rows(L.n_heads / L.n_kv_heads * L.tokens);
-  if (R == 128 && L.scale_block >= 8) return launch_rows(L, mk, mv, box_rows, st);
+  // rows_kernel takes the scales of 8 keys at a time; with smaller blocks: groups of 64 rows (8 x 127 tokens over 1-2k keys
+  // 84 us, where it takes 45)
+  if (R == 128 && L.scale_block >= GROUP) return launch_rows(L, mk, mv, box_rows, st);
   switch (L.head_dim) {
     case 32: return launch_tc_hd<32>(L, R, mk, mv, box_rows, st);
     case 64: return launch_tc_hd<64>(L, R, mk, mv, box_rows, st);
