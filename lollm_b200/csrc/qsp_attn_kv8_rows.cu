@@ -9,13 +9,14 @@
 // and O: hi holds the upper 4 bits; what is left is at most 8 units of a bf16's last place, which e5m2's 3 bits
 // hold exactly, so q is exact down to 2^-16 of a row whose largest value is 224 to 448. A weight is
 // off by half a step of lo, 2^-8 of its power of two, or by 2^-14 below 2^-10, where hi is 0; weights are held
-// times 2^BIAS, so that is 2^-18 of the largest.
+// times 2^BIAS, so that is 2^-18 of the largest. (They pass through fp16, 2^-12 more, for the cheaper conversions.)
 //
 // A row of S is one lane of TMEM: two threads have 64 of its keys each, warps i and 4 + i the same 32 rows.
 // They need not know the maximum exactly: m is raised, and O rescaled, only when a score passes it by more
 // than 2^SLACK, which the two warps learn from one barrier with a vote. The scales of the keys multiply
 // the scores, those of the values are added to them as log2 units (so that O's weights are p·vscale, at
-// most 2^SLACK, and the sum takes them back): fp32 pairs of three arrays in shared memory.
+// most 2^SLACK, and the sum takes them back). 8 keys share their scales, so an exponent is one fused multiply-add of
+// a score. (Scales of single keys: 1500 of a tile's cycles were their reads from shared memory.)
 //
 // QK of a tile runs while the weights of the one before are computed (its scores are in registers by then),
 // and the weights' product after it.
@@ -24,7 +25,7 @@
 // exponentials a thread at 16 an SM and cycle are half of that. They overlap but for the start of each; 2700
 // cycles were measured. Against 64 rows a unit (tc_kernel in groups): 8 sequences x 127 tokens over 1k to 2k keys, 2 kv
 // heads of 256, 84 -> 45 us; 64 x 16 over 2k 97 -> 54 us; 4 x 2048 from an empty cache 665 -> 302 us; 27 x 64
-// tokens of 1 x 2 heads over 4k to 9k 93 -> 71 us.
+// tokens of 4 and 2 heads over 4k to 9k 93 -> 69 us.
 #include "qsp_attn_kv8_tc.cuh"
 
 #include <algorithm>
