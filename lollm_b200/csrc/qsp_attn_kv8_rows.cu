@@ -4,12 +4,12 @@
 // A unit is 128 query rows, which are the rows of the products:
 //   S [128, 128 keys] = Q [128, hd] · K^T       A = Q from shared memory, B = K as it lies in the cache
 //   O [128, hd]      += P [128, 128 keys] · V   A = P from TMEM,          B = V read along its rows
-// The codes of K and V are operands as they are. Q (times a power of two per row) and the softmax weights P
-// are sums of an e4m3 and an e5m2 value, hi = e4m3(x), lo = e5m2(x - hi), which accumulate into the same S
-// and O: hi holds the upper 4 bits; what is left is at most 8 units of a bf16's last place, which e5m2's 3 bits
-// hold exactly, so q is exact down to 2^-16 of a row whose largest value is 224 to 448. A weight is
-// off by half a step of lo, 2^-8 of its power of two, or by 2^-14 below 2^-10, where hi is 0; weights are held
-// times 2^BIAS, so that is 2^-18 of the largest. (They pass through fp16, 2^-12 more, for the cheaper conversions.)
+// The codes of K and V are operands as they are. Q (times a power of two per row) is the sum of an e4m3 and an
+// e5m2 value, hi = e4m3(q), lo = e5m2(q - hi), which accumulate into the same S: hi holds the upper 4 bits; what is
+// left is at most 8 units of a bf16's last place, which e5m2's 3 bits hold exactly, for elements down to 2^-6, of a
+// row whose largest is scaled to 224..448; smaller ones are off by at most 2^-14, 2^-21 of the largest. A softmax weight
+// is the sum of three e5m2 values (split_weights, unscaled: they accumulate into the same O), which is bf16's
+// precision down to 2^-20 of the row's largest.
 //
 // A row of S is one lane of TMEM: two threads have 64 of its keys each, warps i and 4 + i the same 32 rows.
 // They need not know the maximum exactly: m is raised, and O rescaled, only when a score passes it by more
@@ -21,11 +21,11 @@
 // QK of a tile runs while the weights of the one before are computed (its scores are in registers by then),
 // and the weights' product after it.
 //
-// A tile takes 1024 + 900 cycles of the tensor cores at hd 256 (hi and lo) and 2100 of the softmax: 64
-// exponentials a thread at 16 an SM and cycle are half of that. They overlap but for the start of each; 2700
-// cycles were measured. Against 64 rows a unit (tc_kernel in groups): 8 sequences x 127 tokens over 1k to 2k keys, 2 kv
-// heads of 256, 84 -> 45 us; 64 x 16 over 2k 97 -> 54 us; 4 x 2048 from an empty cache 665 -> 302 us; 27 x 64
-// tokens of 4 and 2 heads over 4k to 9k 93 -> 69 us.
+// A tile takes 1024 + 1350 cycles of the tensor cores at hd 256 (two parts of Q, three of P) and 2100 of the softmax: 64
+// exponentials a thread at 16 an SM and cycle are half of that. They overlap but for the start of each; about 3300
+// cycles were measured, and 2700 with weights of two parts, whose small ones were lost (8 sequences x 127 tokens over 1k
+// to 2k keys, 2 kv heads of 256, 48 and 53 us; 2 x 512 over 8k 119 and 145 us). At head sizes up to 128, where
+// TMEM has room for the weights of two tiles, the third part costs nothing (8 x 127 of size 64: 27 us).
 #include "qsp_attn_kv8_tc.cuh"
 
 #include <algorithm>
@@ -53,7 +53,9 @@ struct RowsCfg {
   static constexpr int NS = slots(), NSK = NS / 2, NSV = NS - NSK, NSE = NSK + 2;
   static constexpr size_t BYTES = bytes(NS);
   static constexpr int SOFTMAX = 256, THREADS = SOFTMAX + 128;
-  static constexpr int S = 0, P = 128, O = 256, COLS = 512;      // TMEM columns: scores, weights x 2, output
+  // TMEM columns: scores, weights (of two tiles where O leaves room), output
+  static constexpr int NP = HD <= 128 ? 2 : 1, PW = 96, S = 0, P = 128, O = 512 - (HD <= 128 ? 128 : HD), COLS = 512;
+  static_assert(P + NP * PW <= O, "the weights run into O");
   static_assert(NSK >= 2 && NSK <= 4, "ring too short, or too long for the descriptors' slots");
 };
 
@@ -236,11 +238,12 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
     if (lane == 0) put_meta(scratch(L, gridDim.x, RR), w, p);
   } else if (warp == W_MMA) {
     // ---------------- products, in the order QK(0) QK(1) PV(0) QK(2) PV(1) ... of each piece. QK(t) overwrites the
-    // scores of t - 1 once they are in registers. The weights of t go where those of t - 2 were: their product
-    // was issued before QK(t), whose scores the softmax has waited for.
+    // scores of t - 1 once they are in registers. With two buffers the weights of t go where those of t - 2 were:
+    // their product was issued before QK(t), whose scores the softmax has waited for. With one the softmax waits for
+    // the product of t - 1, which is done long before.
     constexpr int STEP = 32 * CW / 16;   // 32 keys of V
     constexpr uint32_t QK_HI = idesc_rows(TILE, false, false), QK_LO = idesc_rows(TILE, true, false);
-    constexpr uint32_t PV_HI = idesc_rows(CW, false, true), PV_LO = idesc_rows(CW, true, true);
+    constexpr uint32_t ID_PV = idesc_rows(CW, true, true);
     const Sdesc dK = sdesc<CW>(sK, 16), dV = sdesc<CW>(sV, 0), dQ = sdesc<CW>(sQ, 16);
     uint32_t tile = 0, kslot = 0, kturn = 0, vslot = 0, vturn = 0;
     for (uint32_t piece = 0;; ++piece) {
@@ -256,7 +259,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
         for (int part = 0; part < 2; ++part)
 #pragma unroll
           for (int cb = 0; cb < CB; ++cb)
-            umma_e4m3_warp<CW / 32, 2, 2>(tmem + C::S, {dQ.lo + (part * RR * HD + cb * RR * CW) / 16, dQ.hi},
+            umma_f8_warp<CW / 32, 2, 2>(tmem + C::S, {dQ.lo + (part * RR * HD + cb * RR * CW) / 16, dQ.hi},
                                           {dK.lo + (kslot * C::SLOT + cb * (TILE * CW)) / 16, dK.hi}, part ? QK_LO : QK_HI, part + cb > 0);
         tc::umma_commit_warp(&kempty[kslot]);
         tc::umma_commit_warp(sfull);
@@ -276,10 +279,10 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
 #pragma unroll
         for (int mb = 0; mb < CB; ++mb)
 #pragma unroll
-          for (int s = 0; s < 8; ++s) {   // 4 steps of 32 keys, hi and lo
-            const int k = s >> 1, lo = s & 1;
-            umma_ts_warp(tmem + C::O + mb * CW, tmem + C::P + pb * 64 + (k >> 1) * 32 + lo * 16 + (k & 1) * 8,
-                         {dV.lo + (vslot * C::SLOT + mb * (TILE * CW)) / 16 + k * STEP, dV.hi}, lo ? PV_LO : PV_HI, j > 0 || s > 0);
+          for (int s = 0; s < 12; ++s) {   // 4 steps of 32 keys, three parts
+            const int k = s / 3, part = s % 3;
+            umma_ts_warp(tmem + C::O + mb * CW, tmem + C::P + pb % C::NP * C::PW + (k >> 1) * 48 + part * 16 + (k & 1) * 8,
+                         {dV.lo + (vslot * C::SLOT + mb * (TILE * CW)) / 16 + k * STEP, dV.hi}, ID_PV, j > 0 || s > 0);
           }
         tc::umma_commit_warp(&vempty[vslot]);
         tc::umma_commit_warp(&pdone[pb]);
@@ -535,8 +538,8 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
             }
           }
         }
-        const uint32_t to = tlane + C::P + (tile & 1) * 64 + half * 32;
-        uint32_t hi[16], lo[16];
+        const uint32_t to = tlane + C::P + tile % C::NP * C::PW + half * 48;
+        uint32_t pa[16], pb[16], pc[16];
 #pragma unroll
         for (int g = 0; g < 64 / GROUP; ++g) {
           float2 sum = make_float2(0.f, 0.f);
@@ -545,14 +548,23 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
             const float2 x = make_float2(ex2(d[k]), ex2(d[k + 1])), y = make_float2(ex2(d[k + 2]), ex2(d[k + 3]));
             sum = add2(add2(x, y), sum);
             const __half2 hx = __floats2half2_rn(x.x, x.y), hy = __floats2half2_rn(y.x, y.y);
-            const uint16_t cx = half2_to_e4m3x2(hx), cy = half2_to_e4m3x2(hy);
-            hi[k / 4] = cx | (uint32_t)cy << 16;
-            lo[k / 4] = half2_to_e5m2x2(__hsub2(hx, e4m3x2_to_half2(cx))) | (uint32_t)half2_to_e5m2x2(__hsub2(hy, e4m3x2_to_half2(cy))) << 16;
+            uint32_t ax, bx, cx, ay, by, cy;
+            split_weights<1>(hx, ax, bx, cx);
+            split_weights<1>(hy, ay, by, cy);
+            pa[k / 4] = upper_bytes(ax, ay);
+            pb[k / 4] = upper_bytes(bx, by);
+            pc[k / 4] = upper_bytes(cx, cy);
           }
           l = fmaf(sum.x + sum.y, s[g].z, l);
         }
-        tm_st16(to, hi);
-        tm_st16(to + 16, lo);
+        if (C::NP == 1 && j > 0) {
+          wait_bar(&pdone[(tile - 1) & 1], ((tile - 1) >> 1) & 1, abort);
+          __syncwarp();
+          tc::fence_after();
+        }
+        tm_st16(to, pa);
+        tm_st16(to + 16, pb);
+        tm_st16(to + 32, pc);
         if (gaps && half == 0) {
           // a key that is not there: its value row is whatever lies in the slot, and 0·NaN is NaN
           wait_bar(&vfull[vslot], vturn, abort);

@@ -3,19 +3,22 @@
 // them in groups of 64; chunks of prompts have a kernel of their own, with 128 (rows_kernel).
 //
 // The products read the codes as they lie in the cache: nothing is dequantised. The other operand
-// is brought to 8 bits without losing what 16 bits hold, as the sum of two e4m3 values:
-//   q·2^-e      = hi + lo/16   hi = e4m3(q·2^-e), lo = e4m3(16·(q·2^-e − hi)), 2^e a power of two per row
-//   p·2^(v)     = hi + lo/16   of the softmax weights
-// e4m3 has 4 significant bits, so hi takes the upper 4 of a bf16's 8 and lo the lower 4, exactly; a
-// weight keeps 8 bits, as it would in bf16. hi and lo are columns of one product, whose halves
-// are added in fp32. The power-of-two scales of the keys multiply the scores; those of the values join
+// is brought to 8 bits as a sum:
+//   q·2^-e      = hi + lo/16        hi = e4m3(q·2^-e), lo = e4m3(16·(q·2^-e − hi)), 2^e a power of two per row
+//   p·2^(v)     = a + (b + c)/4     e5m2, of the softmax weights (split_weights)
+// e4m3 has 4 significant bits, so hi takes the upper 4 of a bf16's 8 and lo the lower 4: exactly for elements down to
+// 2^-6, of a row whose largest is scaled to 224..448; smaller ones are off by at most 2^-14, 2^-21 of the largest. A weight
+// has the precision of bf16 down to 2^-22 of the row's largest. hi and lo, a and b are columns of one product,
+// whose halves are added in fp32; c is a product of its own into b's columns, since TMEM has no more for a third
+// part of 64 rows. The power-of-two scales of the keys multiply the scores; those of the values join
 // the softmax: with y = log2(e)·s + log2(vscale), weights w = 2^(y − m), m the running maximum of y,
 // O = Σ w·vcode, l = Σ w / vscale. A weight's rounding is then relative to the largest contribution.
 //
 // Both products are transposed, so that the 128 rows of a tensor-core tile are keys (then head
 // dims) and not the few query rows of a verify step:
 //   S^T [128 keys, 2R]    = K [128, hd] · Q^T          A = the K tile, B = Q, hi rows then lo rows
-//   O^T [hd, 2R]         += V^T [hd, 128] · P^T        A = the V tile read along its rows, B = P
+//   O^T [hd, 2R]         += V^T [hd, 128] · P^T        A = the V tile read along its rows, B = P, a rows then b rows
+//   O^T [hd, second R]   += V^T [hd, 128] · Pc^T       B = the weights' c rows
 // with R = 8..64 query rows (tokens × heads of the kv head). A thread of the softmax has one key
 // and all R rows: its scales are scalars, the sum over keys is left to the end, and the maximum over
 // keys need not be known exactly: m is raised (and O rescaled in TMEM) only when some score passes it
@@ -26,9 +29,9 @@
 // scores and weights are double-buffered, so the next tile's scores are computed while this one's weights are.
 //
 // Bound by HBM where sequences are long: a tile of 128 keys at hd 256 is 64 KB, 2800 cycles of an SM's share of
-// 6.5 TB/s; its products take 520 cycles of the tensor cores at R = 32, its softmax a chain of 1830 cycles.
-// Measured, 2 kv heads of 256, 64 sequences of 1k to 32k keys: 1 token 174 us, 4 tokens 178 us (6.3 TB/s); of
-// 2048 to 2560 keys: 4 tokens 34 us (4.6 TB/s: 9 us are start, output and launch), 8 tokens (R = 64) 44 us. One token
+// 6.5 TB/s; its products take 780 cycles of the tensor cores at R = 32, its softmax a chain of some 1900 cycles.
+// Measured, 2 kv heads of 256, 64 sequences of 1k to 32k keys: 4 tokens 174 us in a graph of one
+// input (178 with weights of two parts); of 2048 to 2560 keys: 4 tokens 35 us (34), 8 tokens (R = 64) 46 us (43). One token
 // over 33 keys: 6.7 us, a chain of length, plan, page, scales and K, product, softmax, product, gate.
 #include "qsp_attn_kv8_tc.cuh"
 
@@ -44,13 +47,14 @@ struct Cfg {
   static constexpr int CW = HD < 128 ? HD : 128;            // bytes of a swizzled row
   static constexpr int CB = HD / CW;                        // column blocks of a tile
   static constexpr int SLOT = TILE * HD;                    // bytes of a K or V tile
-  static constexpr int QB = N * HD, PB = TILE * N;
+  static constexpr int NC = R < 16 ? 16 : R;                // columns of the weights' third part: an MMA has 16 at least
+  static constexpr int QB = N * HD, PB = TILE * N, PCB = TILE * NC;
   static constexpr int OCC = HD == 256 || R >= 32 ? 1 : 2;  // CTAs per SM
   static constexpr size_t BUDGET = OCC == 1 ? 232448 : 115712;
   // barriers, piece descriptors, row scales (of two pieces), maxima and factors, reduction buffer
   static constexpr int SMALL = 8 * 34 + NDESC * 32 + 4 * (2 * R + 2 * R + 4 * R) + 16;
   // slots of scale exponents: two more than of K
-  static constexpr size_t bytes(int ns) { return (size_t)ns * SLOT + QB + 2 * PB + SMALL + (ns / 2 + 2) * 2 * TILE; }
+  static constexpr size_t bytes(int ns) { return (size_t)ns * SLOT + QB + 2 * PB + 2 * PCB + SMALL + (ns / 2 + 2) * 2 * TILE; }
   static constexpr int slots() {
     int ns = 8;
     while (bytes(ns) > BUDGET) --ns;
@@ -96,12 +100,13 @@ __global__ void __launch_bounds__(Cfg<HD, R_>::THREADS, Cfg<HD, R_>::OCC)
 tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const qsp_attn_kv8_layer L, int n_rg,
           int box_rows) {
   using C = Cfg<HD, R_>;
-  constexpr int R = C::R, N = C::N, RW = C::RW, NWG = C::NWG, NSK = C::NSK, NSV = C::NSV, CW = C::CW, CB = C::CB, EPL = HD / 32;
+  constexpr int R = C::R, N = C::N, NC = C::NC, RW = C::RW, NWG = C::NWG, NSK = C::NSK, NSV = C::NSV, CW = C::CW, CB = C::CB, EPL = HD / 32;
   extern __shared__ __align__(1024) uint8_t sK[];                // the swizzles go by address: 1024-byte tiles
   uint8_t* sV = sK + NSK * C::SLOT;
   uint8_t* sQ = sV + NSV * C::SLOT;
   uint8_t* sP = sQ + C::QB;                                      // [2][128 keys][N]
-  uint64_t* kfull = reinterpret_cast<uint64_t*>(sP + 2 * C::PB);
+  uint8_t* sPc = sP + 2 * C::PB;                                 // [2][128 keys][NC]
+  uint64_t* kfull = reinterpret_cast<uint64_t*>(sPc + 2 * C::PCB);
   uint64_t* kempty = kfull + NSK;
   uint64_t* vfull = kempty + NSK;
   uint64_t* vempty = vfull + NSV;
@@ -176,9 +181,10 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
   } else if (warp == W_MMA) {
     // ---------------- products, in the order QK(0) QK(1) PV(0) QK(2) PV(1) ... of each piece. QK(t) overwrites the
     // scores of t - 2, which had been read when pfull(t - 2) came, before PV(t - 2) and so before QK(t).
-    constexpr uint32_t ID_QK = idesc_e4m3(128, N, false), ID_PV = idesc_e4m3(128, N, true);
+    constexpr uint32_t ID_QK = idesc_f8(128, N, false, false), ID_PV = idesc_f8(128, N, true, true), ID_PC = idesc_f8(128, NC, true, true);
     const Sdesc dK = sdesc<CW>(sK, 16), dV = sdesc<CW>(sV, 0), dQ = sdesc<CW>(sQ, 16);
     const Sdesc dP = N == 16 ? sdesc<16>(sP, 8 * 16) : sdesc<N < 32 ? 32 : N>(sP, 0);
+    const Sdesc dPc = NC == 16 ? sdesc<16>(sPc, 8 * 16) : sdesc<NC < 32 ? 32 : NC>(sPc, 0);
     uint32_t tile = 0, piece = 0, kslot = 0, kturn = 0, vslot = 0, vturn = 0;
     for (;; ++piece) {
       const int n = piece_at(piece).n;
@@ -191,7 +197,7 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
         tc::fence_after();
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb)
-          umma_e4m3_warp<CW / 32, 2, 2>(tmem + sb * N, {dK.lo + (kslot * C::SLOT + cb * (TILE * CW)) / 16, dK.hi},
+          umma_f8_warp<CW / 32, 2, 2>(tmem + sb * N, {dK.lo + (kslot * C::SLOT + cb * (TILE * CW)) / 16, dK.hi},
                                         {dQ.lo + cb * (N * CW) / 16, dQ.hi}, ID_QK, cb > 0);
         tc::umma_commit_warp(&kempty[kslot]);
         tc::umma_commit_warp(&sfull[sb]);
@@ -210,8 +216,12 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
         tc::fence_after();
 #pragma unroll
         for (int mb = 0; mb < CB; ++mb)
-          umma_e4m3_warp<4, 32 * CW / 16, 32 * N / 16>(tmem + 2 * N + mb * N, {dV.lo + (vslot * C::SLOT + mb * (TILE * CW)) / 16, dV.hi},
-                                                       {dP.lo + pb * C::PB / 16, dP.hi}, ID_PV, j > 0);
+        {
+          const Sdesc v = {dV.lo + (vslot * C::SLOT + mb * (TILE * CW)) / 16, dV.hi};
+          umma_f8_warp<4, 32 * CW / 16, 32 * N / 16>(tmem + 2 * N + mb * N, v, {dP.lo + pb * C::PB / 16, dP.hi}, ID_PV, j > 0);
+          // (R = 8: zeros for a's columns)
+          umma_f8_warp<4, 32 * CW / 16, 32 * NC / 16>(tmem + 2 * N + mb * N + N - NC, v, {dPc.lo + pb * C::PCB / 16, dPc.hi}, ID_PC, 1);
+        }
         tc::umma_commit_warp(&vempty[vslot]);
         tc::umma_commit_warp(&pdone[pb]);
         if (++vslot == NSV) {
@@ -222,9 +232,10 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
     }
   } else {
     // ---------------- softmax: thread = key of the tile, RW rows. Row r of the unit is column
-    // (r / RW)·2RW + r % RW of the products (hi), and RW columns further (lo): a warpgroup's are together.
+    // (r / RW)·2RW + r % RW of the scores (hi), and RW columns further (lo): a warpgroup's are together. It is
+    // columns r and R + r of the outputs.
     const int wg = warp >> 2, wq = warp & 3, key_in = wq * 32 + lane, r0 = wg * RW, bar = 1 + wg;
-    const uint32_t tlane = tmem + ((uint32_t)(wq * 32) << 16) + wg * (2 * RW);
+    const uint32_t tlane = tmem + ((uint32_t)(wq * 32) << 16) + wg * (2 * RW), tout = tmem + ((uint32_t)(wq * 32) << 16) + 2 * N + r0;
     const int my_row = r0 + row_of<RW>(lane);
     const bool reducer = lane % (32 / RW) == 0;    // its lane of a row's reduction
     const Scratch ws = scratch(L, gridDim.x, R);
@@ -393,7 +404,7 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
             for (int c = 0; c < CB * (RW / 4); ++c) {   // 8 columns
               const int mb = c / (RW / 4), i0 = c % (RW / 4) * 8;
               uint32_t o[8];
-              const uint32_t where = tlane + 2 * N + mb * N + i0;
+              const uint32_t where = tout + mb * N + i0 / RW * R + i0 % RW;
               tm_ld8(where, o);
               tm_wait_ld8(o);
 #pragma unroll
@@ -404,32 +415,36 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
             tc::fence_before();
           }
         }
-        // weights, as two e4m3 values each. (The buffer's previous product, of tile - 2, was issued before QK of
+        // weights, as three e5m2 values each. (The buffer's previous product, of tile - 2, was issued before QK of
         // this tile and so is done.)
-        uint32_t hi[RW / 4], lo[RW / 4];
+        uint32_t pa[RW / 4], pb[RW / 4], pc[RW / 4];
 #pragma unroll
-        for (int i = 0; i < RW; i += 2) {
-          const float a = ex2(d[i]), z = ex2(d[i + 1]);
-          l[i] = fmaf(a, ivs, l[i]);
-          l[i + 1] = fmaf(z, ivs, l[i + 1]);
-          const __half2 wv = __floats2half2_rn(a, z);
-          const uint16_t h = half2_to_e4m3x2(wv);
-          const uint16_t q = half2_to_e4m3x2(__hmul2(__hsub2(wv, e4m3x2_to_half2(h)), __float2half2_rn(16.f)));
-          if (i % 4 == 0) {
-            hi[i / 4] = h;
-            lo[i / 4] = q;
-          } else {
-            hi[i / 4] |= (uint32_t)h << 16;
-            lo[i / 4] |= (uint32_t)q << 16;
+        for (int i = 0; i < RW; i += 4) {
+          uint32_t x[2][3];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float a = ex2(d[i + 2 * k]), z = ex2(d[i + 2 * k + 1]);
+            l[i + 2 * k] = fmaf(a, ivs, l[i + 2 * k]);
+            l[i + 2 * k + 1] = fmaf(z, ivs, l[i + 2 * k + 1]);
+            split_weights<4>(__floats2half2_rn(a, z), x[k][0], x[k][1], x[k][2]);
           }
+          pa[i / 4] = upper_bytes(x[0][0], x[1][0]);
+          pb[i / 4] = upper_bytes(x[0][1], x[1][1]);
+          pc[i / 4] = upper_bytes(x[0][2], x[1][2]);
         }
-        uint8_t* pr = sP + sb * C::PB;
-        constexpr int PW = N < 16 ? 16 : N;
-        if constexpr (RW == 8) {
-          *reinterpret_cast<uint4*>(pr + swz<PW>(key_in, wg)) = make_uint4(hi[0], hi[1], lo[0], lo[1]);
+        uint8_t *pr = sP + sb * C::PB, *prc = sPc + sb * C::PCB;
+        if constexpr (R == 8) {
+          *reinterpret_cast<uint4*>(pr + swz<N>(key_in, 0)) = make_uint4(pa[0], pa[1], pb[0], pb[1]);
+          *reinterpret_cast<uint4*>(prc + swz<NC>(key_in, 0)) = make_uint4(0, 0, pc[0], pc[1]);
+        } else if constexpr (RW == 8) {
+          const int half = wg % 2 * 8;
+          *reinterpret_cast<uint2*>(pr + swz<N>(key_in, wg / 2) + half) = make_uint2(pa[0], pa[1]);
+          *reinterpret_cast<uint2*>(pr + swz<N>(key_in, R / 16 + wg / 2) + half) = make_uint2(pb[0], pb[1]);
+          *reinterpret_cast<uint2*>(prc + swz<NC>(key_in, wg / 2) + half) = make_uint2(pc[0], pc[1]);
         } else {
-          *reinterpret_cast<uint4*>(pr + swz<PW>(key_in, 2 * wg)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          *reinterpret_cast<uint4*>(pr + swz<PW>(key_in, 2 * wg + 1)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          *reinterpret_cast<uint4*>(pr + swz<N>(key_in, wg)) = make_uint4(pa[0], pa[1], pa[2], pa[3]);
+          *reinterpret_cast<uint4*>(pr + swz<N>(key_in, R / 16 + wg)) = make_uint4(pb[0], pb[1], pb[2], pb[3]);
+          *reinterpret_cast<uint4*>(prc + swz<NC>(key_in, wg)) = make_uint4(pc[0], pc[1], pc[2], pc[3]);
         }
         if (!mine && wg == 0) {
           // a key that is not there: its value row is whatever lies in the slot, and 0·NaN is NaN
@@ -497,14 +512,14 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
 #pragma unroll
         for (int i0 = 0; i0 < RW; i0 += 8) {
           uint32_t oh[8], ol[8];
-          tm_ld8(tlane + 2 * N + mb * N + i0, oh);
-          tm_ld8(tlane + 2 * N + mb * N + RW + i0, ol);
+          tm_ld8(tout + mb * N + i0, oh);
+          tm_ld8(tout + mb * N + R + i0, ol);
           tm_wait_ld8(oh, ol);
           if (p.whole) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               const float g = __uint_as_float((uint32_t)gates[mb * RW + i0 + i] << 16);
-              const float v = fmaf(__uint_as_float(ol[i]), 0.0625f, __uint_as_float(oh[i])) * aux[r0 + i0 + i] * sigmoid_ex2(g);
+              const float v = fmaf(__uint_as_float(ol[i]), 0.25f, __uint_as_float(oh[i])) * aux[r0 + i0 + i] * sigmoid_ex2(g);
               if (row0 + i0 + i < rows_total && dim < HD) *at = __float2bfloat16_rn(v);
               at += HD;
               if (++h == nrep) {
@@ -515,7 +530,7 @@ tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
           } else if (dim < HD) {
             float* to = ws.o + ((int64_t)p.slot * R + r0 + i0) * HD + dim;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) to[i * HD] = fmaf(__uint_as_float(ol[i]), 0.0625f, __uint_as_float(oh[i]));
+            for (int i = 0; i < 8; ++i) to[i * HD] = fmaf(__uint_as_float(ol[i]), 0.25f, __uint_as_float(oh[i]));
           }
           __syncwarp();
         }

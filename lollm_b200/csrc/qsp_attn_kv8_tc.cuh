@@ -1,5 +1,5 @@
 // Shared by the tensor-core kernels of the 8-bit cache: bounded waits, operand descriptors and MMAs on
-// e4m3, TMEM reads, and the warps that load tiles and scales. Each including file has its own error flag.
+// 8-bit floats, TMEM reads, and the warps that load tiles and scales. Each including file has its own error flag.
 #pragma once
 
 #include <limits.h>
@@ -14,7 +14,7 @@ static __device__ int g_kv8_error = 0;
 
 constexpr int CODE_WAIT = 302;       // a bounded wait ran out
 constexpr float SLACK = 4.f;         // log2 units the running maximum may lag behind
-constexpr float BIAS = 4.f;          // weights are held times 2^BIAS: at most 2^(SLACK + BIAS) = 256 <= 448
+constexpr float BIAS = 11.f;         // weights are held times 2^BIAS: at most 2^(SLACK + BIAS) = 32768, under e5m2's 57344
 constexpr float NOTHING = -1e30f;    // maximum of a row that has seen nothing
 
 // A piece of work as the scales' warp hands it to the others, which run up to 4 tiles behind it (and the
@@ -42,14 +42,14 @@ __device__ __forceinline__ int swz(int row, int chunk) {   // byte offset of a 1
   constexpr int M = W / 16 - 1;
   return row * W + ((chunk ^ (row * W / 128 & M)) << 4);
 }
-// kind::f8f6f4, D fp32, A and B e4m3
-__host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N, bool mn_major) {
-  return (1u << 4) | (mn_major ? 3u << 15 : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+// kind::f8f6f4, D fp32, A e4m3, B e4m3 or e5m2
+__host__ __device__ constexpr uint32_t idesc_f8(int M, int N, bool mn_major, bool b_e5m2) {
+  return (1u << 4) | (b_e5m2 ? 1u << 10 : 0u) | (mn_major ? 3u << 15 : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 // `STEPS` MMAs of K = 32 into the same accumulator, the operands' addresses a_step and b_step (in
 // 16-byte units) apart; the first accumulates iff acc != 0. Issued by a converged warp.
 template <int STEPS, int A_STEP, int B_STEP>
-__device__ __forceinline__ void umma_e4m3_warp(uint32_t d, Sdesc a, Sdesc b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void umma_f8_warp(uint32_t d, Sdesc a, Sdesc b, uint32_t idesc, uint32_t acc) {
   static_assert(STEPS == 1 || STEPS == 2 || STEPS == 4, "");
   if constexpr (STEPS == 4) {
     asm volatile(
@@ -77,7 +77,7 @@ __device__ __forceinline__ void umma_e4m3_warp(uint32_t d, Sdesc a, Sdesc b, uin
         "r"(a.lo), "r"(a.hi), "r"(b.lo), "r"(b.hi), "r"(idesc), "r"(acc)
         : "memory");
     if constexpr (STEPS == 2)
-      umma_e4m3_warp<1, A_STEP, B_STEP>(d, {a.lo + A_STEP, a.hi}, {b.lo + B_STEP, b.hi}, idesc, 1);
+      umma_f8_warp<1, A_STEP, B_STEP>(d, {a.lo + A_STEP, a.hi}, {b.lo + B_STEP, b.hi}, idesc, 1);
   }
 }
 
@@ -140,6 +140,29 @@ __device__ __forceinline__ uint16_t half2_to_e4m3x2(__half2 v) {
   asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(*reinterpret_cast<uint32_t*>(&v)));
   return r;
 }
+// ---------------------------------------------------------------- softmax weights as sums of e5m2 values
+// A weight w >= 0, rounded to fp16, is cut into three e5m2 values: the upper byte of an fp16 value is the e5m2 value below it,
+// so a = upper byte(w), b = upper byte(S·(w − a)), c = S·(w − a) − b rounded to one, and w = a + (b + c) / S. Every part keeps
+// 3 bits or more of what is left, so w is off by at most 2^-9 of its power of two (half a bf16 step is 2^-8), or by
+// 2^-17 / S where that is more: 2^-28 / S of a row's largest, which is held as 2^BIAS at least. The relative precision of
+// bf16 thus reaches down to 2^-20 / S of the largest. (Two e4m3 values reached 2^-10, and were 0 under 2^-18: one key with
+// most of the weight and 32k weak ones lost what the weak ones add up to, 6 to 60 per cent of the output.)
+// The subtractions are exact; no conversion is needed, which an SM does at a quarter of the rate or less.
+template <int S>
+__device__ __forceinline__ void split_weights(__half2 w, uint32_t& a, uint32_t& b, uint32_t& c) {   // pairs; parts are upper bytes
+  auto upper = [](uint32_t x) {
+    x &= 0xff00ff00u;
+    return *reinterpret_cast<__half2*>(&x);
+  };
+  auto bits = [](__half2 x) { return *reinterpret_cast<uint32_t*>(&x); };
+  a = bits(w);
+  __half2 r = __hsub2(w, upper(a));
+  if constexpr (S != 1) r = __hmul2(r, __float2half2_rn((float)S));
+  b = bits(r);
+  c = bits(__hsub2(r, upper(b))) + 0x00800080u;   // half of the upper byte's last place: no carry out of a value
+}
+__device__ __forceinline__ uint32_t upper_bytes(uint32_t x, uint32_t y) { return __byte_perm(x, y, 0x7531); }   // of two pairs
+
 __device__ __forceinline__ void bar_sync(int id) { asm volatile("barrier.cta.sync %0, 128;" ::"r"(id) : "memory"); }
 __device__ __forceinline__ bool bar_any(int id, bool p) {
   uint32_t r;
