@@ -55,6 +55,9 @@ class Qwen3_5Cache:
         self.kv8 = self.kv_dtype == F8
         if not self.kv8 and self.kv_dtype != dtype:
             raise RuntimeError(f"kv_dtype must be {dtype} (the model's) or {F8}, not {kv_dtype}")
+        if self.kv8 and (hd not in (32, 64, 128, 256) or cfg.rotary_dim % (hd // 16) != 0):
+            raise RuntimeError(f"an 8-bit cache takes head sizes 32, 64, 128 and 256 with a multiple of head_dim / 16 rotated "
+                               f"dims, not {hd} with {cfg.rotary_dim}")
         pages = (n_attn, self.num_pages, nkv, page_size, hd)
         self.k_scales = self.v_scales = None
         if self.kv8:
