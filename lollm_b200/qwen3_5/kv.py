@@ -111,10 +111,13 @@ class Qwen3_5Cache:
     def append_kv(self, layer: int, k: torch.Tensor, v: torch.Tensor):
         """Write post-RoPE k, v (B, n_kv, t, hd) at each sequence's next positions and return
         the full (K, V) as read_kv does (kv.py:26-33). Compatibility path, not the hot path:
-        the forward appends inside `qsp_attn_prep`."""
+        the forward appends inside `qsp_attn_prep`. An 8-bit cache stores the tokens one by one, as t
+        calls of `qsp_attn_kv8_prep` with one token each would."""
         s = self.attn_slot[layer]
         B, _, t, _ = k.shape
         lens = self.seq_lens.long()
+        if int(lens.max()) + t > self.capacity:   # (on a GPU the page lookup past the table would end the context)
+            raise RuntimeError(f"append_kv: {t} tokens behind {int(lens.max())} pass the capacity ({self.capacity} positions per sequence)")
         if self.kv8:
             for j in range(t):
                 kj, vj = k[:, :, j].float(), v[:, :, j].float()

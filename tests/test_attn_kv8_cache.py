@@ -20,3 +20,17 @@ def test_cache_refuses_heads_that_no_kernel_takes(kw):
     with pytest.raises(RuntimeError, match="8-bit"):
         _cache(raw, kv_dtype=kv8.F8)
     _cache(raw)
+
+
+@pytest.mark.parametrize("kv", [None, kv8.F8])
+def test_append_kv_refuses_what_has_no_page(kv):
+    """A call that would pass the capacity (48) raises before anything is stored."""
+    c = _cache(kv_dtype=kv, scale_block=8)
+    layer = c.cfg.attn_layers[0]
+    x = torch.ones(2, c.cfg.num_key_value_heads, 20, c.cfg.head_dim)
+    c.append_kv(layer, x, x)
+    c.append_kv(layer, x, x)
+    before = c.k_pages.view(torch.uint8).clone()
+    with pytest.raises(RuntimeError, match="capacity"):
+        c.append_kv(layer, 2 * x, x)
+    assert torch.equal(c.k_pages.view(torch.uint8), before) and c.seen_tokens == 40
