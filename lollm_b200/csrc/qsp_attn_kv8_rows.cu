@@ -219,7 +219,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUt
   if (warp == W_K || warp == W_V) {
     const bool is_v = warp == W_V;
     load_tiles<HD, CW>(L, is_v ? &tmV : &tmK, is_v ? sV : sK, is_v ? vfull : kfull, is_v ? vempty : kempty, is_v ? NSV : NSK, box_rows,
-                       n_rg == 1, piece_at, abort);
+                       read_once(L, n_rg), piece_at, abort);
   } else if (warp == W_E) {
     int slot = 0;
     const Piece p = walk_and_scales(L, n_rg, RR, NSK, w, desc, dfull, kfull, kempty, abort, [&](const Scales& x) {

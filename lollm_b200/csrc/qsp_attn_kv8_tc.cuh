@@ -187,7 +187,14 @@ __device__ __forceinline__ void load_box(void* dst, const CUtensorMap* map, uint
       : "memory");
 }
 // K or V tiles of the CTA's pieces into a ring of `slots`, by TMA: boxes of box_rows keys x CW bytes; lane i looks
-// up the page of the tile's i-th box_rows keys, one tile ahead. once: no other CTA reads the tile.
+// up the page of the tile's i-th box_rows keys, one tile ahead. once: see read_once.
+// Is a tile read by one CTA only? Not where a unit's keys are another row group's too, nor where the pool has fewer pages
+// than the table has entries, so that sequences share some (a common prefix). Evict-first keeps what is read once from
+// driving queries, page tables and partials out of L2 (64 x 4 tokens over 2k keys 34.7 us, 37.8 without; over 1k to 32k 174 and
+// 182), but drives shared pages out too (64 x 4 over the same 32k keys 264 us, 248 without; the same 120k 1234 and 1083).
+__device__ __forceinline__ bool read_once(const qsp_attn_kv8_layer& L, int n_rg) {
+  return n_rg == 1 && L.num_pages >= (int64_t)L.batch * L.max_pages;
+}
 template <int HD, int CW, typename PieceAt>
 __device__ __forceinline__ void load_tiles(const qsp_attn_kv8_layer& L, const CUtensorMap* map, uint8_t* ring, uint64_t* full,
                                            uint64_t* empty, int slots, int box_rows, bool once, const PieceAt& piece_at,
