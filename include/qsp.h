@@ -290,7 +290,9 @@ typedef struct qsp_attn_kv8_layer {
  * earlier tokens; when it grows, the earlier codes are rescaled (exact, but for e4m3 subnormals).
  * k is computed in 64 bits and rounded to fp32 before it is quantised, so the stored codes do not
  * depend on the order of a sum. A token whose key or value has a non-finite element in a kv head
- * is stored there as a NaN key and a zero value: every query that sees it gives NaN, no other.
+ * is stored there as a NaN key, which counts nothing in its scale: every query that sees it gives
+ * NaN, no other. Its value is stored as it is, or as zeros that count nothing if it is the value that is
+ * not finite.
  * Repeating a call without moving seq_lens stores the same again. */
 int qsp_attn_kv8_prep(const qsp_attn_kv8_layer* layer, void* stream);
 
