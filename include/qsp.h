@@ -253,7 +253,8 @@ int qsp_attn_verify_static(const qsp_attn_layer* layer, void* stream);
  * positions outside the pages or the RoPE table flagged in *bad_index and left out.
  *
  * Limits: head_dim 32, 64, 128 or 256; rotary_dim a multiple of head_dim / 16; scale_block a power of
- * two up to 64 that divides page_size; q_buf 16-byte aligned; fewer than 2^30 positions a sequence. Only
+ * two up to 64 that divides page_size (bf16: tensor cores where page_size is a multiple of 8, else
+ * CUDA cores); q_buf 16-byte aligned; fewer than 2^30 positions a sequence. Only
  * qsp_attn_kv8_prep writes the pages (a value code must not be NaN in a position that a query can
  * see). A page may be read by many sequences; the pages that a call appends to belong to one each.
  */

@@ -149,7 +149,8 @@ class Qwen3_5Model:
     # ------------------------------------------------------------------ helpers
     def new_cache(self, batch: int, max_len: int | None = None, **kw) -> Qwen3_5Cache:
         """A cache of `max_len` positions per sequence. kv_dtype=torch.float8_e4m3fn keeps keys and
-        values in 8 bits, with one scale for each `scale_block` tokens (16) and kv head."""
+        values in 8 bits, with one scale for each `scale_block` tokens (16) and kv head; a bf16 model then
+        attends on the tensor cores if page_size is a multiple of 8, else on the CUDA cores."""
         max_len = max_len or self.max_positions
         if max_len > self.max_positions:
             raise RuntimeError(f"max_len {max_len} exceeds the RoPE table ({self.max_positions})")

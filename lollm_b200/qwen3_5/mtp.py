@@ -114,7 +114,9 @@ class MTP:
 
 class SpecDecoder:
     """Batched k-deep speculative decoding over independent sequences on one GPU. Further keywords
-    are the cache's (kv_dtype=torch.float8_e4m3fn keeps keys and values in 8 bits)."""
+    are the cache's (kv_dtype=torch.float8_e4m3fn keeps keys and values in 8 bits; a rejected draft can then
+    leave its block's scale larger than needed, which later tokens of the block are rounded with, unless
+    scale_block=1)."""
 
     def __init__(self, model: Qwen3_5Model, mtp: MTP, batch: int, k: int, max_len: int, *,
                  temperature: float = 0.0, top_k: int = 0, top_p: float = 1.0,
@@ -234,9 +236,10 @@ def generate_mtp(model: Qwen3_5Model, mtp: MTP, ids, decode, stop_ids, device=No
                  repetition_penalty=1.1, k: int = 1, seed: int = 0, **cache_kw):
     """Drop-in for the reference generator (mtp.py:92-162), same defaults: yields text pieces
     of one sequence. Greedy (temperature <= 0) output equals `generate()` with the same
-    repetition penalty. temperature > 0 uses the lossless p/q sampler over the filtered
+    repetition penalty; over an 8-bit cache only with scale_block=1, since a rejected draft can leave the
+    scale of its block of tokens larger than `generate()` would have it. temperature > 0 uses the lossless p/q sampler over the filtered
     target and draft distributions (penalty → temperature → top-k → top-p, as sample_next),
-    with uniforms from a seeded device generator. Further keywords are the cache's (kv_dtype)."""
+    with uniforms from a seeded device generator. Further keywords are the cache's (kv_dtype, scale_block)."""
     eos = set(stop_ids)
     prompt = torch.tensor([list(ids)], dtype=torch.int64, device=model.device)
     dec = SpecDecoder(model, mtp, 1, k, prompt.shape[1] + max_new_tokens + k + 2,
