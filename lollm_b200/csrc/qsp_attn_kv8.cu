@@ -593,8 +593,8 @@ static int launch_merge_hd(const qsp_attn_kv8_layer& L, int G, int R, cudaStream
   if (units * MERGE_WARPS <= G && units * std::min(R, rows) <= 2 * tc::sm_count())
     return launch_pdl("qsp_attn_kv8_verify(merge)", merge_kernel<T, HD, true>, dim3((unsigned)units, std::min(R, rows)),
                       dim3(32 * MERGE_WARPS), 0, st, L, G, R, 1, vec);
-  // 128 rows of many units: fewer CTAs, most of which find nothing to do (8 x 127 tokens over 1-2k keys, all whole: 47.6 us
-  // with 1, 45.5 with 4); of few units: one row a warp (1 x 128 over 16k: 55.5 and 64.7)
+  // 128 rows of many units: fewer CTAs, most of which find nothing to do (8 x 127 tokens over 1-2k keys, all whole: 54.5 us
+  // with 1, 52.5 with 4); of few units: one row a warp (1 x 128 over 16k: 60 and 70)
   const int each = R > 64 && 2 * units >= G ? 4 : 1;
   return launch_pdl("qsp_attn_kv8_verify(merge)", merge_kernel<T, HD, false>,
                     dim3(G, (std::min(R, rows) + each * MERGE_WARPS - 1) / (each * MERGE_WARPS)), dim3(32 * MERGE_WARPS), 0, st, L, G, R, each, vec);
@@ -612,7 +612,7 @@ static int launch_merge_t(const qsp_attn_kv8_layer& L, int G, int R, cudaStream_
 
 int launch_merge(const qsp_attn_kv8_layer& L, int G, int R, int keys, cudaStream_t st) {
   // none is divided where units have one tile, or where share() cannot but leave all whole: as many CTAs as units, none
-  // of more than merge_cost (16 x 17 tokens over 700 keys: 29.2 us with the launch, 26.9 without)
+  // of more than merge_cost (16 x 17 tokens over 700 keys: 30.6 us with the launch, 26.8 without)
   const int64_t tiles = ((int64_t)L.max_pages * L.page_size + keys - 1) / keys;
   const int64_t units = (int64_t)L.batch * L.n_kv_heads * ((L.n_heads / L.n_kv_heads * L.tokens + R - 1) / R);
   if (tiles <= 1 || (units <= G && UNIT_COST + tiles <= merge_cost(R))) return QSP_OK;

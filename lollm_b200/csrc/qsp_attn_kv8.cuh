@@ -121,9 +121,9 @@ __device__ __forceinline__ int exp_of(float scale) { return ((__float_as_int(sca
 // describes it in meta[c] for the merge kernel.
 // Dividing has a price: a second piece for most CTAs and the merge. Where no CTA would have more than
 // merge_cost tiles less to do for it, each unit goes whole to one CTA: 64 sequences of 2048 to 2560 keys,
-// 2 kv heads: 128 CTAs with at most 20 tiles each instead of 148 with 15.6 on average (38.8 us divided, 35.4 whole).
+// 2 kv heads: 128 CTAs with at most 20 tiles each instead of 148 with 15.6 on average (37.1 us divided, 34.9 whole).
 // Units of 128 rows leave partials of 128 KB (hd 256), so dividing costs more: 2 x 512 tokens over 8k keys took
-// 144 us with a bound of 10 tiles, which divides them, 124 us with 12.
+// 173 us with a bound of 10 tiles, which divides them, 152 us with 12.
 constexpr int UNIT_COST = 3;
 __host__ __device__ __forceinline__ int merge_cost(int R) { return R > 64 ? 12 : 6; }
 

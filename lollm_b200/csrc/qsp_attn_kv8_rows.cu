@@ -24,8 +24,10 @@
 // A tile takes 1024 + 1350 cycles of the tensor cores at hd 256 (two parts of Q, three of P) and 2100 of the softmax: 64
 // exponentials a thread at 16 an SM and cycle are half of that. They overlap but for the start of each; about 3300
 // cycles were measured, and 2700 with weights of two parts, whose small ones were lost (8 sequences x 127 tokens over 1k
-// to 2k keys, 2 kv heads of 256, 48 and 53 us; 2 x 512 over 8k 119 and 145 us). At head sizes up to 128, where
-// TMEM has room for the weights of two tiles, the third part costs nothing (8 x 127 of size 64: 27 us).
+// to 2k keys, 2 kv heads of 256, 48 and 53 us; 2 x 512 over 8k 119 and 141 to 154 us). At head sizes up to 128, where
+// TMEM has room for the weights of two tiles, the third part costs nothing (8 x 127 of size 64: 28 us). Against 64
+// rows a unit (tc_kernel in groups): 8 x 127 72 -> 52 us, 64 x 16 over 2k 87 -> 58, 4 x 2048 from an empty cache 451 -> 315,
+// 27 x 64 tokens of 4 and 2 heads over 4k to 9k 88 -> 77.
 #include "qsp_attn_kv8_tc.cuh"
 
 #include <algorithm>

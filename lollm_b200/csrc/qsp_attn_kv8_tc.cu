@@ -30,9 +30,9 @@
 //
 // Bound by HBM where sequences are long: a tile of 128 keys at hd 256 is 64 KB, 2800 cycles of an SM's share of
 // 6.5 TB/s; its products take 780 cycles of the tensor cores at R = 32, its softmax a chain of some 1900 cycles.
-// Measured, 2 kv heads of 256, 64 sequences of 1k to 32k keys: 4 tokens 174 us in a graph of one
-// input (178 with weights of two parts); of 2048 to 2560 keys: 4 tokens 35 us (34), 8 tokens (R = 64) 46 us (43). One token
-// over 33 keys: 6.7 us, a chain of length, plan, page, scales and K, product, softmax, product, gate.
+// Measured, 2 kv heads of 256, 64 sequences of 1k to 32k keys, 4 tokens: 174 us in a graph on one input, 210 (5.3 TB/s)
+// on inputs that change (197 with weights of two parts); of 2048 to 2560 keys: 4 tokens 35 us in a graph, 38 on inputs that
+// change (34, 36), 8 tokens (R = 64) 46 us (43). One token over 33 keys: 6.8 us, a chain of length, plan, page, scales and K, product, softmax, product, gate.
 #include "qsp_attn_kv8_tc.cuh"
 
 #include <algorithm>
@@ -603,7 +603,7 @@ int launch_tc(const qsp_attn_kv8_layer& L, cudaStream_t st) {
     return set_error(QSP_ERR_CUDA, "qsp_attn_kv8_verify: no tensor map for the pages");
   const int R = tc_rows(L.n_heads / L.n_kv_heads * L.tokens);
   // rows_kernel takes the scales of 8 keys at a time; with smaller blocks: groups of 64 rows (8 x 127 tokens over 1-2k keys
-  // 84 us, where it takes 45)
+  // 72 us, where it takes 52)
   if (R == 128 && L.scale_block >= GROUP) return launch_rows(L, mk, mv, box_rows, st);
   switch (L.head_dim) {
     case 32: return launch_tc_hd<32>(L, R, mk, mv, box_rows, st);
