@@ -301,8 +301,8 @@ int qsp_attn_kv8_prep(const qsp_attn_kv8_layer* layer, void* stream);
  * pages, times σ(gate) (attention.py:43-51, 84-91; blocks.py:229-235), rounded to dtype once. The
  * keys of all sequences are divided evenly over the SMs and the parts merged by a second launch,
  * in a fixed order (repeated calls give the same bits). A query that sees no key gives zero.
- * bf16: a softmax weight (times its value's scale) is held to 2^-9, as good as in bf16, down to 2^-20 of the
- * largest of its row among the keys that one SM takes, and rounds to zero below 2^-28 of it (2^-22 and
+ * bf16: a softmax weight (times its value's scale) is held to 2^-8 or better, as bf16 would, down to 2^-20 of
+ * the largest of its row among the keys that one SM takes, and rounds to zero below 2^-28 of it (2^-22 and
  * 2^-30 up to 64 query rows a kv head). fp32: in fp32.
  * `workspace` must not be shared by two calls that overlap in time. */
 int qsp_attn_kv8_verify(const qsp_attn_kv8_layer* layer, void* stream);
